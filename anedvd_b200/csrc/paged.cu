@@ -1,0 +1,641 @@
+// paged.cu -- serving from a paged KV cache: the checks behind the cuq_* entry
+// points, rotary positions with the append, and the eviction.  The attention
+// over the cache is in paged_attn.cu, the gathered attention weight in
+// paged_mass.cu.
+#include <cmath>
+#include <new>
+
+#include "paged.cuh"
+
+namespace cuq {
+int sm_count_current();
+
+constexpr int ROPE_MAX_PAIRS = 64;
+
+// Angle per position of each pair, as a fraction of a turn in units of 2^-64.
+// pos * turns then wraps by itself: the product modulo 2^64 is the angle's
+// fractional turn, off by at most |pos| 2^-65 turns (2^-34 at pos = 2^31).
+struct RopeTable {
+    uint64_t turns[ROPE_MAX_PAIRS];
+    float mul;  // factor on cosine and sine
+    uint32_t rot;
+    int adjacent;
+};
+}  // namespace cuq
+
+struct cuq_rope_plan {
+    cuq::RopeTable t;
+};
+
+namespace cuq {
+namespace {
+
+// ------------------------------------------------- rotary + append ----
+//
+// Bound by HBM for prompts (every value is read and written once) and by
+// latency for a few tokens.  A CTA takes T tokens: its threads first work out
+// the T * rot/2 cosines and sines, one each, into shared memory, then walk the
+// (token, head, unit) triples, a unit being the 16 values that hold 8 whole
+// pairs: two 16-byte vectors at j and j + rot/2, or 16 values in a row.
+struct RopeArgs {
+    PagedArgs a;
+    const int32_t *positions;
+    void *q_out;
+    size_t q_out_stride;
+    const void *q, *k, *v;
+    size_t q_stride, kv_stride;
+    uint32_t heads;
+};
+
+template <typename T>
+__device__ __forceinline__ void store_as(int type, void *base, size_t at, const float (&v)[8]) {
+    if (type == CUQ_F32)
+        store8(reinterpret_cast<float *>(base) + at, v);
+    else if (type == CUQ_F16)
+        store8(reinterpret_cast<__half *>(base) + at, v);
+    else
+        store8(reinterpret_cast<__nv_bfloat16 *>(base) + at, v);
+}
+
+constexpr int ROPE_THREADS = 256;
+
+template <typename TI, int HD, int T>
+__global__ void __launch_bounds__(ROPE_THREADS) rope_append_kernel(RopeArgs p, RopeTable tab, int out_type,
+                                                                    int cache_type) {
+    __shared__ float2 cs[T][ROPE_MAX_PAIRS];
+    __shared__ int s_pos[T], s_slot[T], s_page[T];
+    __shared__ int s_seq[T];
+    const uint32_t tok0 = blockIdx.x * T;
+    // the sequence of a token: how many sequences end at or before it
+    for (int i = 0; i < T; i++) {
+        const int tok = (int)(tok0 + i);
+        int n = 0;
+        for (uint32_t base = 0; base < p.a.n_seqs; base += ROPE_THREADS) {
+            const uint32_t b = base + threadIdx.x;
+            n += __syncthreads_count(b < p.a.n_seqs && __ldg(p.a.q_start + b + 1) <= tok);
+        }
+        if (threadIdx.x == 0) {
+            int seq = -1, slot = -1, page = -1;
+            if (n < (int)p.a.n_seqs && tok < (int)p.a.n_tok) {
+                uint32_t first;
+                const uint32_t nq = p.a.tokens(n, first);
+                if ((uint32_t)tok >= first && (uint32_t)tok < first + nq) {
+                    seq = n;
+                    const int len = (int)p.a.len(n);
+                    slot = len - (int)nq + (tok - (int)first);
+                    if (slot >= 0) page = p.a.page(n, (uint32_t)slot >> p.a.page_shift);
+                }
+            }
+            s_seq[i] = seq;
+            s_slot[i] = slot;
+            s_page[i] = page;
+            s_pos[i] = seq < 0 ? 0 : p.positions ? __ldg(p.positions + tok) : slot;
+        }
+    }
+    __syncthreads();
+    const uint32_t half = tab.rot / 2;
+    for (uint32_t i = threadIdx.x; i < T * half; i += ROPE_THREADS) {
+        const uint32_t t = i / half, j = i % half;
+        const int64_t turn = (int64_t)((uint64_t)(int64_t)s_pos[t] * tab.turns[j]);
+        // the top 32 bits are the turn in [-1/2, 1/2): 2^-32 turns is far below
+        // the fp32 step of the cosine and sine
+        const float x = (float)(int32_t)(turn >> 32) * 0x1p-31f;  // in units of pi
+        float si, co;
+        sincospif(x, &si, &co);
+        cs[t][j] = make_float2(co * tab.mul, si * tab.mul);
+    }
+    __syncthreads();
+    constexpr uint32_t UNITS = HD / 16;
+    const uint32_t rows = p.heads + 2 * p.a.kv_heads, rot_units = tab.rot / 16;
+    for (uint32_t i = threadIdx.x; i < T * rows * UNITS; i += ROPE_THREADS) {
+        const uint32_t t = i / (rows * UNITS), r = (i / UNITS) % rows, u = i % UNITS;
+        const uint32_t tok = tok0 + t;
+        if (s_seq[t] < 0) continue;
+        const bool is_q = r < p.heads, is_k = !is_q && r < p.heads + p.a.kv_heads;
+        if (!is_q && s_page[t] < 0) continue;
+        const bool turn = u < rot_units && (is_q || is_k);
+        const uint32_t h = is_q ? r : is_k ? r - p.heads : r - p.heads - p.a.kv_heads;
+        const TI *src = reinterpret_cast<const TI *>(is_q ? p.q : is_k ? p.k : p.v) +
+                        (size_t)tok * (is_q ? p.q_stride : p.kv_stride) + (size_t)h * HD;
+        const bool apart = turn && !tab.adjacent;
+        const uint32_t e0 = apart ? 8 * u : 16 * u, e1 = apart ? half + 8 * u : 16 * u + 8;
+        float a[8], b[8];
+        load8(src + e0, a);
+        load8(src + e1, b);
+        if (apart) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float2 c = cs[t][8 * u + j];
+                const float x = a[j], y = b[j];
+                a[j] = x * c.x - y * c.y;
+                b[j] = x * c.y + y * c.x;
+            }
+        } else if (turn) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float2 c = cs[t][8 * u + j], d = cs[t][8 * u + 4 + j];
+                float x = a[2 * j], y = a[2 * j + 1];
+                a[2 * j] = x * c.x - y * c.y;
+                a[2 * j + 1] = x * c.y + y * c.x;
+                x = b[2 * j], y = b[2 * j + 1];
+                b[2 * j] = x * d.x - y * d.y;
+                b[2 * j + 1] = x * d.y + y * d.x;
+            }
+        }
+        if (is_q) {
+            const size_t at = (size_t)tok * p.q_out_stride + (size_t)h * HD;
+            store_as<TI>(out_type, p.q_out, at + e0, a);
+            store_as<TI>(out_type, p.q_out, at + e1, b);
+        } else {
+            const size_t at = p.a.row<HD>(s_page[t], h, (uint32_t)s_slot[t]);
+            void *pool = is_k ? p.a.k : p.a.v;
+            store_as<TI>(cache_type, pool, at + e0, a);
+            store_as<TI>(cache_type, pool, at + e1, b);
+        }
+    }
+}
+
+template <typename TI>
+int launch_rope_append(const RopeArgs &p, const RopeTable &t, int out_type, int cache_type, uint32_t hd,
+                       cudaStream_t s) {
+    const bool many = p.a.n_tok >= 1024;
+    const uint32_t grid = many ? (p.a.n_tok + 3) / 4 : p.a.n_tok;
+    if (hd == 64 && many)
+        rope_append_kernel<TI, 64, 4><<<grid, ROPE_THREADS, 0, s>>>(p, t, out_type, cache_type);
+    else if (hd == 64)
+        rope_append_kernel<TI, 64, 1><<<grid, ROPE_THREADS, 0, s>>>(p, t, out_type, cache_type);
+    else if (many)
+        rope_append_kernel<TI, 128, 4><<<grid, ROPE_THREADS, 0, s>>>(p, t, out_type, cache_type);
+    else
+        rope_append_kernel<TI, 128, 1><<<grid, ROPE_THREADS, 0, s>>>(p, t, out_type, cache_type);
+    CUQ_CUDA_TRY(cudaGetLastError());
+    return CUQ_OK;
+}
+
+// ------------------------------------------------------- eviction ----
+//
+// Selection: one CTA per (sequence, KV head).  Masses become 32-bit keys in
+// their order (NaN lowest); four 8-bit histogram passes find the key of the
+// last slot kept and how many of its equals are kept; one ordered pass then
+// writes the kept slots by prefix sums.  The order of the histogram's atomics
+// does not matter: they count whole numbers.
+constexpr int SEL_THREADS = 1024;
+
+__device__ __forceinline__ uint32_t mass_key(float m) {
+    if (m != m) return 0u;
+    const uint32_t u = __float_as_uint(m + 0.f);  // -0 becomes +0
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+
+struct EvictArgs {
+    PagedArgs a;
+    const float *mass;
+    size_t mass_stride;
+    uint32_t keep, sink, recent;
+    int32_t *kept, *new_len;
+    float *mass_out;
+    size_t mass_out_stride;
+};
+
+__global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(EvictArgs p) {
+    __shared__ uint32_t hist[256];
+    __shared__ uint32_t s_prefix, s_need, warp_sum[33];
+    const uint32_t b = blockIdx.x / p.a.kv_heads, h = blockIdx.x % p.a.kv_heads;
+    const uint32_t n = p.a.len(b), kept_n = min(n, p.keep);
+    const float *mass = p.mass + ((size_t)b * p.a.kv_heads + h) * p.mass_stride;
+    int32_t *kept = p.kept + ((size_t)b * p.a.kv_heads + h) * p.keep;
+    float *mass_out = p.mass_out ? p.mass_out + ((size_t)b * p.a.kv_heads + h) * p.mass_out_stride : nullptr;
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (h == 0 && tid == 0) p.new_len[b] = (int32_t)kept_n;
+    if (n <= p.keep) {
+        for (uint32_t i = tid; i < p.keep; i += SEL_THREADS) kept[i] = i < n ? (int32_t)i : -1;
+        if (mass_out && mass_out != mass)
+            for (uint32_t i = tid; i < n; i += SEL_THREADS) mass_out[i] = mass[i];
+        return;
+    }
+    // the slots in between, of which `need` are kept
+    const uint32_t lo = p.sink, hi = n - p.recent;
+    if (tid == 0) {
+        s_prefix = 0;
+        s_need = p.keep - p.sink - p.recent;
+    }
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        if (tid < 256) hist[tid] = 0;
+        __syncthreads();
+        const uint32_t prefix = s_prefix, need = s_need;
+        for (uint32_t i = lo + tid; i < hi; i += SEL_THREADS) {
+            const uint32_t key = mass_key(mass[i]);
+            if (shift == 24 || (key >> (shift + 8)) == prefix) atomicAdd(&hist[(key >> shift) & 255u], 1u);
+        }
+        __syncthreads();
+        if (tid == 0) {  // the bin, from the top, in which the need-th key lies
+            uint32_t above = 0;
+            int bin = 255;
+            for (; bin > 0 && above + hist[bin] < need; bin--) above += hist[bin];
+            s_prefix = (prefix << 8) | (uint32_t)bin;
+            s_need = need - above;
+        }
+        __syncthreads();
+    }
+    const uint32_t edge = s_prefix, equals = s_need;  // keep keys above edge, and the first `equals` equal to it
+    // ordered pass: tiles of SEL_THREADS slots, running counts of kept and of equals
+    uint32_t out_base = 0, eq_base = 0;
+    for (uint32_t t0 = 0; t0 < n; t0 += SEL_THREADS) {
+        const uint32_t i = t0 + tid;
+        const float m = i < n ? mass[i] : 0.f;
+        const bool forced = i < n && (i < lo || i >= hi);
+        const uint32_t key = (i < n && !forced) ? mass_key(m) : 0u;
+        const bool above = i < n && !forced && key > edge, equal = i < n && !forced && key == edge;
+        // exclusive rank of this slot among the tile's equals, then among its kept
+        const uint32_t be = __ballot_sync(~0u, equal);
+        if (lane == 0) warp_sum[warp] = __popc(be);
+        __syncthreads();
+        uint32_t eq_before = 0, eq_total = 0;
+        for (int w = 0; w < SEL_THREADS / 32; w++) {
+            if (w < (int)warp) eq_before += warp_sum[w];
+            eq_total += warp_sum[w];
+        }
+        const uint32_t rank = eq_base + eq_before + __popc(be & ((1u << lane) - 1u));
+        const bool take = forced || above || (equal && rank < equals);
+        const uint32_t bt = __ballot_sync(~0u, take);
+        __syncthreads();
+        if (lane == 0) warp_sum[warp] = __popc(bt);
+        __syncthreads();
+        uint32_t before = 0, total = 0;
+        for (int w = 0; w < SEL_THREADS / 32; w++) {
+            if (w < (int)warp) before += warp_sum[w];
+            total += warp_sum[w];
+        }
+        const uint32_t at = out_base + before + __popc(bt & ((1u << lane) - 1u));
+        // in place: at <= i, so the slots this tile writes have been read
+        if (take && at < p.keep) {
+            kept[at] = (int32_t)i;
+            if (mass_out) mass_out[at] = m;
+        }
+        out_base += total;
+        eq_base += eq_total;
+        __syncthreads();
+    }
+    if (mass_out)
+        for (uint32_t i = kept_n + tid; i < n; i += SEL_THREADS) mass_out[i] = 0.f;
+}
+
+// Compaction, in place: a CTA owns one slice of SLICE bytes of every row of one
+// (sequence, KV head, pool), so no other CTA reads or writes what it does.  New
+// slot j takes old slot kept[j] >= j, in order: a chunk of rows is read whole
+// before it is written, and no later chunk reads what an earlier one wrote.
+constexpr int MOVE_THREADS = 256;
+constexpr int MOVE_VECS = 8;  // 16-byte vectors per thread in one chunk
+
+template <int HD, int SLICE>
+__global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(EvictArgs p) {
+    constexpr uint32_t VPR = SLICE / 16;                               // vectors per row
+    constexpr uint32_t ROWS = MOVE_THREADS * MOVE_VECS / VPR;          // rows per chunk
+    constexpr uint32_t SLICES = HD * 2 / SLICE;
+    uint32_t x = blockIdx.x;
+    const uint32_t slice = x % SLICES;
+    x /= SLICES;
+    const bool is_v = x & 1;
+    x >>= 1;
+    const uint32_t h = x % p.a.kv_heads, b = x / p.a.kv_heads;
+    const uint32_t n = p.a.len(b);
+    if (n <= p.keep) return;  // every slot stays where it is
+    const int32_t *kept = p.kept + ((size_t)b * p.a.kv_heads + h) * p.keep;
+    uint8_t *pool = reinterpret_cast<uint8_t *>(is_v ? p.a.v : p.a.k);
+    const uint32_t v = threadIdx.x % VPR, r0 = threadIdx.x / VPR;
+    for (uint32_t c = 0; c < p.keep; c += ROWS) {
+        uint4 val[MOVE_VECS];
+        bool ok[MOVE_VECS];
+#pragma unroll
+        for (int i = 0; i < MOVE_VECS; i++) {
+            const uint32_t j = c + r0 + i * (MOVE_THREADS / VPR);
+            ok[i] = false;
+            if (j < p.keep) {
+                const uint32_t src = (uint32_t)kept[j];
+                if (src != j && src < n) {
+                    const int pg = p.a.page(b, src >> p.a.page_shift);
+                    ok[i] = pg >= 0;
+                    if (ok[i])
+                        val[i] = *reinterpret_cast<const uint4 *>(pool + p.a.row<HD>(pg, h, src) * 2 + slice * SLICE +
+                                                                  v * 16);
+                }
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < MOVE_VECS; i++) {
+            const uint32_t j = c + r0 + i * (MOVE_THREADS / VPR);
+            if (!ok[i]) continue;
+            const int pg = p.a.page(b, j >> p.a.page_shift);
+            if (pg >= 0)
+                *reinterpret_cast<uint4 *>(pool + p.a.row<HD>(pg, h, j) * 2 + slice * SLICE + v * 16) = val[i];
+        }
+        __syncthreads();
+    }
+}
+
+// ----------------------------------------------------- argument checks ----
+
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+bool aligned4(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
+
+int check_paged(const char *who, const cuq_paged_kv *kv, const cuq_batch *b, bool queries, PagedArgs &a) {
+    CUQ_CHECK_ARG(kv && b, "%s: null descriptor", who);
+    if (kv->type != CUQ_F16 && kv->type != CUQ_BF16) {
+        set_error("%s: unsupported cache type %d (F16 or BF16)", who, kv->type);
+        return CUQ_EUNSUPPORTED;
+    }
+    if (kv->head_dim != 64 && kv->head_dim != 128) {
+        set_error("%s: unsupported head_dim %u (64 or 128)", who, kv->head_dim);
+        return CUQ_EUNSUPPORTED;
+    }
+    const uint32_t ps = kv->page_size;
+    if (ps < 16 || ps > 256 || (ps & (ps - 1))) {
+        set_error("%s: unsupported page_size %u (a power of two, 16 to 256)", who, ps);
+        return CUQ_EUNSUPPORTED;
+    }
+    CUQ_CHECK_ARG(kv->k && kv->v && aligned16(kv->k) && aligned16(kv->v), "%s: pools must be 16-byte aligned", who);
+    CUQ_CHECK_ARG(kv->kv_heads > 0 && kv->kv_heads <= 65535 && kv->n_pages > 0 && kv->n_pages <= 0x7FFFFFFFu,
+                  "%s: bad pool (%u pages, %u KV heads)", who, kv->n_pages, kv->kv_heads);
+    const uint64_t dense = (uint64_t)kv->kv_heads * ps * kv->head_dim;
+    const uint64_t stride = kv->page_stride ? kv->page_stride : dense;
+    CUQ_CHECK_ARG(stride >= dense && stride % 8 == 0 && stride < (1ull << 38),
+                  "%s: page_stride %llu (at least %llu, a multiple of 8)", who, (unsigned long long)stride,
+                  (unsigned long long)dense);
+    CUQ_CHECK_ARG(b->n_seqs <= 65535, "%s: %u sequences (at most 65535)", who, b->n_seqs);
+    CUQ_CHECK_ARG(b->n_tok <= 0x3FFFFFFFu && b->max_kv <= 0x3FFFFFFFu && b->max_q <= 0x3FFFFFFFu &&
+                      b->pages_stride <= 0x3FFFFFFFu,
+                  "%s: batch sizes past 2^30", who);
+    if (b->n_seqs) {
+        CUQ_CHECK_ARG(b->kv_len && b->pages && aligned4(b->kv_len) && aligned4(b->pages),
+                      "%s: kv_len and pages must be given", who);
+        CUQ_CHECK_ARG(!queries || (b->q_start && aligned4(b->q_start)), "%s: q_start must be given", who);
+    }
+    a.k = kv->k;
+    a.v = kv->v;
+    a.page_stride = stride;
+    a.n_pages = kv->n_pages;
+    a.page_size = ps;
+    a.page_shift = (uint32_t)__builtin_ctz(ps);
+    a.kv_heads = kv->kv_heads;
+    a.q_start = b->q_start;
+    a.kv_len = b->kv_len;
+    a.pages = b->pages;
+    a.n_seqs = b->n_seqs;
+    a.n_tok = b->n_tok;
+    a.pages_stride = b->pages_stride;
+    a.max_q = b->max_q < b->n_tok ? b->max_q : b->n_tok;
+    const uint64_t slots = (uint64_t)b->pages_stride * ps;
+    a.max_kv = slots < b->max_kv ? (uint32_t)slots : b->max_kv;
+    return CUQ_OK;
+}
+
+int check_heads(const char *who, const cuq_paged_kv *kv, uint32_t heads) {
+    CUQ_CHECK_ARG(heads > 0 && heads <= 65535 && heads % kv->kv_heads == 0,
+                  "%s: heads (%u) must be a positive multiple of kv_heads (%u)", who, heads, kv->kv_heads);
+    return CUQ_OK;
+}
+
+int check_query(const char *who, const cuq_paged_kv *kv, const void *q, size_t q_stride, int type, uint32_t heads,
+                float scale, int causal, uint32_t window, PagedQuery &out) {
+    int rc = check_heads(who, kv, heads);
+    if (rc) return rc;
+    if (!(type == kv->type || (type == CUQ_F32 && kv->type == CUQ_F16))) {
+        set_error("%s: unsupported type %d over a cache of type %d (the cache's own, or F32 over F16)", who, type,
+                  kv->type);
+        return CUQ_EUNSUPPORTED;
+    }
+    CUQ_CHECK_ARG(q && aligned16(q), "%s: q must be 16-byte aligned", who);
+    CUQ_CHECK_ARG(q_stride % 8 == 0 && q_stride >= (size_t)heads * kv->head_dim,
+                  "%s: q_stride %zu (a multiple of 8, at least %zu)", who, q_stride, (size_t)heads * kv->head_dim);
+    CUQ_CHECK_ARG(std::isfinite(scale), "%s: scale must be finite", who);
+    CUQ_CHECK_ARG(causal || window == 0, "%s: a window needs a causal mask", who);
+    out.q = q;
+    out.q_stride = q_stride;
+    out.heads = heads;
+    out.group = heads / kv->kv_heads;
+    out.scale = scale;
+    out.causal = causal ? 1 : 0;
+    out.window = window;
+    return CUQ_OK;
+}
+
+}  // namespace
+}  // namespace cuq
+
+using namespace cuq;
+
+extern "C" {
+
+cuq_rope_plan *cuq_rope_plan_create(const cuq_rope_params *p) {
+    auto bad = [](const char *what) -> cuq_rope_plan * {
+        set_error("cuq_rope_plan_create: %s", what);
+        return nullptr;
+    };
+    if (!p) return bad("null argument");
+    if (p->rot_dim == 0 || p->rot_dim % 16 || p->rot_dim > 2 * ROPE_MAX_PAIRS)
+        return bad("rot_dim must be a multiple of 16, 16 to 128");
+    if (!(p->theta > 1.0f) || !std::isfinite(p->theta)) return bad("theta must be above 1");
+    if (p->scaling < CUQ_ROPE_NONE || p->scaling > CUQ_ROPE_YARN) return bad("unknown scaling");
+    if (p->scaling != CUQ_ROPE_NONE && !(p->factor >= 1.0f && std::isfinite(p->factor)))
+        return bad("factor must be at least 1");
+    if (p->scaling == CUQ_ROPE_LLAMA3 &&
+        !(p->orig_ctx > 0 && p->low_freq > 0 && p->high_freq > p->low_freq && std::isfinite(p->high_freq)))
+        return bad("LLAMA3 needs orig_ctx and 0 < low_freq < high_freq");
+    if (p->scaling == CUQ_ROPE_YARN &&
+        !(p->orig_ctx > 0 && p->beta_slow > 0 && p->beta_fast >= p->beta_slow && std::isfinite(p->beta_fast) &&
+          p->attn_factor >= 0 && std::isfinite(p->attn_factor)))
+        return bad("YARN needs orig_ctx, 0 < beta_slow <= beta_fast and attn_factor >= 0");
+    cuq_rope_plan *plan = new (std::nothrow) cuq_rope_plan();
+    if (!plan) return bad("out of memory");
+    const double two_pi = 6.283185307179586476925286766559;
+    const uint32_t half = p->rot_dim / 2;
+    double low = 0, high = 1;
+    if (p->scaling == CUQ_ROPE_YARN) {
+        auto at = [&](double turns) {  // the pair index at which orig_ctx holds that many turns
+            return p->rot_dim * std::log((double)p->orig_ctx / (turns * two_pi)) / (2 * std::log((double)p->theta));
+        };
+        low = std::fmax(0.0, std::floor(at(p->beta_fast)));
+        high = std::fmin((double)p->rot_dim - 1, std::ceil(at(p->beta_slow)));
+    }
+    plan->t.mul = 1.f;
+    for (uint32_t j = 0; j < half; j++) {
+        double f = std::pow((double)p->theta, -2.0 * j / p->rot_dim);
+        if (p->scaling == CUQ_ROPE_LINEAR) {
+            f /= p->factor;
+        } else if (p->scaling == CUQ_ROPE_LLAMA3) {
+            double s = ((double)p->orig_ctx * f / two_pi - p->low_freq) / ((double)p->high_freq - p->low_freq);
+            s = std::fmin(1.0, std::fmax(0.0, s));
+            f = (1 - s) * f / p->factor + s * f;
+        } else if (p->scaling == CUQ_ROPE_YARN) {
+            const double r = std::fmin(1.0, std::fmax(0.0, (j - low) / std::fmax(high - low, 0.001)));
+            f = f / p->factor * r + f * (1 - r);
+        }
+        plan->t.turns[j] = (uint64_t)std::llrint(std::ldexp(f / two_pi, 63)) * 2;  // f <= 1: below 2^61
+    }
+    for (uint32_t j = half; j < (uint32_t)ROPE_MAX_PAIRS; j++) plan->t.turns[j] = 0;
+    if (p->scaling == CUQ_ROPE_YARN)
+        plan->t.mul = p->attn_factor > 0 ? p->attn_factor : (float)(0.1 * std::log((double)p->factor) + 1.0);
+    plan->t.rot = p->rot_dim;
+    plan->t.adjacent = p->adjacent ? 1 : 0;
+    return plan;
+}
+
+void cuq_rope_plan_free(cuq_rope_plan *p) { delete p; }
+
+int cuq_rope_append(const cuq_rope_plan *rope, const cuq_paged_kv *kv, const cuq_batch *batch,
+                    const int32_t *positions, void *q_out, size_t q_out_stride, int out_type, const void *q,
+                    size_t q_stride, const void *k, const void *v, size_t kv_stride, int in_type, uint32_t heads,
+                    void *stream) {
+    const char *who = "cuq_rope_append";
+    RopeArgs p;
+    CUQ_CHECK_ARG(rope, "%s: null plan", who);
+    int rc = check_paged(who, kv, batch, true, p.a);
+    if (rc == CUQ_OK) rc = check_heads(who, kv, heads);
+    if (rc) return rc;
+    CUQ_CHECK_ARG(rope->t.rot <= kv->head_dim, "%s: rot_dim %u exceeds head_dim %u", who, rope->t.rot, kv->head_dim);
+    if (in_type != CUQ_F32 && in_type != CUQ_F16 && in_type != CUQ_BF16) {
+        set_error("%s: unsupported type %d (F32, F16 or BF16)", who, in_type);
+        return CUQ_EUNSUPPORTED;
+    }
+    if (out_type != in_type && out_type != kv->type) {
+        set_error("%s: unsupported output type %d (the input's or the cache's)", who, out_type);
+        return CUQ_EUNSUPPORTED;
+    }
+    CUQ_CHECK_ARG(q && k && v && q_out && aligned16(q) && aligned16(k) && aligned16(v) && aligned16(q_out),
+                  "%s: q, k, v and q_out must be 16-byte aligned", who);
+    CUQ_CHECK_ARG(positions == nullptr || aligned4(positions), "%s: positions must be 4-byte aligned", who);
+    const size_t qd = (size_t)heads * kv->head_dim, kd = (size_t)kv->kv_heads * kv->head_dim;
+    CUQ_CHECK_ARG(q_stride % 8 == 0 && q_stride >= qd && q_out_stride % 8 == 0 && q_out_stride >= qd &&
+                      kv_stride % 8 == 0 && kv_stride >= kd,
+                  "%s: strides must be multiples of 8, at least %zu (q) and %zu (k, v)", who, qd, kd);
+    CUQ_CHECK_ARG(q_out != q || (out_type == in_type && q_out_stride == q_stride),
+                  "%s: q_out may be q only with its type and stride", who);
+    if (batch->n_tok == 0 || batch->n_seqs == 0) return CUQ_OK;
+    p.positions = positions;
+    p.q_out = q_out;
+    p.q_out_stride = q_out_stride;
+    p.q = q;
+    p.k = k;
+    p.v = v;
+    p.q_stride = q_stride;
+    p.kv_stride = kv_stride;
+    p.heads = heads;
+    cudaStream_t s = (cudaStream_t)stream;
+    if (in_type == CUQ_F32)
+        return launch_rope_append<float>(p, rope->t, out_type, kv->type, kv->head_dim, s);
+    if (in_type == CUQ_F16)
+        return launch_rope_append<__half>(p, rope->t, out_type, kv->type, kv->head_dim, s);
+    return launch_rope_append<__nv_bfloat16>(p, rope->t, out_type, kv->type, kv->head_dim, s);
+}
+
+size_t cuq_attention_paged_workspace(const cuq_paged_kv *kv, const cuq_batch *batch, uint32_t heads, int type) {
+    AttnPagedCall c{};
+    if (check_paged("cuq_attention_paged_workspace", kv, batch, false, c.a) != CUQ_OK) return 0;
+    if (check_heads("cuq_attention_paged_workspace", kv, heads) != CUQ_OK) return 0;
+    c.q.heads = heads;
+    c.q.group = heads / kv->kv_heads;
+    c.type = type;
+    c.cache_type = kv->type;
+    c.hd = kv->head_dim;
+    return attention_paged_workspace(c, sm_count_current());
+}
+
+int cuq_attention_paged(const cuq_paged_kv *kv, const cuq_batch *batch, void *out, size_t out_stride, const void *q,
+                        size_t q_stride, int type, float *lse, uint32_t heads, float scale, int causal,
+                        uint32_t window, void *workspace, size_t workspace_bytes, void *stream) {
+    const char *who = "cuq_attention_paged";
+    AttnPagedCall c{};
+    int rc = check_paged(who, kv, batch, true, c.a);
+    if (rc == CUQ_OK) rc = check_query(who, kv, q, q_stride, type, heads, scale, causal, window, c.q);
+    if (rc) return rc;
+    CUQ_CHECK_ARG(out && aligned16(out) && out != q, "%s: out must be 16-byte aligned and not q", who);
+    CUQ_CHECK_ARG(out_stride % 8 == 0 && out_stride >= (size_t)heads * kv->head_dim,
+                  "%s: out_stride %zu (a multiple of 8, at least %zu)", who, out_stride,
+                  (size_t)heads * kv->head_dim);
+    CUQ_CHECK_ARG(lse == nullptr || aligned4(lse), "%s: lse must be 4-byte aligned", who);
+    c.out = out;
+    c.out_stride = out_stride;
+    c.lse = lse;
+    c.type = type;
+    c.cache_type = kv->type;
+    c.hd = kv->head_dim;
+    c.workspace = workspace;
+    const int sms = sm_count_current();
+    const size_t need = attention_paged_workspace(c, sms);
+    CUQ_CHECK_ARG(workspace_bytes >= need && (need == 0 || workspace),
+                  "%s: workspace of %zu bytes, %zu needed (cuq_attention_paged_workspace)", who, workspace_bytes, need);
+    CUQ_CHECK_ARG(need == 0 || (reinterpret_cast<uintptr_t>(workspace) & 255) == 0,
+                  "%s: workspace must be 256-byte aligned", who);
+    if (batch->n_tok == 0 || batch->n_seqs == 0 || c.a.max_q == 0) return CUQ_OK;
+    return launch_attention_paged(c, sms, (cudaStream_t)stream);
+}
+
+int cuq_attention_mass(const cuq_paged_kv *kv, const cuq_batch *batch, float *mass, size_t mass_stride,
+                       const void *q, size_t q_stride, int type, const float *lse, uint32_t heads, float scale,
+                       int causal, uint32_t window, uint32_t last_q, float decay, void *stream) {
+    const char *who = "cuq_attention_mass";
+    MassPagedCall c{};
+    int rc = check_paged(who, kv, batch, true, c.a);
+    if (rc == CUQ_OK) rc = check_query(who, kv, q, q_stride, type, heads, scale, causal, window, c.q);
+    if (rc) return rc;
+    CUQ_CHECK_ARG(mass && lse && aligned4(mass) && aligned4(lse), "%s: mass and lse must be given", who);
+    CUQ_CHECK_ARG(mass_stride >= c.a.max_kv, "%s: mass_stride %zu is below max_kv %u", who, mass_stride, c.a.max_kv);
+    CUQ_CHECK_ARG(std::isfinite(decay), "%s: decay must be finite", who);
+    if (batch->n_seqs == 0 || c.a.max_kv == 0) return CUQ_OK;
+    c.mass = mass;
+    c.mass_stride = mass_stride;
+    c.lse = lse;
+    c.type = type;
+    c.cache_type = kv->type;
+    c.hd = kv->head_dim;
+    c.last_q = last_q;
+    c.decay = decay;
+    return launch_attention_mass(c, sm_count_current(), (cudaStream_t)stream);
+}
+
+int cuq_kv_evict(const cuq_paged_kv *kv, const cuq_batch *batch, const float *mass, size_t mass_stride,
+                 uint32_t keep, uint32_t sink, uint32_t recent, int32_t *kept, int32_t *new_len, float *mass_out,
+                 size_t mass_out_stride, void *stream) {
+    const char *who = "cuq_kv_evict";
+    EvictArgs p;
+    int rc = check_paged(who, kv, batch, false, p.a);
+    if (rc) return rc;
+    CUQ_CHECK_ARG(keep > 0 && keep <= 0x3FFFFFFFu && (uint64_t)sink + recent <= keep,
+                  "%s: keep %u with sink %u and recent %u (sink + recent <= keep)", who, keep, sink, recent);
+    CUQ_CHECK_ARG(mass && kept && new_len && aligned4(mass) && aligned4(kept) && aligned4(new_len),
+                  "%s: mass, kept and new_len must be given", who);
+    CUQ_CHECK_ARG(new_len != batch->kv_len, "%s: new_len must not be the batch's kv_len", who);
+    CUQ_CHECK_ARG(mass_stride >= p.a.max_kv, "%s: mass_stride %zu is below max_kv %u", who, mass_stride, p.a.max_kv);
+    CUQ_CHECK_ARG(mass_out == nullptr || (aligned4(mass_out) && mass_out_stride >= p.a.max_kv),
+                  "%s: mass_out_stride %zu is below max_kv %u", who, mass_out_stride, p.a.max_kv);
+    CUQ_CHECK_ARG(mass_out != mass || mass_out_stride == mass_stride, "%s: mass in place needs its own stride", who);
+    if (batch->n_seqs == 0) return CUQ_OK;
+    p.mass = mass;
+    p.mass_stride = mass_stride;
+    p.keep = keep;
+    p.sink = sink;
+    p.recent = recent;
+    p.kept = kept;
+    p.new_len = new_len;
+    p.mass_out = mass_out;
+    p.mass_out_stride = mass_out_stride;
+    cudaStream_t s = (cudaStream_t)stream;
+    const uint32_t rows = batch->n_seqs * kv->kv_heads;
+    evict_select_kernel<<<rows, SEL_THREADS, 0, s>>>(p);
+    CUQ_CUDA_TRY(cudaGetLastError());
+    if (p.a.max_kv <= keep) return CUQ_OK;  // nothing can move
+    if (kv->head_dim == 64)
+        evict_move_kernel<64, 64><<<rows * 2 * 2, MOVE_THREADS, 0, s>>>(p);
+    else
+        evict_move_kernel<128, 64><<<rows * 2 * 4, MOVE_THREADS, 0, s>>>(p);
+    CUQ_CUDA_TRY(cudaGetLastError());
+    return CUQ_OK;
+}
+
+int cuq_paged_status(void *stream) {
+    CUQ_CUDA_TRY(cudaStreamSynchronize((cudaStream_t)stream));
+    return CUQ_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,144 @@
+// paged.cuh -- what the paged-cache kernels share: the device view of a cache
+// and a batch (include/cuq.h, cuq_paged_kv / cuq_batch), typed loads and stores.
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+
+namespace cuq {
+
+// The cache and the batch as a kernel sees them.  Every length and page id that
+// comes from device memory is cut or checked here, so no kernel reads past a
+// pool, a table or a token tensor whatever the arrays hold.
+struct PagedArgs {
+    void *k, *v;
+    uint64_t page_stride;            // elements
+    uint32_t n_pages, page_size, page_shift, kv_heads;
+    const int32_t *q_start, *kv_len, *pages;
+    uint32_t n_seqs, n_tok, pages_stride, max_q, max_kv;  // max_kv: already cut to the table's slots
+
+    __device__ __forceinline__ uint32_t len(uint32_t b) const {
+        const int n = __ldg(kv_len + b);
+        return n <= 0 ? 0u : min((uint32_t)n, max_kv);
+    }
+    // first token row of sequence b and its token count (at most n_tok rows in all)
+    __device__ __forceinline__ uint32_t tokens(uint32_t b, uint32_t &first) const {
+        const int a = __ldg(q_start + b), e = __ldg(q_start + b + 1);
+        first = a <= 0 ? 0u : min((uint32_t)a, n_tok);
+        const uint32_t end = e <= 0 ? 0u : min((uint32_t)e, n_tok);
+        return end > first ? end - first : 0u;
+    }
+    __device__ __forceinline__ int page(uint32_t b, uint32_t col) const {
+        const int id = __ldg(pages + (size_t)b * pages_stride + col);
+        return (id >= 0 && (uint32_t)id < n_pages) ? id : -1;
+    }
+    // element offset of row `slot` of KV head h inside a pool; the page id is valid
+    template <int HD>
+    __device__ __forceinline__ size_t row(int page_id, uint32_t h, uint32_t slot) const {
+        return (size_t)page_id * page_stride + ((size_t)h * page_size + (slot & (page_size - 1))) * HD;
+    }
+};
+
+// q, lse and the mask of the attention ops.
+struct PagedQuery {
+    const void *q;
+    size_t q_stride;
+    uint32_t heads, group;
+    float scale;
+    int causal;
+    uint32_t window;
+
+    // the slots [lo, hi) that the query at slot `pos` of a cache of n slots sees
+    __device__ __forceinline__ void range(int pos, uint32_t n, uint32_t &lo, uint32_t &hi) const {
+        lo = 0;
+        hi = n;
+        if (pos < 0) {
+            hi = 0;
+            return;
+        }
+        if (causal) {
+            hi = min(n, (uint32_t)pos + 1);
+            if (window && (uint32_t)pos + 1 > window) lo = (uint32_t)pos + 1 - window;
+        }
+    }
+};
+
+template <typename T>
+struct Pair;  // two 16-bit values in one register
+template <>
+struct Pair<__half> {
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+    static __device__ __forceinline__ float2 unpack(uint32_t u) {
+        return __half22float2(*reinterpret_cast<const __half2 *>(&u));
+    }
+};
+template <>
+struct Pair<__nv_bfloat16> {
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+    static __device__ __forceinline__ float2 unpack(uint32_t u) {
+        return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
+    }
+};
+
+// eight values of any of the three types, as fp32
+template <typename T>
+__device__ __forceinline__ void load8(const T *p, float (&v)[8]) {
+    const uint4 u = __ldg(reinterpret_cast<const uint4 *>(p));
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 f = Pair<T>::unpack(w[i]);
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+    }
+}
+template <>
+__device__ __forceinline__ void load8<float>(const float *p, float (&v)[8]) {
+    const float4 a = __ldg(reinterpret_cast<const float4 *>(p)), b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
+template <typename T>
+__device__ __forceinline__ void store8(T *p, const float (&v)[8]) {
+    *reinterpret_cast<uint4 *>(p) = make_uint4(Pair<T>::pack(v[0], v[1]), Pair<T>::pack(v[2], v[3]),
+                                               Pair<T>::pack(v[4], v[5]), Pair<T>::pack(v[6], v[7]));
+}
+template <>
+__device__ __forceinline__ void store8<float>(float *p, const float (&v)[8]) {
+    reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+
+// Launchers (paged_attn.cu, paged_mass.cu): arguments are checked in paged.cu.
+struct AttnPagedCall {
+    PagedArgs a;
+    PagedQuery q;
+    void *out;
+    size_t out_stride;
+    float *lse;
+    int type, cache_type;
+    uint32_t hd;
+    void *workspace;
+};
+size_t attention_paged_workspace(const AttnPagedCall &c, int sm_count);
+int launch_attention_paged(const AttnPagedCall &c, int sm_count, cudaStream_t s);
+
+struct MassPagedCall {
+    PagedArgs a;
+    PagedQuery q;
+    float *mass;
+    size_t mass_stride;
+    const float *lse;
+    int type, cache_type;
+    uint32_t hd, last_q;
+    float decay;
+};
+int launch_attention_mass(const MassPagedCall &c, int sm_count, cudaStream_t s);
+
+}  // namespace cuq

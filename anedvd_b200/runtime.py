@@ -47,6 +47,14 @@ SIGNATURES = [
     ("cuq_attention_prefill", I32, [P, P, P, P, U32, U32, U32, U32, U32, U32, P]),
     ("cuq_argmax", I32, [P, U32, P, P]),
     ("cuq_sample", I32, [P, U32, P, P, U32, P, P, P]),
+    ("cuq_rope_plan_create", P, [P]),
+    ("cuq_rope_plan_free", None, [P]),
+    ("cuq_rope_append", I32, [P, P, P, P, P, SZ, I32, P, SZ, P, P, SZ, I32, U32, P]),
+    ("cuq_attention_paged_workspace", SZ, [P, P, U32, I32]),
+    ("cuq_attention_paged", I32, [P, P, P, SZ, P, SZ, I32, P, U32, F32, I32, U32, P, SZ, P]),
+    ("cuq_attention_mass", I32, [P, P, P, SZ, P, SZ, I32, P, U32, F32, I32, U32, U32, F32, P]),
+    ("cuq_kv_evict", I32, [P, P, P, SZ, U32, U32, U32, P, P, P, SZ, P]),
+    ("cuq_paged_status", I32, [P]),
     ("cuq_model_create", P, [P, P]),
     ("cuq_upload_tensor", I32, [P, I32, I32, I32, P, SZ, U32, U32]),
     ("cuq_upload_f32", I32, [P, I32, I32, P, SZ]),
@@ -125,6 +133,27 @@ class CuqSamplerParams(ctypes.Structure):
                          min_keep_delta)
 
 
+class CuqPagedKv(ctypes.Structure):
+    """cuq_paged_kv: the pools of a paged KV cache."""
+    _fields_ = [("k", P), ("v", P), ("type", ctypes.c_int32), ("n_pages", U32), ("page_size", U32), ("kv_heads", U32),
+                ("head_dim", U32), ("page_stride", U64)]
+
+
+class CuqBatch(ctypes.Structure):
+    """cuq_batch: the sequences that share one call."""
+    _fields_ = [("q_start", P), ("kv_len", P), ("pages", P), ("n_seqs", U32), ("n_tok", U32), ("pages_stride", U32),
+                ("max_q", U32), ("max_kv", U32)]
+
+
+ROPE_NONE, ROPE_LINEAR, ROPE_LLAMA3, ROPE_YARN = 0, 1, 2, 3
+
+
+class CuqRopeParams(ctypes.Structure):
+    _fields_ = [("rot_dim", U32), ("adjacent", ctypes.c_int32), ("theta", F32), ("scaling", ctypes.c_int32),
+                ("factor", F32), ("low_freq", F32), ("high_freq", F32), ("beta_fast", F32), ("beta_slow", F32),
+                ("attn_factor", F32), ("orig_ctx", U32)]
+
+
 class CuqStats(ctypes.Structure):
     _fields_ = [("tokens", U64), ("prefill_tokens", U64), ("decode_ms", ctypes.c_double),
                 ("prefill_ms", ctypes.c_double), ("weight_bytes", U64), ("kv_bytes", U64),
@@ -176,6 +205,23 @@ def check(rc):
 
 def init(device=0):
     return check(load().cuq_init(device))
+
+
+class RopePlan:
+    """A cuq_rope_plan handle (`handle`): the frequencies of one CuqRopeParams."""
+
+    def __init__(self, params):
+        self.handle = load().cuq_rope_plan_create(ctypes.byref(params))
+        if not self.handle:
+            raise CuqError(EINVAL, last_error())
+
+    def close(self):
+        if getattr(self, "handle", None):
+            load().cuq_rope_plan_free(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        self.close()
 
 
 class GgufFile:

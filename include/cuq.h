@@ -187,6 +187,137 @@ typedef struct {
 int cuq_sample(float *logits_dev, uint32_t vocab, const cuq_sampler_params *params, const uint32_t *recent_dev,
                uint32_t n_recent, uint32_t *rng_dev, uint32_t *token_dev, void *stream);
 
+/* ------------------------------------------------- paged KV cache ---- */
+
+/* Serving several sequences from one paged cache.  No counterpart in the
+ * reference, whose session owns one contiguous cache; these ops stand beside
+ * cuq_rope, cuq_attention_decode / _prefill and cuq_kv_write for callers that
+ * batch requests.  All of them only enqueue work on `stream` and allocate
+ * nothing, so they can be captured in a graph; all pointers are dev pointers of
+ * the current device unless marked host, and the two descriptors are host
+ * structs read at the call.
+ *
+ * The cache is two pools k, v of [n_pages][kv_heads][page_size][head_dim]
+ * values (one head's rows of a page are contiguous), pages page_stride elements
+ * apart (0: kv_heads * page_size * head_dim).  type: CUQ_F16 or CUQ_BF16;
+ * page_size a power of two, 16 to 256; head_dim 64 or 128; pools 16-byte
+ * aligned, page_stride a multiple of 8. */
+typedef struct {
+    void *k, *v;
+    int32_t type;
+    uint32_t n_pages, page_size, kv_heads, head_dim;
+    uint64_t page_stride;
+} cuq_paged_kv;
+
+/* A batch of sequences.  The new tokens of sequence b are the rows
+ * [q_start[b], q_start[b + 1]) of the token tensors (q_start ascending, up to
+ * n_tok; rows from q_start[n_seqs] on belong to no sequence and are left as
+ * they are).  kv_len[b] counts its cached slots INCLUDING the new tokens, so
+ * new token i stands at slot kv_len[b] - (q_start[b + 1] - q_start[b]) + i; a
+ * token whose slot is negative is not cached and sees nothing.  pages[b][j] is
+ * the pool page of slots [j * page_size, (j + 1) * page_size); an id outside
+ * [0, n_pages) is a hole: nothing is read from it or written to it, and
+ * attention treats its slots as masked (pages given back behind a sliding
+ * window).  max_q and max_kv (host) bound the new tokens and the cached slots
+ * of any one sequence: tokens past max_q are not attended, and lengths are cut
+ * to min(max_kv, pages_stride * page_size).  Lengths and tables are read on the
+ * device, so a captured graph follows them. */
+typedef struct {
+    const int32_t *q_start;  /* [n_seqs + 1] (cuq_kv_evict: unused) */
+    const int32_t *kv_len;   /* [n_seqs] */
+    const int32_t *pages;    /* [n_seqs][pages_stride] */
+    uint32_t n_seqs, n_tok, pages_stride, max_q, max_kv;
+} cuq_batch;
+
+/* Rotary positions: the first rot_dim (a multiple of 16, at most head_dim)
+ * values of a head turn by pos * f_j, f_j = theta^(-2j / rot_dim), in pairs
+ * (j, j + rot_dim / 2), or (2j, 2j + 1) with `adjacent`.  scaling stretches the
+ * frequencies for contexts longer than trained:
+ *   LINEAR f / factor;
+ *   LLAMA3 by turns t = orig_ctx f / 2 pi: f / factor below low_freq, f above
+ *     high_freq, and (1 - s) f / factor + s f, s = (t - low) / (high - low), between;
+ *   YARN   f / factor * r + f (1 - r) with r rising linearly over the pair
+ *     indices at which orig_ctx holds beta_fast (floor) to beta_slow (ceil)
+ *     turns, and cosine and sine times attn_factor (0: 0.1 ln(factor) + 1).
+ * Unlike cuq_rope, which follows the reference's fp32 angles, the angle here is
+ * exact for every position (64-bit fixed-point turns). */
+#define CUQ_ROPE_NONE 0
+#define CUQ_ROPE_LINEAR 1
+#define CUQ_ROPE_LLAMA3 2
+#define CUQ_ROPE_YARN 3
+typedef struct {
+    uint32_t rot_dim;
+    int32_t adjacent;
+    float theta;
+    int32_t scaling;
+    float factor, low_freq, high_freq, beta_fast, beta_slow, attn_factor;
+    uint32_t orig_ctx;
+} cuq_rope_params;
+/* The frequencies of one set of parameters, computed once (host memory only;
+ * usable from any thread, stream and device).  NULL on failure. */
+typedef struct cuq_rope_plan cuq_rope_plan;
+cuq_rope_plan *cuq_rope_plan_create(const cuq_rope_params *params);
+void cuq_rope_plan_free(cuq_rope_plan *p);
+
+/* Rotate the batch's q and k by their positions and append k and v to the
+ * cache.  q [n_tok][heads][head_dim] at q_stride elements per token, k and v
+ * [n_tok][kv_heads][head_dim] at kv_stride (so one packed q||k||v row works),
+ * of in_type CUQ_F32, CUQ_F16 or CUQ_BF16; strides are multiples of 8, pointers
+ * 16-byte aligned.  q_out, out_type in_type or the cache's type, may be q
+ * itself (same type and stride), otherwise it overlaps nothing.  positions
+ * [n_tok] are the rotary positions (any int32; NULL: the token's slot, which is
+ * right unless slots were evicted).  Rows are rotated in fp32 and rounded once. */
+int cuq_rope_append(const cuq_rope_plan *rope, const cuq_paged_kv *kv, const cuq_batch *batch,
+                    const int32_t *positions, void *q_out, size_t q_out_stride, int out_type, const void *q,
+                    size_t q_stride, const void *k, const void *v, size_t kv_stride, int in_type, uint32_t heads,
+                    void *stream);
+
+/* Attention of the batch's new tokens (already appended) over the cache: out =
+ * softmax(scale q k^T) v per head, query head h reading KV head
+ * h / (heads / kv_heads).  type is that of q and out: the cache's, or CUQ_F32
+ * with an fp16 cache (q and the probabilities then run as fp16 hi + lo pairs).
+ * causal: a token sees the slots up to its own; window > 0 (causal only): and
+ * of those the last `window`.  A token that sees nothing gets out 0 and lse
+ * -inf.  lse [n_tok][heads] (may be NULL): the natural log of the sum of
+ * exponentials.  workspace: cuq_attention_paged_workspace bytes, 256-byte
+ * aligned (may be NULL when that is 0); two calls that may run at the same
+ * time need one each. */
+size_t cuq_attention_paged_workspace(const cuq_paged_kv *kv, const cuq_batch *batch, uint32_t heads, int type);
+int cuq_attention_paged(const cuq_paged_kv *kv, const cuq_batch *batch, void *out, size_t out_stride, const void *q,
+                        size_t q_stride, int type, float *lse, uint32_t heads, float scale, int causal,
+                        uint32_t window, void *workspace, size_t workspace_bytes, void *stream);
+
+/* The attention weight every cached slot gathers:
+ *   mass[b][kv head][slot] = decay * mass + sum of exp(scale q k - lse)
+ * over the batch's queries (only the last last_q of each sequence when > 0) and
+ * the query heads of the group, with the lse that cuq_attention_paged wrote for
+ * the same arguments.  mass is f32 [n_seqs][kv_heads][mass_stride] (mass_stride
+ * >= max_kv); slots at or past kv_len are left as they are.  decay 0 overwrites
+ * (whatever mass held, NaN too).  Sums are in fp32 in a fixed order. */
+int cuq_attention_mass(const cuq_paged_kv *kv, const cuq_batch *batch, float *mass, size_t mass_stride,
+                       const void *q, size_t q_stride, int type, const float *lse, uint32_t heads, float scale,
+                       int causal, uint32_t window, uint32_t last_q, float decay, void *stream);
+
+/* Evict: of each sequence and KV head keep the first `sink` and the last
+ * `recent` slots and, of the others, those with the largest mass (equal mass:
+ * the lowest slot; NaN counts as the smallest), `keep` in all (sink + recent <=
+ * keep), in their order, moved to slots [0, n), n = min(kv_len, keep).  The
+ * rows move in place inside the sequence's own pages; rows on a hole are not
+ * moved and rows are not moved onto one.  kept [n_seqs][kv_heads][keep] gets the old slot of each new one
+ * (-1 behind the last), new_len [n_seqs] the new length (not the array of
+ * kv_len).  mass_out (NULL: none; mass itself: in place; otherwise no overlap)
+ * gets the kept slots' mass at [0, n) and 0 at [n, kv_len).  Keys keep the
+ * rotary positions they were cached with.  No two sequences may share a page
+ * that holds one of their slots. */
+int cuq_kv_evict(const cuq_paged_kv *kv, const cuq_batch *batch, const float *mass, size_t mass_stride,
+                 uint32_t keep, uint32_t sink, uint32_t recent, int32_t *kept, int32_t *new_len, float *mass_out,
+                 size_t mass_out_stride, void *stream);
+
+/* Waits for `stream` and reports whether a bounded wait inside one of the
+ * current device's paged kernels gave up since the last such call
+ * (CUQ_ETIMEOUT, then cleared). */
+int cuq_paged_status(void *stream);
+
 /* ------------------------------------------------------------ engine ---- */
 
 /* Model geometry: the fields of model.Config (model.zig:10-244) this path uses. */
