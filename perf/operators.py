@@ -379,7 +379,8 @@ def _handles(s):
     from anedvd_b200 import runtime as rt
 
     c = s["case"]
-    rt.init(torch.cuda.current_device())
+    if not rt.load().cuq_ready():  # once in a program
+        rt.init(torch.cuda.current_device())
     kv = rt.CuqPagedKv(k=s["k"].data_ptr(), v=s["v"].data_ptr(), type=GGML[c["cache"]], n_pages=s["n_pages"],
                        page_size=c["page"], kv_heads=c["kv_heads"], head_dim=c["hd"], page_stride=0)
     start = s.get("q_start")
