@@ -635,7 +635,14 @@ int cuq_kv_evict(const cuq_paged_kv *kv, const cuq_batch *batch, const float *ma
 
 int cuq_paged_status(void *stream) {
     CUQ_CUDA_TRY(cudaStreamSynchronize((cudaStream_t)stream));
-    return CUQ_OK;
+    int few = 0, many = 0;
+    int rc = attention_few_status((cudaStream_t)stream, &few);
+    if (rc == CUQ_OK) rc = attention_many_status((cudaStream_t)stream, &many);
+    if (rc == CUQ_OK && (few || many)) {
+        set_error("a wait inside a paged-cache kernel gave up");
+        rc = CUQ_ETIMEOUT;
+    }
+    return rc;
 }
 
 }  // extern "C"

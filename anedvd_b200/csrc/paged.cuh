@@ -115,7 +115,16 @@ __device__ __forceinline__ void store8<float>(float *p, const float (&v)[8]) {
     reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
 }
 
-// Launchers (paged_attn.cu, paged_mass.cu): arguments are checked in paged.cu.
+// ------------------------------------------------------------ attention ----
+//
+// A sequence's rows are its (new token, query head of the group) pairs, token
+// major.  Sequences of up to ATTN_FEW rows per KV head go to the mma.sync kernel
+// (paged_attn.cu), whose tile is 16 rows and whose time is the cache's bytes;
+// larger ones to the tcgen05 kernel (paged_attn_tc.cu), 2 x 128 rows.  Both may
+// split the slots over CTAs: partial results, out normalised and the log2 of the
+// sum of exponentials, go to the workspace and are joined by the merge kernel.
+constexpr uint32_t ATTN_FEW = 16;
+
 struct AttnPagedCall {
     PagedArgs a;
     PagedQuery q;
@@ -126,8 +135,35 @@ struct AttnPagedCall {
     uint32_t hd;
     void *workspace;
 };
+
+// How a call is split; a function of the call's host-side sizes alone.
+struct AttnPlan {
+    bool few, many;        // which kernels run
+    uint32_t few_chunk;    // slots per CTA of the mma.sync kernel
+    uint32_t few_splits, many_splits;
+    uint32_t many_tiles;   // bound of the 256-row tiles of all sequences
+    // whether a sequence of `tokens` attended tokens is the mma.sync kernel's
+    __device__ __forceinline__ bool is_few(uint32_t tokens, uint32_t group) const {
+        return few && tokens * group <= ATTN_FEW;
+    }
+};
+AttnPlan attention_paged_plan(const AttnPagedCall &c, int sm_count);
 size_t attention_paged_workspace(const AttnPagedCall &c, int sm_count);
 int launch_attention_paged(const AttnPagedCall &c, int sm_count, cudaStream_t s);
+
+// What both kernels get beside the cache and the queries.
+struct AttnOut {
+    void *out;
+    size_t out_stride;
+    float *lse;
+    // parts: normalised outputs [splits][rows][hd] and log2 sums [splits][rows];
+    // rows are [n_seqs][kv_heads][ATTN_FEW] of the few, [n_tok][heads] of the many
+    float *few_o, *few_lse, *many_o, *many_lse;
+    AttnPlan plan;
+};
+int launch_attention_many(const AttnPagedCall &c, const AttnOut &o, cudaStream_t s);
+int attention_many_status(cudaStream_t s, int *timed_out);  // read and cleared
+int attention_few_status(cudaStream_t s, int *timed_out);
 
 struct MassPagedCall {
     PagedArgs a;

@@ -1,0 +1,469 @@
+// paged_attn_tc.cu -- attention of many new tokens over a paged KV cache on the
+// 5th-generation tensor cores (the rows and the split: paged_attn.cu).
+//
+// A CTA takes 256 rows of one KV head as two streams of 128 (a row is a TMEM
+// lane) and walks its part of the slots in tiles of 128 keys:
+//   * warp 9 loads each tile's K and V pages by TMA (128-byte swizzle) into a ring;
+//   * one lane of warp 8 issues S = Q K^T (both operands in shared memory) and
+//     O += P V (P in tensor memory, V with its dims contiguous) for both streams;
+//   * warps 0-3 and 4-7 are the streams' softmax: a thread owns a row, reads its
+//     128 scores from tensor memory, keeps the running maximum and sum in
+//     registers and writes P over S as 16-bit pairs.
+// While one stream is in its softmax the other's products run.  S of tile j + 1 is
+// issued behind O += P V of tile j, so when S is there, O is complete: the softmax
+// threads rescale O themselves, and only when a row's maximum has grown by more
+// than 2^8 (until then P stays below 2^8 and the sum takes it as it is).
+// fp32 queries are two fp16 operands, and P is then two, which together fill S.
+// What bounds it: per 128 x 128 tile the two products take 1024 cycles of the
+// tensor pipe at head_dim 128 (512 at 64) and the exponentials 1024 of the MUFU.
+#include "paged_tc.cuh"
+
+namespace cuq {
+
+using namespace ptc;
+
+namespace {
+
+__device__ int g_timeout;
+
+constexpr int NT = 384;  // warps 0-3, 4-7 softmax, 8 MMA, 9 TMA, 10-11 idle
+constexpr int KEYS = 128;
+
+template <int HD, bool SPLIT>
+struct ManyGeo {
+    static constexpr int CB = HD / 64;
+    static constexpr int TILE = KEYS * HD * 2;                  // bytes of a K or V tile
+    static constexpr int Q = 128 * HD * 2 * (SPLIT ? 2 : 1);    // bytes of one stream's queries
+    static constexpr int ST = (HD == 128) ? (SPLIT ? 3 : 5) : 6;
+    static constexpr int SMEM = 1024 + 2 * Q + ST * TILE;
+};
+
+struct ManyBars {
+    uint64_t q_full[2], kv_full[6], kv_empty[6], s_full[2], p_full[2], o_full[2], clean;
+};
+
+template <typename TQ, typename TC, int HD>
+__global__ void __launch_bounds__(NT, 1) attn_many_kernel(PagedArgs a, PagedQuery q, AttnOut o,
+                                                           const __grid_constant__ CUtensorMap mk,
+                                                           const __grid_constant__ CUtensorMap mv) {
+    constexpr bool SPLIT = std::is_same<TQ, float>::value;
+    using G = ManyGeo<HD, SPLIT>;
+    constexpr int ST = G::ST;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ ManyBars bars;
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_flag;
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t kvh = blockIdx.x % a.kv_heads, split = blockIdx.y;
+
+    // the tile: tiles are counted over the sequences that are this kernel's
+    uint32_t b = 0, tile = blockIdx.x / a.kv_heads, ntile = 0;
+    {
+        bool found = false;
+        for (uint32_t s0 = 0; s0 < a.n_seqs && !found; s0 += 32) {
+            uint32_t cnt = 0, f;
+            if (s0 + lane < a.n_seqs) {
+                const uint32_t tq = min(a.tokens(s0 + lane, f), a.max_q);
+                if (tq && !o.plan.is_few(tq, q.group)) cnt = (tq * q.group + 255) / 256;
+            }
+            uint32_t incl = cnt;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const uint32_t up = __shfl_up_sync(~0u, incl, d);
+                if (lane >= (uint32_t)d) incl += up;
+            }
+            const uint32_t hit = __ballot_sync(~0u, tile < incl);
+            if (hit) {
+                const int l = __ffs(hit) - 1;
+                b = s0 + l;
+                ntile = __shfl_sync(~0u, cnt, l);
+                tile -= __shfl_sync(~0u, incl, l) - ntile;
+                found = true;
+            } else {
+                tile -= __shfl_sync(~0u, incl, 31);
+            }
+        }
+        if (!found) return;  // the same for every warp
+    }
+    tile = ntile - 1 - tile;  // a causal sequence's last tiles see the most slots: first
+    uint32_t first;
+    const uint32_t nq = a.tokens(b, first), n = a.len(b), tq = min(nq, a.max_q);
+    const uint32_t rows = tq * q.group, row0 = tile * 256;
+    const uint32_t my_rows = min(rows - row0, 256u);
+    const int pos0 = (int)n - (int)nq;
+    const bool two = my_rows > 128;
+    // the slots that any of the rows sees, in tiles, and this split's part of them
+    uint32_t j0, j1;
+    {
+        uint32_t lo0, hi0, lo1, hi1;
+        q.range(max(pos0 + (int)(row0 / q.group), 0), n, lo0, hi0);
+        q.range(pos0 + (int)((row0 + my_rows - 1) / q.group), n, lo1, hi1);
+        j0 = lo0 / KEYS;
+        j1 = hi1 > lo0 ? (hi1 + KEYS - 1) / KEYS : j0;
+        const uint32_t per = (j1 - j0 + o.plan.many_splits - 1) / o.plan.many_splits;
+        j0 = min(j1, j0 + split * per);
+        j1 = min(j1, j0 + per);
+    }
+    const uint32_t nt = j1 - j0;
+
+    if (warp == 8) tmem_alloc512(&tmem_slot);
+    if (tid == 0) {
+        abort_flag = 0;
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&bars.q_full[i], 128);
+            mbar_init(&bars.s_full[i], 1);
+            mbar_init(&bars.p_full[i], 128);
+            mbar_init(&bars.o_full[i], 1);
+        }
+        for (int i = 0; i < ST; i++) {
+            mbar_init(&bars.kv_full[i], 1);
+            mbar_init(&bars.kv_empty[i], 1);
+        }
+        mbar_init(&bars.clean, 1);
+        mbar_init_fence();
+    }
+    // are there holes among the slots?  (then the softmax looks each tile's pages up)
+    int hole = 0;
+    for (uint32_t s = (j0 * KEYS >> a.page_shift) + tid; ((uint64_t)s << a.page_shift) < min(n, j1 * KEYS); s += NT)
+        hole |= a.page(b, s) < 0;
+    tc_fence_before();
+    hole = __syncthreads_or(hole);
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    uint8_t *ring = smem + 2 * G::Q;
+
+    if (warp == 8) {
+        // ------------------------------------------------------ MMA issuer
+        if (lane == 0 && nt) {
+            const uint32_t id_s = idesc<TC>(128, KEYS, false), id_o = idesc<TC>(128, HD, true);
+            const uint32_t qa = smem_u32(smem), ra = smem_u32(ring);
+            const uint32_t ns = two ? 2 : 1;
+            auto stage = [&](uint32_t x) { return ra + (x % ST) * G::TILE; };
+            auto wait_kv = [&](uint32_t x) { return mbar_wait(&bars.kv_full[x % ST], (x / ST) & 1, &abort_flag); };
+            auto qk = [&](uint32_t s, uint32_t x) {  // S_s = Q_s K^T with K in stage x
+                const uint32_t kb = stage(x), qb = qa + s * G::Q;
+#pragma unroll
+                for (int part = 0; part < (SPLIT ? 2 : 1); part++)
+#pragma unroll
+                    for (int ks = 0; ks < HD / 16; ks++) {
+                        const uint32_t off = (ks / 4) * (128 * 128) + (ks % 4) * 32;
+                        umma_ss(tmem + s * 128, sdesc_sw128(qb + part * (128 * HD * 2) + off, 16, 1024),
+                                sdesc_sw128(kb + off, 16, 1024), id_s, part | ks ? 1u : 0u);
+                    }
+            };
+            auto pv = [&](uint32_t s, uint32_t x, bool acc) {  // O_s += P_s V with V in stage x
+                const uint32_t vb = stage(x), d = tmem + 256 + s * 128;
+#pragma unroll
+                for (int part = 0; part < (SPLIT ? 2 : 1); part++)
+#pragma unroll
+                    for (int ks = 0; ks < KEYS / 16; ks++)
+                        umma_ts(d, tmem + s * 128 + part * 64 + ks * 8,
+                                sdesc_sw128(vb + ks * 2048, KEYS * 128, 1024), id_o, (acc || part || ks) ? 1u : 0u);
+            };
+            // stage x may be loaded again; only where it will be, so that no arrival is left in flight at the end
+            auto freed = [&](uint32_t x) {
+                if (x + ST < 2 * nt) umma_commit(&bars.kv_empty[x % ST]);
+            };
+            const bool tail = j1 * KEYS > n;
+            bool ok = mbar_wait(&bars.q_full[0], 0, &abort_flag) && (!two || mbar_wait(&bars.q_full[1], 0, &abort_flag)) &&
+                      wait_kv(0);
+            if (ok) {
+                tc_fence_after();
+                for (uint32_t s = 0; s < ns; s++) {
+                    qk(s, 0);
+                    umma_commit(&bars.s_full[s]);
+                }
+                freed(0);
+            }
+            for (uint32_t j = 0; ok && j < nt; j++) {
+                const uint32_t xv = 2 * j + 1, xk = 2 * j + 2;
+                const bool more = j + 1 < nt;
+                ok = wait_kv(xv) && (!more || wait_kv(xk)) &&
+                     (more || !tail || mbar_wait(&bars.clean, 0, &abort_flag));
+                for (uint32_t s = 0; ok && s < ns; s++) {
+                    ok = mbar_wait(&bars.p_full[s], j & 1, &abort_flag);
+                    if (!ok) break;
+                    tc_fence_after();
+                    pv(s, xv, j > 0);
+                    if (more) {
+                        qk(s, xk);
+                        umma_commit(&bars.s_full[s]);
+                    } else {
+                        umma_commit(&bars.o_full[s]);
+                    }
+                }
+                if (ok) {
+                    freed(xv);
+                    if (more) freed(xk);
+                }
+            }
+        }
+    } else if (warp == 9) {
+        // ------------------------------------------------------ TMA: K and V pages
+        const uint32_t box = min(a.page_size, (uint32_t)KEYS), nbox = KEYS / box;
+        auto page_of = [&](uint32_t j) -> int {  // of this lane's box of tile j; past the end: a hole
+            const uint32_t slot = j * KEYS + lane * box;
+            if (lane >= nbox || slot >= n) return (int)a.n_pages;
+            const int pg = a.page(b, slot >> a.page_shift);
+            return pg < 0 ? (int)a.n_pages : pg;
+        };
+        int pg = page_of(j0);
+        bool ok = true;
+        for (uint32_t j = 0; ok && j < nt; j++) {
+            const int next = j + 1 < nt ? page_of(j0 + j + 1) : 0;
+            const int slot = (int)(((j0 + j) * KEYS + lane * box) & (a.page_size - 1));
+#pragma unroll
+            for (int v = 0; v < 2; v++) {
+                const uint32_t x = 2 * j + v, st = x % ST;
+                if (x >= (uint32_t)ST && !mbar_wait(&bars.kv_empty[st], ((x / ST) - 1) & 1, &abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                if (lane == 0) mbar_expect_tx(&bars.kv_full[st], G::TILE);
+                __syncwarp();
+                if (lane < nbox) {
+                    const uint32_t dst = smem_u32(ring + st * G::TILE) + lane * box * 128;
+#pragma unroll
+                    for (int cb = 0; cb < G::CB; cb++)
+                        tma_load_page(dst + cb * (KEYS * 128), v ? &mv : &mk, cb * 64, slot, (int)kvh, pg,
+                                      &bars.kv_full[st]);
+                }
+            }
+            pg = next;
+        }
+        // V rows past the sequence's end may hold anything, and 0 * inf is not 0
+        if (ok && nt && j1 * KEYS > n) {
+            const uint32_t x = 2 * nt - 1, st = x % ST;
+            if (mbar_wait(&bars.kv_full[st], (x / ST) & 1, &abort_flag)) {
+                const uint32_t r0 = n - (j1 - 1) * KEYS;
+                for (uint32_t i = lane; i < (KEYS - r0) * (HD / 8); i += 32) {
+                    const uint32_t r = r0 + i / (HD / 8), c = i % (HD / 8);
+                    *reinterpret_cast<uint4 *>(ring + st * G::TILE + (c / 8) * (KEYS * 128) + sw128(r, c & 7)) =
+                        make_uint4(0, 0, 0, 0);
+                }
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars.clean);
+            }
+        }
+    } else if (warp < 8) {
+        // ------------------------------------------------------ softmax
+        const uint32_t s = warp >> 2, t = tid & 127;
+        if (s == 0 || two) {
+            // queries: a negative scale goes into their sign, so that the largest score has the largest weight
+            uint8_t *sq = smem + s * G::Q;
+            for (uint32_t i = t; i < 128 * HD / 8; i += 128) {
+                const uint32_t r = i / (HD / 8), c = i % (HD / 8);
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) v[e] = 0.f;
+                if (s * 128 + r < my_rows) {
+                    const uint32_t rr = row0 + s * 128 + r;
+                    const uint32_t tok = first + rr / q.group, head = kvh * q.group + rr % q.group;
+                    load8(reinterpret_cast<const TQ *>(q.q) + (size_t)tok * q.q_stride + (size_t)head * HD + c * 8, v);
+                }
+                if (q.scale < 0.f)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) v[e] = -v[e];
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) split_pack<TC>(v[2 * e], v[2 * e + 1], hi[e], lo[e]);
+                const uint32_t at = (c / 8) * (128 * 128) + sw128(r, c & 7);
+                *reinterpret_cast<uint4 *>(sq + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                if (SPLIT)
+                    *reinterpret_cast<uint4 *>(sq + 128 * HD * 2 + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
+            fence_async_smem();
+            mbar_arrive(&bars.q_full[s]);
+
+            const uint32_t rr = row0 + s * 128 + t;
+            const bool live = s * 128 + t < my_rows;
+            uint32_t lo = 0, hi = 0;
+            if (live) q.range(pos0 + (int)(rr / q.group), n, lo, hi);
+            // a tile inside every row's range needs no mask
+            const uint32_t all_lo = __reduce_max_sync(~0u, live ? lo : 0u);
+            const uint32_t all_hi = __reduce_min_sync(~0u, live ? hi : 0xFFFFFFFFu);
+            const float c2 = fmaxf(fabsf(q.scale) * 1.4426950408889634f, 1e-30f);
+            const float grow = 8.f / c2;
+            const uint32_t lane_base = (warp & 3) << 21;  // this warp's TMEM lanes
+            const uint32_t ts = tmem + s * 128 + lane_base, to = tmem + 256 + s * 128 + lane_base;
+            float m = -INFINITY, l = 0.f;
+            bool ok = true;
+            for (uint32_t j = 0; j < nt; j++) {
+                if (!mbar_wait(&bars.s_full[s], j & 1, &abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                float x[128];
+#pragma unroll
+                for (int i = 0; i < 4; i++) tmem_ld32(ts + i * 32, x + i * 32);
+                tmem_wait_ld();
+                const uint32_t k0 = (j0 + j) * KEYS;
+                if (hole || k0 < all_lo || k0 + KEYS > all_hi) {
+                    uint32_t gone = 0;  // 16-slot units on a hole
+                    if (hole) {
+                        const uint32_t slot = k0 + (lane & 7) * 16;
+                        gone = __ballot_sync(~0u, lane < 8 && slot < n && a.page(b, slot >> a.page_shift) < 0);
+                    }
+                    const int rlo = (int)lo - (int)k0, rhi = (int)hi - (int)k0;
+#pragma unroll
+                    for (int i = 0; i < 128; i++)
+                        if (i < rlo || i >= rhi || ((gone >> (i / 16)) & 1u)) x[i] = -INFINITY;
+                }
+                float mx[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+                for (int i = 4; i < 128; i += 4) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) mx[e] = fmaxf(mx[e], x[i + e]);
+                }
+                const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                const bool up = mt > m + grow || (m == -INFINITY && mt > m);
+                if (__any_sync(~0u, up)) {
+                    const float mn = up ? mt : m;
+                    const float f = up ? ex2((m - mn) * c2) : 1.f;  // 0 from -inf
+                    m = mn;
+                    l *= f;
+                    if (j > 0) {  // O is complete: S was issued behind it
+#pragma unroll 1
+                        for (int i = 0; i < HD / 16; i++) {
+                            float ov[16];
+                            asm volatile(
+                                "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
+                                "%14,%15}, [%16];"
+                                : "=f"(ov[0]), "=f"(ov[1]), "=f"(ov[2]), "=f"(ov[3]), "=f"(ov[4]), "=f"(ov[5]),
+                                  "=f"(ov[6]), "=f"(ov[7]), "=f"(ov[8]), "=f"(ov[9]), "=f"(ov[10]), "=f"(ov[11]),
+                                  "=f"(ov[12]), "=f"(ov[13]), "=f"(ov[14]), "=f"(ov[15])
+                                : "r"(to + i * 16));
+                            tmem_wait_ld();
+                            uint32_t r[16];
+#pragma unroll
+                            for (int e = 0; e < 16; e++) r[e] = __float_as_uint(ov[e] * f);
+                            tmem_st16(to + i * 16, r);
+                        }
+                    }
+                }
+                const float mm = m == -INFINITY ? 0.f : m;
+                const f32x2 cc = pack2(c2, c2), nm = pack2(-mm * c2, -mm * c2);
+                f32x2 sum = pack2(0.f, 0.f);
+#pragma unroll
+                for (int i = 0; i < 128; i += 32) {
+                    uint32_t ph[16], pl[16];
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        float u, v;
+                        unpack2(fma2(pack2(x[i + e], x[i + e + 1]), cc, nm), u, v);
+                        u = ex2(u);
+                        v = ex2(v);
+                        sum = add2(sum, pack2(u, v));
+                        if (SPLIT)
+                            split_pack<TC>(u, v, ph[e / 2], pl[e / 2]);
+                        else
+                            ph[e / 2] = Pair<TC>::pack(u, v);
+                    }
+                    tmem_st16(ts + i / 2, ph);
+                    if (SPLIT) tmem_st16(ts + 64 + i / 2, pl);
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                mbar_arrive(&bars.p_full[s]);
+                float u, v;
+                unpack2(sum, u, v);
+                l += u + v;
+            }
+            // ---------------------------------------------------- output
+            float inv = 0.f, lse2 = -INFINITY;
+            if (nt && ok) {
+                ok = mbar_wait(&bars.o_full[s], 0, &abort_flag);
+                tc_fence_after();
+                inv = l == 0.f ? 0.f : 1.f / l;
+                if (l != 0.f) lse2 = m * c2 + log2f(l);
+            }
+            const uint32_t tok = first + rr / q.group, head = kvh * q.group + rr % q.group;
+            const bool direct = o.plan.many_splits == 1;
+            const size_t prow = ((size_t)split * a.n_tok + tok) * q.heads + head;
+            if (ok) {
+                if (live) {
+                    if (direct && o.lse) o.lse[(size_t)tok * q.heads + head] = lse2 * 0.6931471805599453f;
+                    if (!direct) o.many_lse[prow] = lse2;
+                }
+                if (nt || direct) {
+                    TQ *dst = reinterpret_cast<TQ *>(o.out) + (size_t)tok * o.out_stride + (size_t)head * HD;
+                    float *part = o.many_o + prow * HD;
+#pragma unroll 1
+                    for (int i = 0; i < HD / 32; i++) {
+                        float ov[32];
+                        if (nt) {
+                            tmem_ld32(to + i * 32, ov);
+                            tmem_wait_ld();
+                        }
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8) {
+                            float w[8];
+#pragma unroll
+                            for (int k = 0; k < 8; k++) w[k] = nt ? ov[e + k] * inv : 0.f;
+                            if (live) {
+                                if (direct)
+                                    store8(dst + i * 32 + e, w);
+                                else
+                                    store8(part + i * 32 + e, w);
+                            }
+                        }
+                    }
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (abort_flag) {  // let the copies and products in flight end before the block's memory is given back
+        if (tid == 0) g_timeout = 1;
+        const unsigned long long t0 = now_ns();
+        while (now_ns() - t0 < 1000000ull) {
+        }
+    }
+    if (warp == 8) {
+        tc_fence_after();
+        tmem_free512(tmem);
+    }
+}
+
+template <typename TQ, typename TC, int HD>
+int launch_many(const AttnPagedCall &c, const AttnOut &o, cudaStream_t s) {
+    using G = ManyGeo<HD, std::is_same<TQ, float>::value>;
+    const uint32_t box = c.a.page_size < KEYS ? c.a.page_size : KEYS;
+    CUtensorMap mk, mv;
+    int rc = make_page_map(&mk, c.a.k, c.a, HD, c.cache_type, box);
+    if (rc == CUQ_OK) rc = make_page_map(&mv, c.a.v, c.a, HD, c.cache_type, box);
+    if (rc) return rc;
+    auto kern = attn_many_kernel<TQ, TC, HD>;
+    CUQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM));
+    kern<<<dim3(c.a.kv_heads * o.plan.many_tiles, o.plan.many_splits), NT, G::SMEM, s>>>(c.a, c.q, o, mk, mv);
+    CUQ_CUDA_TRY(cudaGetLastError());
+    return CUQ_OK;
+}
+
+}  // namespace
+
+int launch_attention_many(const AttnPagedCall &c, const AttnOut &o, cudaStream_t s) {
+    if (c.type == CUQ_F32)
+        return c.hd == 64 ? launch_many<float, __half, 64>(c, o, s) : launch_many<float, __half, 128>(c, o, s);
+    if (c.type == CUQ_F16)
+        return c.hd == 64 ? launch_many<__half, __half, 64>(c, o, s) : launch_many<__half, __half, 128>(c, o, s);
+    return c.hd == 64 ? launch_many<__nv_bfloat16, __nv_bfloat16, 64>(c, o, s)
+                      : launch_many<__nv_bfloat16, __nv_bfloat16, 128>(c, o, s);
+}
+
+int attention_many_status(cudaStream_t s, int *timed_out) {
+    CUQ_CUDA_TRY(cudaMemcpyFromSymbolAsync(timed_out, g_timeout, sizeof(int), 0, cudaMemcpyDeviceToHost, s));
+    CUQ_CUDA_TRY(cudaStreamSynchronize(s));
+    if (*timed_out) {
+        const int zero = 0;
+        CUQ_CUDA_TRY(cudaMemcpyToSymbolAsync(g_timeout, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, s));
+        CUQ_CUDA_TRY(cudaStreamSynchronize(s));
+    }
+    return CUQ_OK;
+}
+
+}  // namespace cuq
