@@ -396,8 +396,8 @@ int check_heads(const char *who, const cuq_paged_kv *kv, uint32_t heads) {
     return CUQ_OK;
 }
 
-int check_query(const char *who, const cuq_paged_kv *kv, const void *q, size_t q_stride, int type, uint32_t heads,
-                float scale, int causal, uint32_t window, PagedQuery &out) {
+int check_query(const char *who, const cuq_paged_kv *kv, uint32_t n_tok, const void *q, size_t q_stride, int type,
+                uint32_t heads, float scale, int causal, uint32_t window, PagedQuery &out) {
     int rc = check_heads(who, kv, heads);
     if (rc) return rc;
     if (!(type == kv->type || (type == CUQ_F32 && kv->type == CUQ_F16))) {
@@ -409,6 +409,7 @@ int check_query(const char *who, const cuq_paged_kv *kv, const void *q, size_t q
     CUQ_CHECK_ARG(q_stride % 8 == 0 && q_stride >= (size_t)heads * kv->head_dim,
                   "%s: q_stride %zu (a multiple of 8, at least %zu)", who, q_stride, (size_t)heads * kv->head_dim);
     CUQ_CHECK_ARG(std::isfinite(scale), "%s: scale must be finite", who);
+    CUQ_CHECK_ARG((uint64_t)n_tok * heads <= 0x7FFFFFFFu, "%s: %u tokens of %u heads pass 2^31 rows", who, n_tok, heads);
     CUQ_CHECK_ARG(causal || window == 0, "%s: a window needs a causal mask", who);
     out.q = q;
     out.q_stride = q_stride;
@@ -416,7 +417,7 @@ int check_query(const char *who, const cuq_paged_kv *kv, const void *q, size_t q
     out.group = heads / kv->kv_heads;
     out.scale = scale;
     out.causal = causal ? 1 : 0;
-    out.window = window;
+    out.window = window < (1u << 30) ? window : (1u << 30);  // slots are below 2^30
     return CUQ_OK;
 }
 
@@ -547,7 +548,7 @@ int cuq_attention_paged(const cuq_paged_kv *kv, const cuq_batch *batch, void *ou
     const char *who = "cuq_attention_paged";
     AttnPagedCall c{};
     int rc = check_paged(who, kv, batch, true, c.a);
-    if (rc == CUQ_OK) rc = check_query(who, kv, q, q_stride, type, heads, scale, causal, window, c.q);
+    if (rc == CUQ_OK) rc = check_query(who, kv, batch->n_tok, q, q_stride, type, heads, scale, causal, window, c.q);
     if (rc) return rc;
     CUQ_CHECK_ARG(out && aligned16(out) && out != q, "%s: out must be 16-byte aligned and not q", who);
     CUQ_CHECK_ARG(out_stride % 8 == 0 && out_stride >= (size_t)heads * kv->head_dim,
@@ -577,7 +578,7 @@ int cuq_attention_mass(const cuq_paged_kv *kv, const cuq_batch *batch, float *ma
     const char *who = "cuq_attention_mass";
     MassPagedCall c{};
     int rc = check_paged(who, kv, batch, true, c.a);
-    if (rc == CUQ_OK) rc = check_query(who, kv, q, q_stride, type, heads, scale, causal, window, c.q);
+    if (rc == CUQ_OK) rc = check_query(who, kv, batch->n_tok, q, q_stride, type, heads, scale, causal, window, c.q);
     if (rc) return rc;
     CUQ_CHECK_ARG(mass && lse && aligned4(mass) && aligned4(lse), "%s: mass and lse must be given", who);
     CUQ_CHECK_ARG(mass_stride >= c.a.max_kv, "%s: mass_stride %zu is below max_kv %u", who, mass_stride, c.a.max_kv);
@@ -635,10 +636,11 @@ int cuq_kv_evict(const cuq_paged_kv *kv, const cuq_batch *batch, const float *ma
 
 int cuq_paged_status(void *stream) {
     CUQ_CUDA_TRY(cudaStreamSynchronize((cudaStream_t)stream));
-    int few = 0, many = 0;
+    int few = 0, many = 0, mass = 0;
     int rc = attention_few_status((cudaStream_t)stream, &few);
     if (rc == CUQ_OK) rc = attention_many_status((cudaStream_t)stream, &many);
-    if (rc == CUQ_OK && (few || many)) {
+    if (rc == CUQ_OK) rc = attention_mass_status((cudaStream_t)stream, &mass);
+    if (rc == CUQ_OK && (few || many || mass)) {
         set_error("a wait inside a paged-cache kernel gave up");
         rc = CUQ_ETIMEOUT;
     }

@@ -176,5 +176,6 @@ struct MassPagedCall {
     float decay;
 };
 int launch_attention_mass(const MassPagedCall &c, int sm_count, cudaStream_t s);
+int attention_mass_status(cudaStream_t s, int *timed_out);
 
 }  // namespace cuq

@@ -1,70 +1,493 @@
 // paged_mass.cu -- the attention weight that each cached slot gathers:
 //   mass[b][kv head][s] = decay mass + sum over queries and heads of exp(scale q k_s - lse).
-#include "paged.cuh"
+//
+// With lse known this is a column sum of a softmax, so the product is taken the
+// other way round: S^T = K Q^T on tcgen05, a slot is a TMEM lane and a thread, and
+// the sum over queries stays in that thread's registers: no maximum, no exchange
+// between lanes, no atomics, one fixed order.
+//
+// An item is 256 slots of one KV head of one sequence, two 128-slot streams that
+// share the query tiles (128 (token, head) rows).  Persistent CTAs walk items:
+//   * warp 9 loads K pages by TMA (a ring of two items);
+//   * warps 10-13 gather query rows and their lse into a ring of query tiles; a
+//     tile that the next item uses again stays where it is;
+//   * one lane of warp 8 issues S^T into two TMEM buffers per stream;
+//   * warps 0-3 and 4-7 sum 2^(S c - lse log2 e) over the columns.
+// Few queries: bound by the bytes of K, with only the columns that hold queries
+// computed.  Many: by the exponentials (16 a cycle and SM); then the query tiles of
+// an item are dealt out over a cluster, whose CTAs' sums are joined in rank order
+// through distributed shared memory.
+#include "paged_tc.cuh"
 
 namespace cuq {
 
+using namespace ptc;
+
 namespace {
 
-// One warp per slot; lanes hold HD / 32 dims, one query at a time.
+__device__ int g_timeout;
+
+constexpr int NT = 448;
+constexpr int ITEM = 256;         // slots
+constexpr int MAX_SEQS = 4096;    // sequences of one launch (the item table)
+
+template <int HD, bool SPLIT>
+struct MassGeo {
+    static constexpr int CB = HD / 64;
+    static constexpr int TILE = 128 * HD * 2;
+    static constexpr int Q = TILE * (SPLIT ? 2 : 1);
+    static constexpr int QST = (HD == 128 ? 2 : 4) / (SPLIT ? 2 : 1);
+    static constexpr int SMEM = 1024 + 4 * TILE + QST * Q + MAX_SEQS * 4;
+};
+
+struct MassArgs {
+    PagedArgs a;
+    PagedQuery q;
+    float *mass;
+    size_t mass_stride;
+    const float *lse;
+    uint32_t last_q, seq0, seqs;  // this launch's sequences
+    float decay;
+};
+
+// One item as every role sees it.
+struct Item {
+    uint32_t b, h, k0, n;        // sequence, KV head, first slot, slots of the sequence
+    uint32_t first;              // first token row
+    int pos0;                    // slot of token 0
+    uint32_t i0, tq;             // tokens [i0, tq) count
+    uint32_t qt0, steps;         // first query tile and this CTA's number of them
+};
+
 template <typename TQ, typename TC, int HD>
-__global__ void __launch_bounds__(128) mass_simple(PagedArgs a, PagedQuery q, float *mass, size_t mass_stride,
-                                                   const float *lse, uint32_t last_q, float decay) {
-    constexpr int E = HD / 32;
-    const uint32_t lane = threadIdx.x & 31;
-    const uint32_t kvh = blockIdx.y, b = blockIdx.z;
-    const uint32_t n = a.len(b), s = blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (s >= n) return;
-    uint32_t first;
-    const uint32_t nq = a.tokens(b, first);
-    const uint32_t i1 = min(nq, a.max_q), i0 = (last_q && nq > last_q) ? nq - last_q : 0;
-    const int pg = a.page(b, s >> a.page_shift);
-    float sum = 0.f;
-    if (pg >= 0) {
-        const TC *kr = reinterpret_cast<const TC *>(a.k) + a.row<HD>(pg, kvh, s) + lane * E;
-        float kv[E];
-#pragma unroll
-        for (int e = 0; e < E; e++) kv[e] = (float)kr[e];
-        for (uint32_t i = i0; i < i1; i++) {
-            uint32_t lo, hi;
-            q.range((int)n - (int)nq + (int)i, n, lo, hi);
-            if (s < lo || s >= hi) continue;
-            for (uint32_t g = 0; g < q.group; g++) {
-                const uint32_t tok = first + i, head = kvh * q.group + g;
-                const TQ *qr = reinterpret_cast<const TQ *>(q.q) + (size_t)tok * q.q_stride + (size_t)head * HD +
-                               lane * E;
-                float d = 0.f;
-#pragma unroll
-                for (int e = 0; e < E; e++) d += (float)qr[e] * kv[e];
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(~0u, d, o);
-                sum += __expf(d * q.scale - lse[(size_t)tok * q.heads + head]);
+__global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_constant__ CUtensorMap mk) {
+    constexpr bool SPLIT = std::is_same<TQ, float>::value;
+    using G = MassGeo<HD, SPLIT>;
+    constexpr int QST = G::QST;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t k_full[2], k_empty[2], q_full[QST], q_empty[QST], s_full[2][2], s_empty[2][2];
+    __shared__ float s_lse[QST][128];
+    __shared__ float s_red[ITEM];
+    __shared__ uint32_t s_scan[NT / 32], tmem_slot;
+    __shared__ int abort_flag;
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t *kring = smem, *qring = smem + 4 * G::TILE;
+    uint32_t *s_ends = reinterpret_cast<uint32_t *>(qring + QST * G::Q);  // items of sequences 0..i, per KV head
+    const PagedArgs &a = p.a;
+    const PagedQuery &q = p.q;
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    uint32_t rank, ranks;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
+
+    if (warp == 8) tmem_alloc512(&tmem_slot);
+    if (tid == 0) {
+        abort_flag = 0;
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&k_full[i], 1);
+            mbar_init(&k_empty[i], 1);
+            for (int s = 0; s < 2; s++) {
+                mbar_init(&s_full[s][i], 1);
+                mbar_init(&s_empty[s][i], 128);
             }
         }
+        for (int i = 0; i < QST; i++) {
+            mbar_init(&q_full[i], 128);
+            mbar_init(&q_empty[i], 1 + 256);
+        }
+        mbar_init_fence();
     }
-    if (lane == 0) {
-        float *m = mass + ((size_t)b * a.kv_heads + kvh) * mass_stride + s;
-        *m = decay == 0.f ? sum : decay * *m + sum;
+    // the item table: running sums of ceil(len / 256)
+    uint32_t run = 0;
+    for (uint32_t s0 = 0; s0 < p.seqs; s0 += NT) {
+        const uint32_t i = s0 + tid;
+        uint32_t v = i < p.seqs ? (a.len(p.seq0 + i) + ITEM - 1) / ITEM : 0;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const uint32_t up = __shfl_up_sync(~0u, v, d);
+            if (lane >= (uint32_t)d) v += up;
+        }
+        if (lane == 31) s_scan[warp] = v;
+        __syncthreads();
+        uint32_t before = run;
+        for (uint32_t w = 0; w < NT / 32; w++) {
+            if (w < warp) before += s_scan[w];
+            run += s_scan[w];
+        }
+        if (i < p.seqs) s_ends[i] = before + v;
+        __syncthreads();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    const uint32_t total = run * a.kv_heads;
+    // few queries: neighbouring items, which share their query tile; else dealt out,
+    // since a causal mask gives the first slots the most queries
+    const uint32_t cluster = blockIdx.x / ranks, clusters = gridDim.x / ranks;
+    const uint32_t most = p.last_q ? min(p.last_q, a.max_q) : a.max_q;
+    const bool near = (uint64_t)most * q.group <= 128;
+    const uint32_t per = near ? (total + clusters - 1) / clusters : 1;
+    const uint32_t x0 = cluster * per, x1 = near ? min(total, x0 + per) : total, xs = near ? 1 : clusters;
+
+    auto item = [&](uint32_t x, Item &t) {
+        // sequence-major: find the sequence in the table, then its KV head and slots
+        uint32_t lo = 0, hi = p.seqs - 1;
+        while (lo < hi) {
+            const uint32_t mid = (lo + hi) / 2;
+            if ((uint64_t)s_ends[mid] * a.kv_heads > x)
+                hi = mid;
+            else
+                lo = mid + 1;
+        }
+        const uint32_t base = lo ? s_ends[lo - 1] : 0, cnt = s_ends[lo] - base, y = x - base * a.kv_heads;
+        t.b = p.seq0 + lo;
+        t.h = y / cnt;
+        t.k0 = (y % cnt) * ITEM;
+        t.n = a.len(t.b);
+        const uint32_t nq = a.tokens(t.b, t.first);
+        t.pos0 = (int)t.n - (int)nq;
+        t.tq = min(nq, a.max_q);
+        t.i0 = (p.last_q && nq > p.last_q) ? nq - p.last_q : 0;
+        if (t.pos0 < 0) t.i0 = max(t.i0, (uint32_t)-t.pos0);  // tokens before slot 0 see nothing
+        t.qt0 = t.steps = 0;
+        if (t.i0 < t.tq) {
+            uint32_t ia = t.i0, ib = t.tq;
+            if (q.causal) {
+                ia = (uint32_t)max((int)ia, (int)t.k0 - t.pos0);
+                if (q.window) ib = (uint32_t)max(0ll, min((long long)ib, (long long)t.k0 + ITEM - 1 + q.window - t.pos0));
+            }
+            if (ia < ib) {
+                t.qt0 = (ia - t.i0) * q.group / 128;
+                const uint32_t tiles = ((ib - t.i0) * q.group + 127) / 128 - t.qt0;
+                t.steps = tiles > rank ? (tiles - rank + ranks - 1) / ranks : 0;
+            }
+        }
+    };
+    // rows of query tile qt of item t
+    auto tile_rows = [&](const Item &t, uint32_t qt) { return min(128u, (t.tq - t.i0) * q.group - qt * 128); };
+
+    if (warp == 8) {
+        // ------------------------------------------------------ MMA issuer
+        if (lane == 0) {
+            const uint32_t ka = smem_u32(kring), qa = smem_u32(qring);
+            uint32_t kx = 0, qx = 0, st = 0, ob = ~0u, oh = 0, oq = 0;
+            bool ok = true, held = false;
+            for (uint32_t x = x0; ok && x < x1; x += xs) {
+                Item t;
+                item(x, t);
+                if (!t.steps) continue;
+                ok = mbar_wait(&k_full[kx & 1], (kx >> 1) & 1, &abort_flag);
+                for (uint32_t e = 0; ok && e < t.steps; e++, st++) {
+                    const uint32_t qt = t.qt0 + rank + e * ranks;
+                    if (!held || t.b != ob || t.h != oh || qt != oq) {
+                        if (held) {
+                            umma_commit(&q_empty[qx % QST]);
+                            qx++;
+                        }
+                        held = true;
+                        ob = t.b, oh = t.h, oq = qt;
+                        ok = mbar_wait(&q_full[qx % QST], (qx / QST) & 1, &abort_flag);
+                        if (!ok) break;
+                    }
+                    const uint32_t nr = tile_rows(t, qt), id = idesc<TC>(128, (nr + 31) / 32 * 32, false);
+                    const uint32_t buf = st & 1, qb = qa + (qx % QST) * G::Q;
+                    for (uint32_t s = 0; s < 2; s++) {
+                        if (st >= 2 && !mbar_wait(&s_empty[s][buf], ((st >> 1) - 1) & 1, &abort_flag)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint32_t kb = ka + ((kx & 1) * 2 + s) * G::TILE;
+#pragma unroll
+                        for (int part = 0; part < (SPLIT ? 2 : 1); part++)
+#pragma unroll
+                            for (int ks = 0; ks < HD / 16; ks++) {
+                                const uint32_t off = (ks / 4) * (128 * 128) + (ks % 4) * 32;
+                                umma_ss(tmem + (s * 2 + buf) * 128, sdesc_sw128(kb + off, 16, 1024),
+                                        sdesc_sw128(qb + part * G::TILE + off, 16, 1024), id, part | ks ? 1u : 0u);
+                            }
+                        umma_commit(&s_full[s][buf]);
+                    }
+                }
+                if (ok) umma_commit(&k_empty[kx & 1]);
+                kx++;
+            }
+            if (ok && held) umma_commit(&q_empty[qx % QST]);
+        }
+    } else if (warp == 9) {
+        // ------------------------------------------------------ TMA: K pages
+        const uint32_t box = min(a.page_size, 128u), nbox = ITEM / box;
+        uint32_t kx = 0;
+        bool ok = true;
+        for (uint32_t x = x0; ok && x < x1; x += xs) {
+            Item t;
+            item(x, t);
+            if (!t.steps) continue;
+            const uint32_t st = kx & 1, slot = t.k0 + lane * box;
+            int pg = (int)a.n_pages;  // outside the pool: zeros
+            if (lane < nbox && slot < t.n) {
+                pg = a.page(t.b, slot >> a.page_shift);
+                if (pg < 0) pg = (int)a.n_pages;
+            }
+            if (kx >= 2) ok = mbar_wait(&k_empty[st], ((kx >> 1) - 1) & 1, &abort_flag);
+            if (!ok) break;
+            if (lane == 0) mbar_expect_tx(&k_full[st], 2 * G::TILE);
+            __syncwarp();
+            if (lane < nbox) {
+                const uint32_t row = lane * box;
+                const uint32_t dst = smem_u32(kring) + (st * 2 + row / 128) * G::TILE + (row & 127) * 128;
+#pragma unroll
+                for (int cb = 0; cb < G::CB; cb++)
+                    tma_load_page(dst + cb * (128 * 128), &mk, cb * 64, (int)(slot & (a.page_size - 1)), (int)t.h, pg,
+                                  &k_full[st]);
+            }
+            kx++;
+        }
+        for (uint32_t i = kx > 2 ? kx - 2 : 0; ok && i < kx; i++)  // drain
+            ok = mbar_wait(&k_empty[i & 1], (i >> 1) & 1, &abort_flag);
+    } else if (warp >= 10) {
+        // ------------------------------------------------------ query tiles
+        const uint32_t t128 = tid - 320;
+        uint32_t qx = 0, ob = ~0u, oh = 0, oq = 0;
+        bool ok = true;
+        for (uint32_t x = x0; ok && x < x1; x += xs) {
+            Item t;
+            item(x, t);
+            for (uint32_t e = 0; ok && e < t.steps; e++) {
+                const uint32_t qt = t.qt0 + rank + e * ranks;
+                if (qx && t.b == ob && t.h == oh && qt == oq) continue;
+                ob = t.b, oh = t.h, oq = qt;
+                const uint32_t st = qx % QST, nr = tile_rows(t, qt), r0 = t.i0 * q.group + qt * 128;
+                if (qx >= (uint32_t)QST && !mbar_wait(&q_empty[st], ((qx / QST) - 1) & 1, &abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                // a row that saw nothing counts nothing; its products are kept finite
+                float ls = INFINITY;
+                if (t128 < nr) {
+                    const uint32_t r = r0 + t128;
+                    ls = __ldg(p.lse + (size_t)(t.first + r / q.group) * q.heads + t.h * q.group + r % q.group);
+                    ls = ls == -INFINITY ? INFINITY : ls * 1.4426950408889634f;
+                }
+                s_lse[st][t128] = ls;
+                uint8_t *dst = qring + st * G::Q;
+                constexpr int CH = HD / 8;
+#pragma unroll 4
+                for (uint32_t i = t128; i < 128 * CH; i += 128) {
+                    const uint32_t r = i / CH, c = i % CH;
+                    const uint32_t at = (c / 8) * (128 * 128) + sw128(r, c & 7);
+                    const uint32_t rr = r0 + r, tok = t.first + rr / q.group, head = t.h * q.group + rr % q.group;
+                    const bool live =
+                        r < nr && __ldg(p.lse + (size_t)tok * q.heads + head) != -INFINITY;
+                    const TQ *src = reinterpret_cast<const TQ *>(q.q) + (size_t)tok * q.q_stride + (size_t)head * HD + c * 8;
+                    if (SPLIT) {
+                        float v[8];
+#pragma unroll
+                        for (int k = 0; k < 8; k++) v[k] = 0.f;
+                        if (live) load8(src, v);
+                        uint32_t hi[4], lo[4];
+#pragma unroll
+                        for (int k = 0; k < 4; k++) split_pack<TC>(v[2 * k], v[2 * k + 1], hi[k], lo[k]);
+                        *reinterpret_cast<uint4 *>(dst + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        *reinterpret_cast<uint4 *>(dst + G::TILE + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    } else {
+                        uint4 v = make_uint4(0, 0, 0, 0);
+                        if (live) v = __ldg(reinterpret_cast<const uint4 *>(src));
+                        *reinterpret_cast<uint4 *>(dst + at) = v;
+                    }
+                }
+                fence_async_smem();
+                mbar_arrive(&q_full[st]);
+                qx++;
+            }
+        }
+        for (uint32_t i = qx > (uint32_t)QST ? qx - QST : 0; ok && i < qx; i++)  // drain
+            ok = mbar_wait(&q_empty[i % QST], (i / QST) & 1, &abort_flag);
+    } else {
+        // ------------------------------------------------------ column sums
+        const uint32_t s = warp >> 2, t128 = tid & 127;
+        const uint32_t ts = tmem + s * 256 + ((warp & 3) << 21);
+        const float c2 = q.scale * 1.4426950408889634f;
+        const f32x2 cc = pack2(c2, c2);
+        uint32_t qx = 0, st = 0, ob = ~0u, oh = 0, oq = 0;
+        bool ok = true, held = false;
+        for (uint32_t x = x0; ok && x < x1; x += xs) {
+            Item t;
+            item(x, t);
+            const uint32_t k = t.k0 + s * 128 + t128;       // this thread's slot
+            const uint32_t kw = k - lane;                   // its warp's first
+            float sum = 0.f;
+            for (uint32_t e = 0; e < t.steps; e++, st++) {
+                const uint32_t qt = t.qt0 + rank + e * ranks;
+                if (!held || t.b != ob || t.h != oh || qt != oq) {
+                    if (held) {
+                        mbar_arrive(&q_empty[qx % QST]);
+                        qx++;
+                    }
+                    held = true;
+                    ob = t.b, oh = t.h, oq = qt;
+                    ok = mbar_wait(&q_full[qx % QST], (qx / QST) & 1, &abort_flag);
+                    if (!ok) break;
+                }
+                const uint32_t buf = st & 1, nr = tile_rows(t, qt), r0 = t.i0 * q.group + qt * 128;
+                ok = mbar_wait(&s_full[s][buf], (st >> 1) & 1, &abort_flag);
+                if (!ok) break;
+                tc_fence_after();
+                // columns [clo, chi) see slot k; the warp's slots are kw .. kw + 31
+                int clo = 0, chi = (int)nr;
+                bool masked = false;
+                if (q.causal) {
+                    auto col = [&](long long i) {  // token i's first column, cut to the tile
+                        const long long v = i * q.group - (long long)r0;
+                        return (int)max(0ll, min((long long)nr, v));
+                    };
+                    clo = col((long long)k - t.pos0);
+                    masked = col((long long)kw + 31 - t.pos0) > 0;
+                    if (q.window) {
+                        chi = col((long long)k + q.window - t.pos0);
+                        masked |= col((long long)kw + q.window - t.pos0) < (int)nr;
+                    }
+                }
+                const float *ls = s_lse[qx % QST];
+                f32x2 acc = pack2(0.f, 0.f);
+                for (uint32_t c0 = 0; c0 < nr; c0 += 32) {
+                    float v[32];
+                    tmem_ld32(ts + buf * 128 + c0, v);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        const float4 l4 = *reinterpret_cast<const float4 *>(ls + c0 + i);
+                        float u0, u1, u2, u3;
+                        unpack2(fma2(pack2(v[i], v[i + 1]), cc, pack2(-l4.x, -l4.y)), u0, u1);
+                        unpack2(fma2(pack2(v[i + 2], v[i + 3]), cc, pack2(-l4.z, -l4.w)), u2, u3);
+                        if (masked) {
+                            const int c = (int)c0 + i;
+                            u0 = (c >= clo && c < chi) ? u0 : -INFINITY;
+                            u1 = (c + 1 >= clo && c + 1 < chi) ? u1 : -INFINITY;
+                            u2 = (c + 2 >= clo && c + 2 < chi) ? u2 : -INFINITY;
+                            u3 = (c + 3 >= clo && c + 3 < chi) ? u3 : -INFINITY;
+                        }
+                        acc = add2(acc, pack2(ex2(u0), ex2(u1)));
+                        acc = add2(acc, pack2(ex2(u2), ex2(u3)));
+                    }
+                }
+                tc_fence_before();
+                mbar_arrive(&s_empty[s][buf]);
+                float u, v;
+                unpack2(acc, u, v);
+                sum += u + v;
+            }
+            if (ok && k < t.n) {
+                if (a.page(t.b, k >> a.page_shift) < 0) sum = 0.f;  // a hole gathers nothing
+                if (ranks == 1) {
+                    float *m = p.mass + ((size_t)t.b * a.kv_heads + t.h) * p.mass_stride + k;
+                    *m = p.decay == 0.f ? sum : p.decay * *m + sum;
+                }
+            }
+            if (ranks > 1) s_red[s * 128 + t128] = sum;
+        }
+        if (ok && held) mbar_arrive(&q_empty[qx % QST]);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (abort_flag) {
+        if (tid == 0) g_timeout = 1;
+        const unsigned long long t0 = now_ns();
+        while (now_ns() - t0 < 1000000ull) {
+        }
+    }
+    if (warp == 8) {
+        tc_fence_after();
+        tmem_free512(tmem);
+    }
+    if (ranks > 1) {  // one item per cluster: rank 0 joins the sums in rank order
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (rank == 0 && tid < ITEM && x0 < x1) {
+            Item t;
+            item(x0, t);
+            const uint32_t k = t.k0 + tid;
+            float sum = 0.f;
+            for (uint32_t r = 0; r < ranks; r++) {
+                uint32_t at;
+                float v;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(&s_red[tid])), "r"(r));
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+                sum += v;
+            }
+            if (k < t.n) {
+                float *m = p.mass + ((size_t)t.b * a.kv_heads + t.h) * p.mass_stride + k;
+                *m = p.decay == 0.f ? sum : p.decay * *m + sum;
+            }
+        }
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
 }
 
-template <typename TQ, typename TC>
-int launch_simple(const MassPagedCall &c, cudaStream_t s) {
-    const dim3 grid((c.a.max_kv + 3) / 4, c.a.kv_heads, c.a.n_seqs);
-    if (c.hd == 64)
-        mass_simple<TQ, TC, 64><<<grid, 128, 0, s>>>(c.a, c.q, c.mass, c.mass_stride, c.lse, c.last_q, c.decay);
-    else
-        mass_simple<TQ, TC, 128><<<grid, 128, 0, s>>>(c.a, c.q, c.mass, c.mass_stride, c.lse, c.last_q, c.decay);
-    CUQ_CUDA_TRY(cudaGetLastError());
+template <typename TQ, typename TC, int HD>
+int launch_mass(const MassPagedCall &c, int sm_count, cudaStream_t s) {
+    using G = MassGeo<HD, std::is_same<TQ, float>::value>;
+    CUtensorMap mk;
+    int rc = make_page_map(&mk, c.a.k, c.a, HD, c.cache_type, c.a.page_size < 128 ? c.a.page_size : 128);
+    if (rc) return rc;
+    auto kern = mass_kernel<TQ, TC, HD>;
+    CUQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM));
+    MassArgs p{};
+    p.a = c.a;
+    p.q = c.q;
+    p.mass = c.mass;
+    p.mass_stride = c.mass_stride;
+    p.lse = c.lse;
+    p.last_q = c.last_q;
+    p.decay = c.decay;
+    const uint64_t tokens = c.last_q && c.last_q < c.a.max_q ? c.last_q : c.a.max_q;
+    const uint64_t tiles = (tokens * c.q.group + 127) / 128;
+    for (uint32_t seq0 = 0; seq0 < c.a.n_seqs; seq0 += MAX_SEQS) {
+        p.seq0 = seq0;
+        p.seqs = c.a.n_seqs - seq0 < (uint32_t)MAX_SEQS ? c.a.n_seqs - seq0 : (uint32_t)MAX_SEQS;
+        const uint64_t items = (uint64_t)p.seqs * c.a.kv_heads * ((c.a.max_kv + ITEM - 1) / ITEM);
+        uint32_t ranks = 1;
+        while (ranks < 8 && ranks * 2 <= tiles && items * ranks * 2 <= (uint64_t)sm_count) ranks *= 2;
+        const uint64_t want = items * ranks;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)(ranks > 1 || want < (uint64_t)sm_count ? want : (uint64_t)sm_count));
+        cfg.blockDim = dim3(NT);
+        cfg.dynamicSmemBytes = G::SMEM;
+        cfg.stream = s;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = ranks;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        CUQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, p, mk));
+    }
     return CUQ_OK;
 }
 
 }  // namespace
 
-int launch_attention_mass(const MassPagedCall &c, int, cudaStream_t s) {
-    if (c.type == CUQ_F32) return launch_simple<float, __half>(c, s);
-    if (c.type == CUQ_F16) return launch_simple<__half, __half>(c, s);
-    return launch_simple<__nv_bfloat16, __nv_bfloat16>(c, s);
+int launch_attention_mass(const MassPagedCall &c, int sm_count, cudaStream_t s) {
+    if (c.type == CUQ_F32)
+        return c.hd == 64 ? launch_mass<float, __half, 64>(c, sm_count, s) : launch_mass<float, __half, 128>(c, sm_count, s);
+    if (c.type == CUQ_F16)
+        return c.hd == 64 ? launch_mass<__half, __half, 64>(c, sm_count, s)
+                          : launch_mass<__half, __half, 128>(c, sm_count, s);
+    return c.hd == 64 ? launch_mass<__nv_bfloat16, __nv_bfloat16, 64>(c, sm_count, s)
+                      : launch_mass<__nv_bfloat16, __nv_bfloat16, 128>(c, sm_count, s);
+}
+
+int attention_mass_status(cudaStream_t s, int *timed_out) {
+    CUQ_CUDA_TRY(cudaMemcpyFromSymbolAsync(timed_out, g_timeout, sizeof(int), 0, cudaMemcpyDeviceToHost, s));
+    CUQ_CUDA_TRY(cudaStreamSynchronize(s));
+    if (*timed_out) {
+        const int zero = 0;
+        CUQ_CUDA_TRY(cudaMemcpyToSymbolAsync(g_timeout, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, s));
+        CUQ_CUDA_TRY(cudaStreamSynchronize(s));
+    }
+    return CUQ_OK;
 }
 
 }  // namespace cuq
