@@ -174,12 +174,14 @@ int launch_rope_append(const RopeArgs &p, const RopeTable &t, int out_type, int 
 
 // ------------------------------------------------------- eviction ----
 //
-// Selection: one CTA per (sequence, KV head).  Masses become 32-bit keys in
-// their order (NaN lowest); four 8-bit histogram passes find the key of the
-// last slot kept and how many of its equals are kept; one ordered pass then
-// writes the kept slots by prefix sums.  The order of the histogram's atomics
-// does not matter: they count whole numbers.
-constexpr int SEL_THREADS = 1024;
+// Selection, bound by latency: a cluster of CTAs takes one (sequence, KV head),
+// each a contiguous slice of its slots.  Masses become 32-bit keys in their order
+// (NaN lowest).  Three histogram passes (11, 11, 10 bits) find the key of the last
+// slot kept and how many of its equals are kept; every CTA counts its own slice and
+// adds the bins it hit into rank 0's through distributed shared memory, whose scan
+// tells all the digit.  A last pass writes the kept slots at their prefix sums.
+// Histogram atomics count whole numbers, so their order does not matter.
+constexpr int SEL_THREADS = 512, SEL_BINS = 2048, SEL_PER = 4;
 
 __device__ __forceinline__ uint32_t mass_key(float m) {
     if (m != m) return 0u;
@@ -197,141 +199,309 @@ struct EvictArgs {
     size_t mass_out_stride;
 };
 
-__global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(EvictArgs p) {
-    __shared__ uint32_t hist[256];
-    __shared__ uint32_t s_prefix, s_need, warp_sum[33];
-    const uint32_t b = blockIdx.x / p.a.kv_heads, h = blockIdx.x % p.a.kv_heads;
-    const uint32_t n = p.a.len(b), kept_n = min(n, p.keep);
-    const float *mass = p.mass + ((size_t)b * p.a.kv_heads + h) * p.mass_stride;
-    int32_t *kept = p.kept + ((size_t)b * p.a.kv_heads + h) * p.keep;
-    float *mass_out = p.mass_out ? p.mass_out + ((size_t)b * p.a.kv_heads + h) * p.mass_out_stride : nullptr;
-    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (h == 0 && tid == 0) p.new_len[b] = (int32_t)kept_n;
-    if (n <= p.keep) {
-        for (uint32_t i = tid; i < p.keep; i += SEL_THREADS) kept[i] = i < n ? (int32_t)i : -1;
-        if (mass_out && mass_out != mass)
-            for (uint32_t i = tid; i < n; i += SEL_THREADS) mass_out[i] = mass[i];
-        return;
-    }
-    // the slots in between, of which `need` are kept
-    const uint32_t lo = p.sink, hi = n - p.recent;
-    if (tid == 0) {
-        s_prefix = 0;
-        s_need = p.keep - p.sink - p.recent;
-    }
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
-        __syncthreads();
-        const uint32_t prefix = s_prefix, need = s_need;
-        for (uint32_t i = lo + tid; i < hi; i += SEL_THREADS) {
-            const uint32_t key = mass_key(mass[i]);
-            if (shift == 24 || (key >> (shift + 8)) == prefix) atomicAdd(&hist[(key >> shift) & 255u], 1u);
-        }
-        __syncthreads();
-        if (tid == 0) {  // the bin, from the top, in which the need-th key lies
-            uint32_t above = 0;
-            int bin = 255;
-            for (; bin > 0 && above + hist[bin] < need; bin--) above += hist[bin];
-            s_prefix = (prefix << 8) | (uint32_t)bin;
-            s_need = need - above;
-        }
-        __syncthreads();
-    }
-    const uint32_t edge = s_prefix, equals = s_need;  // keep keys above edge, and the first `equals` equal to it
-    // ordered pass: tiles of SEL_THREADS slots, running counts of kept and of equals
-    uint32_t out_base = 0, eq_base = 0;
-    for (uint32_t t0 = 0; t0 < n; t0 += SEL_THREADS) {
-        const uint32_t i = t0 + tid;
-        const float m = i < n ? mass[i] : 0.f;
-        const bool forced = i < n && (i < lo || i >= hi);
-        const uint32_t key = (i < n && !forced) ? mass_key(m) : 0u;
-        const bool above = i < n && !forced && key > edge, equal = i < n && !forced && key == edge;
-        // exclusive rank of this slot among the tile's equals, then among its kept
-        const uint32_t be = __ballot_sync(~0u, equal);
-        if (lane == 0) warp_sum[warp] = __popc(be);
-        __syncthreads();
-        uint32_t eq_before = 0, eq_total = 0;
-        for (int w = 0; w < SEL_THREADS / 32; w++) {
-            if (w < (int)warp) eq_before += warp_sum[w];
-            eq_total += warp_sum[w];
-        }
-        const uint32_t rank = eq_base + eq_before + __popc(be & ((1u << lane) - 1u));
-        const bool take = forced || above || (equal && rank < equals);
-        const uint32_t bt = __ballot_sync(~0u, take);
-        __syncthreads();
-        if (lane == 0) warp_sum[warp] = __popc(bt);
-        __syncthreads();
-        uint32_t before = 0, total = 0;
-        for (int w = 0; w < SEL_THREADS / 32; w++) {
-            if (w < (int)warp) before += warp_sum[w];
-            total += warp_sum[w];
-        }
-        const uint32_t at = out_base + before + __popc(bt & ((1u << lane) - 1u));
-        // in place: at <= i, so the slots this tile writes have been read
-        if (take && at < p.keep) {
-            kept[at] = (int32_t)i;
-            if (mass_out) mass_out[at] = m;
-        }
-        out_base += total;
-        eq_base += eq_total;
-        __syncthreads();
-    }
-    if (mass_out)
-        for (uint32_t i = kept_n + tid; i < n; i += SEL_THREADS) mass_out[i] = 0.f;
+__device__ __forceinline__ uint32_t peer_smem(const void *p, uint32_t rank) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+                 : "=r"(at)
+                 : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    return at;
+}
+__device__ __forceinline__ void peer_add(uint32_t at, uint32_t v) {
+    asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
+}
+__device__ __forceinline__ void peer_store(uint32_t at, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// Compaction, in place: a CTA owns one slice of SLICE bytes of every row of one
-// (sequence, KV head, pool), so no other CTA reads or writes what it does.  New
-// slot j takes old slot kept[j] >= j, in order: a chunk of rows is read whole
-// before it is written, and no later chunk reads what an earlier one wrote.
-constexpr int MOVE_THREADS = 256;
-constexpr int MOVE_VECS = 8;  // 16-byte vectors per thread in one chunk
-
-template <int HD, int SLICE>
-__global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(EvictArgs p) {
-    constexpr uint32_t VPR = SLICE / 16;                               // vectors per row
-    constexpr uint32_t ROWS = MOVE_THREADS * MOVE_VECS / VPR;          // rows per chunk
-    constexpr uint32_t SLICES = HD * 2 / SLICE;
-    uint32_t x = blockIdx.x;
-    const uint32_t slice = x % SLICES;
-    x /= SLICES;
-    const bool is_v = x & 1;
-    x >>= 1;
-    const uint32_t h = x % p.a.kv_heads, b = x / p.a.kv_heads;
-    const uint32_t n = p.a.len(b);
-    if (n <= p.keep) return;  // every slot stays where it is
-    const int32_t *kept = p.kept + ((size_t)b * p.a.kv_heads + h) * p.keep;
-    uint8_t *pool = reinterpret_cast<uint8_t *>(is_v ? p.a.v : p.a.k);
-    const uint32_t v = threadIdx.x % VPR, r0 = threadIdx.x / VPR;
-    for (uint32_t c = 0; c < p.keep; c += ROWS) {
-        uint4 val[MOVE_VECS];
-        bool ok[MOVE_VECS];
+__global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(EvictArgs p) {
+    __shared__ uint32_t hist[SEL_BINS];  // this slice's counts
+    __shared__ uint32_t sums[SEL_BINS];  // rank 0: the cluster's
+    __shared__ uint32_t s_digit, s_need, s_above[16], s_equal[16], warp_a[SEL_THREADS / 32], warp_e[SEL_THREADS / 32];
+    uint32_t rank, ranks;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
+    const uint32_t x = blockIdx.x / ranks, b = x / p.a.kv_heads, h = x % p.a.kv_heads;
+    const uint32_t n = p.a.len(b), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const float *mass = p.mass + ((size_t)b * p.a.kv_heads + h) * p.mass_stride;
+    int32_t *kept = p.kept + ((size_t)b * p.a.kv_heads + h) * p.keep;
+    if (h == 0 && rank == 0 && tid == 0) p.new_len[b] = (int32_t)min(n, p.keep);
+    if (n <= p.keep) {  // the same for the whole cluster
+        for (uint32_t i = rank * SEL_THREADS + tid; i < p.keep; i += ranks * SEL_THREADS)
+            kept[i] = i < n ? (int32_t)i : -1;
+        return;
+    }
+    // the slots in between, of which `need` are kept, and this CTA's slice of all slots
+    const uint32_t lo = p.sink, hi = n - p.recent;
+    const uint32_t per = (n + ranks - 1) / ranks, i0 = min(n, rank * per), i1 = min(n, i0 + per);
+    const uint32_t m0 = max(i0, lo), m1 = min(i1, hi);
+    uint32_t need = p.keep - p.sink - p.recent, prefix = 0;
+    constexpr int SHIFT[3] = {21, 10, 0}, BITS[3] = {11, 11, 10};
 #pragma unroll
-        for (int i = 0; i < MOVE_VECS; i++) {
-            const uint32_t j = c + r0 + i * (MOVE_THREADS / VPR);
-            ok[i] = false;
-            if (j < p.keep) {
-                const uint32_t src = (uint32_t)kept[j];
-                if (src != j && src < n) {
-                    const int pg = p.a.page(b, src >> p.a.page_shift);
-                    ok[i] = pg >= 0;
-                    if (ok[i])
-                        val[i] = *reinterpret_cast<const uint4 *>(pool + p.a.row<HD>(pg, h, src) * 2 + slice * SLICE +
-                                                                  v * 16);
-                }
+    for (int pass = 0; pass < 3; pass++) {
+        if (need == 0) break;  // nothing in between is kept
+        const int shift = SHIFT[pass], bins = 1 << BITS[pass];
+        for (uint32_t i = tid; i < SEL_BINS; i += SEL_THREADS) hist[i] = sums[i] = 0;
+        if (ranks > 1)
+            cluster_sync();  // rank 0's sums are clear
+        else
+            __syncthreads();
+        for (uint32_t i = m0 + tid; i < m1; i += SEL_THREADS * SEL_PER) {
+            float m[SEL_PER];
+#pragma unroll
+            for (int e = 0; e < SEL_PER; e++) m[e] = i + e * SEL_THREADS < m1 ? __ldg(mass + i + e * SEL_THREADS) : 0.f;
+#pragma unroll
+            for (int e = 0; e < SEL_PER; e++) {
+                const uint32_t key = mass_key(m[e]);
+                if (i + e * SEL_THREADS < m1 && (pass == 0 || (key >> (shift + BITS[pass])) == prefix))
+                    atomicAdd(&hist[(key >> shift) & (bins - 1)], 1u);
             }
         }
         __syncthreads();
+        if (ranks > 1) {
+            for (uint32_t i = tid; i < (uint32_t)bins; i += SEL_THREADS)
+                if (hist[i]) peer_add(peer_smem(&sums[i], 0), hist[i]);
+            cluster_sync();
+        }
+        if (rank == 0) {  // the bin, from the top, in which the need-th key lies
+            const uint32_t *c = ranks > 1 ? sums : hist;
+            constexpr int PER = SEL_BINS / SEL_THREADS;
+            uint32_t v[PER], own = 0;  // thread t: bins [bins - PER (t + 1), bins - PER t), from the top
 #pragma unroll
-        for (int i = 0; i < MOVE_VECS; i++) {
-            const uint32_t j = c + r0 + i * (MOVE_THREADS / VPR);
-            if (!ok[i]) continue;
-            const int pg = p.a.page(b, j >> p.a.page_shift);
-            if (pg >= 0)
-                *reinterpret_cast<uint4 *>(pool + p.a.row<HD>(pg, h, j) * 2 + slice * SLICE + v * 16) = val[i];
+            for (int e = 0; e < PER; e++) {
+                const int bin = bins - 1 - (int)(tid * PER) - e;
+                v[e] = bin >= 0 ? c[bin] : 0u;
+                own += v[e];
+            }
+            uint32_t incl = own;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const uint32_t up = __shfl_up_sync(~0u, incl, d);
+                if (lane >= (uint32_t)d) incl += up;
+            }
+            if (lane == 31) warp_a[warp] = incl;
+            __syncthreads();
+            uint32_t above = incl - own;
+            for (uint32_t w = 0; w < warp; w++) above += warp_a[w];
+#pragma unroll
+            for (int e = 0; e < PER; e++) {
+                if (above < need && above + v[e] >= need) {  // one thread only (need > 0)
+                    const uint32_t bin = (uint32_t)(bins - 1 - (int)(tid * PER) - e);
+                    for (uint32_t r = 0; r < ranks; r++) {
+                        peer_store(peer_smem(&s_digit, r), bin);
+                        peer_store(peer_smem(&s_need, r), need - above);
+                    }
+                }
+                above += v[e];
+            }
+        }
+        if (ranks > 1)
+            cluster_sync();
+        else
+            __syncthreads();
+        prefix = (prefix << BITS[pass]) | s_digit;
+        need = s_need;
+    }
+    // kept: keys above `prefix`, and the first `need` equal to it.  The key 2^32 - 1
+    // stands for "none" when nothing in between is kept (no float has it).
+    const uint32_t edge = need == 0 ? 0xFFFFFFFFu : prefix;
+    auto kind = [&](uint32_t i, float m, uint32_t &above, uint32_t &equal) {
+        const bool forced = i < lo || i >= hi;
+        const uint32_t key = mass_key(m);
+        above = forced || key > edge;
+        equal = !forced && key == edge;
+    };
+    uint32_t ca = 0, ce = 0;
+    for (uint32_t i = i0 + tid; i < i1; i += SEL_THREADS * SEL_PER) {
+        float m[SEL_PER];
+#pragma unroll
+        for (int e = 0; e < SEL_PER; e++) m[e] = i + e * SEL_THREADS < i1 ? __ldg(mass + i + e * SEL_THREADS) : 0.f;
+#pragma unroll
+        for (int e = 0; e < SEL_PER; e++) {
+            uint32_t u = 0, v = 0;
+            if (i + e * SEL_THREADS < i1) kind(i + e * SEL_THREADS, m[e], u, v);
+            ca += u;
+            ce += v;
+        }
+    }
+    ca = __reduce_add_sync(~0u, ca);
+    ce = __reduce_add_sync(~0u, ce);
+    __syncthreads();
+    if (lane == 0) warp_a[warp] = ca, warp_e[warp] = ce;
+    __syncthreads();
+    if (tid == 0) {
+        uint32_t u = 0, v = 0;
+        for (int w = 0; w < SEL_THREADS / 32; w++) u += warp_a[w], v += warp_e[w];
+        for (uint32_t r = 0; r < ranks; r++) {
+            peer_store(peer_smem(&s_above[rank], r), u);
+            peer_store(peer_smem(&s_equal[rank], r), v);
+        }
+    }
+    if (ranks > 1)
+        cluster_sync();
+    else
+        __syncthreads();
+    uint32_t base_a = 0, base_e = 0;
+    for (uint32_t r = 0; r < rank; r++) base_a += s_above[r], base_e += s_equal[r];
+    // output: tiles of SEL_PER neighbouring slots a thread
+    for (uint32_t t0 = i0; t0 < i1; t0 += SEL_THREADS * SEL_PER) {
+        const uint32_t i = t0 + tid * SEL_PER;
+        uint32_t u[SEL_PER], v[SEL_PER], na = 0, ne = 0;
+#pragma unroll
+        for (int e = 0; e < SEL_PER; e++) {
+            u[e] = v[e] = 0;
+            if (i + e < i1) kind(i + e, __ldg(mass + i + e), u[e], v[e]);
+            na += u[e];
+            ne += v[e];
+        }
+        uint32_t ia = na, ie = ne;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const uint32_t ua = __shfl_up_sync(~0u, ia, d), ue = __shfl_up_sync(~0u, ie, d);
+            if (lane >= (uint32_t)d) ia += ua, ie += ue;
         }
         __syncthreads();
+        if (lane == 31) warp_a[warp] = ia, warp_e[warp] = ie;
+        __syncthreads();
+        uint32_t at_a = base_a + ia - na, at_e = base_e + ie - ne;
+        for (uint32_t w = 0; w < SEL_THREADS / 32; w++) {
+            if (w < warp) at_a += warp_a[w], at_e += warp_e[w];
+            base_a += warp_a[w];
+            base_e += warp_e[w];
+        }
+#pragma unroll
+        for (int e = 0; e < SEL_PER; e++) {
+            if (u[e] || (v[e] && at_e < need)) {
+                const uint32_t at = at_a + min(at_e, need);
+                if (at < p.keep) kept[at] = (int32_t)(i + e);
+            }
+            at_a += u[e];
+            at_e += v[e];
+        }
     }
+}
+
+// Compaction, in place: a CTA owns one slice of SLICE bytes of every row of one
+// (sequence, KV head, pool), so no other CTA reads or writes what it does; one CTA
+// more per (sequence, KV head) moves the mass.  New slot j takes old slot kept[j] >=
+// j, in order: a chunk of rows is read whole before it is written, and no later
+// chunk reads what an earlier one wrote, so the next chunk's reads are under way
+// while this one is written.
+constexpr int MOVE_THREADS = 256;
+constexpr int MOVE_VECS = 8;  // vectors per thread in one chunk
+
+template <int HD, int SLICE>
+__global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(EvictArgs p) {
+    constexpr uint32_t VPR = SLICE / 16;                      // vectors per row
+    constexpr uint32_t ROWS = MOVE_THREADS * MOVE_VECS / VPR;  // rows per chunk
+    constexpr uint32_t SLICES = HD * 2 / SLICE, STEP = MOVE_THREADS / VPR;
+    griddep_wait();
+    uint32_t x = blockIdx.x;
+    const uint32_t part = x % (2 * SLICES + 1);
+    x /= 2 * SLICES + 1;
+    const uint32_t h = x % p.a.kv_heads, b = x / p.a.kv_heads;
+    const uint32_t n = p.a.len(b);
+    const int32_t *kept = p.kept + ((size_t)b * p.a.kv_heads + h) * p.keep;
+    if (part == 2 * SLICES) {
+        if (!p.mass_out) return;
+        const float *src = p.mass + ((size_t)b * p.a.kv_heads + h) * p.mass_stride;
+        float *dst = p.mass_out + ((size_t)b * p.a.kv_heads + h) * p.mass_out_stride;
+        const uint32_t live = min(n, p.keep);
+        for (uint32_t c = 0; c < live; c += MOVE_THREADS * MOVE_VECS) {
+            float v[MOVE_VECS];
+#pragma unroll
+            for (int i = 0; i < MOVE_VECS; i++) {
+                const uint32_t j = c + i * MOVE_THREADS + threadIdx.x;
+                v[i] = j < live ? src[kept[j]] : 0.f;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < MOVE_VECS; i++) {
+                const uint32_t j = c + i * MOVE_THREADS + threadIdx.x;
+                if (j < live) dst[j] = v[i];
+            }
+            __syncthreads();
+        }
+        for (uint32_t i = live + threadIdx.x; i < n; i += MOVE_THREADS) dst[i] = 0.f;
+        return;
+    }
+    if (n <= p.keep) return;  // every slot stays where it is
+    const bool is_v = part >= SLICES;
+    uint8_t *pool = reinterpret_cast<uint8_t *>(is_v ? p.a.v : p.a.k) + (part % SLICES) * SLICE;
+    const uint32_t r0 = threadIdx.x / VPR, off = (threadIdx.x % VPR) * 16;
+    uint4 val[MOVE_VECS];
+    uint32_t ok = 0;  // a bit for each vector that moves
+    auto read = [&](uint32_t c) {
+        uint32_t src[MOVE_VECS];
+        int pg[MOVE_VECS];
+#pragma unroll
+        for (int i = 0; i < MOVE_VECS; i++) {
+            const uint32_t j = c + r0 + i * STEP;
+            src[i] = j < p.keep ? (uint32_t)__ldg(kept + j) : j;
+            if (src[i] >= n) src[i] = j;
+        }
+#pragma unroll
+        for (int i = 0; i < MOVE_VECS; i++)
+            pg[i] = src[i] != c + r0 + i * STEP ? p.a.page(b, src[i] >> p.a.page_shift) : -1;
+        ok = 0;
+#pragma unroll
+        for (int i = 0; i < MOVE_VECS; i++)
+            if (pg[i] >= 0) {
+                ok |= 1u << i;
+                val[i] = *reinterpret_cast<const uint4 *>(pool + p.a.row<HD>(pg[i], h, src[i]) * 2 + off);
+            }
+    };
+    read(0);
+    for (uint32_t c = 0; c < p.keep; c += ROWS) {
+        uint4 out[MOVE_VECS];
+        const uint32_t move = ok;
+#pragma unroll
+        for (int i = 0; i < MOVE_VECS; i++) out[i] = val[i];
+        __syncthreads();  // chunk c is read by every thread
+        if (c + ROWS < p.keep) read(c + ROWS);
+#pragma unroll
+        for (int i = 0; i < MOVE_VECS; i++) {
+            const uint32_t j = c + r0 + i * STEP;
+            if (!((move >> i) & 1u)) continue;
+            const int pg = p.a.page(b, j >> p.a.page_shift);
+            if (pg >= 0) *reinterpret_cast<uint4 *>(pool + p.a.row<HD>(pg, h, j) * 2 + off) = out[i];
+        }
+    }
+}
+
+int launch_evict(const EvictArgs &p, uint32_t hd, int sm_count, cudaStream_t s) {
+    const uint32_t rows = p.a.n_seqs * p.a.kv_heads;
+    // a slice of 4096 slots a CTA keeps its passes short; clusters of up to 8
+    uint32_t ranks = 1;
+    while (ranks < 8 && (uint64_t)ranks * 4096 < p.a.max_kv && (uint64_t)rows * ranks * 2 <= 4u * sm_count) ranks *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(rows * ranks);
+    cfg.blockDim = dim3(SEL_THREADS);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ranks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    CUQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, evict_select_kernel, p));
+    if (p.a.max_kv <= p.keep && !p.mass_out) return CUQ_OK;  // nothing can move
+    // slices of 32 bytes (a DRAM sector) while that leaves SMs idle otherwise, else of 64
+    const bool wide = (uint64_t)rows * (2 * (hd * 2 / 32)) > 4u * (uint64_t)sm_count;
+    const uint32_t parts = 2 * (hd * 2 / (wide ? 64 : 32)) + 1;
+    const dim3 grid(rows * parts), block(MOVE_THREADS);
+    cudaError_t e;
+    if (hd == 64)
+        e = wide ? launch_maybe_pdl(evict_move_kernel<64, 64>, grid, block, 0, s, true, p)
+                 : launch_maybe_pdl(evict_move_kernel<64, 32>, grid, block, 0, s, true, p);
+    else
+        e = wide ? launch_maybe_pdl(evict_move_kernel<128, 64>, grid, block, 0, s, true, p)
+                 : launch_maybe_pdl(evict_move_kernel<128, 32>, grid, block, 0, s, true, p);
+    CUQ_CUDA_TRY(e);
+    return CUQ_OK;
 }
 
 // ----------------------------------------------------- argument checks ----
@@ -621,17 +791,7 @@ int cuq_kv_evict(const cuq_paged_kv *kv, const cuq_batch *batch, const float *ma
     p.new_len = new_len;
     p.mass_out = mass_out;
     p.mass_out_stride = mass_out_stride;
-    cudaStream_t s = (cudaStream_t)stream;
-    const uint32_t rows = batch->n_seqs * kv->kv_heads;
-    evict_select_kernel<<<rows, SEL_THREADS, 0, s>>>(p);
-    CUQ_CUDA_TRY(cudaGetLastError());
-    if (p.a.max_kv <= keep) return CUQ_OK;  // nothing can move
-    if (kv->head_dim == 64)
-        evict_move_kernel<64, 64><<<rows * 2 * 2, MOVE_THREADS, 0, s>>>(p);
-    else
-        evict_move_kernel<128, 64><<<rows * 2 * 4, MOVE_THREADS, 0, s>>>(p);
-    CUQ_CUDA_TRY(cudaGetLastError());
-    return CUQ_OK;
+    return launch_evict(p, kv->head_dim, sm_count_current(), (cudaStream_t)stream);
 }
 
 int cuq_paged_status(void *stream) {
