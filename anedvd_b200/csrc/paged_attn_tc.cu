@@ -39,7 +39,7 @@ struct ManyGeo {
 };
 
 struct ManyBars {
-    uint64_t q_full[2], kv_full[6], kv_empty[6], s_full[2], p_full[2], o_full[2], clean;
+    uint64_t q_full[2], kv_full[6], kv_empty[6], s_full[2], p_full[2][2], o_full[2], clean;
 };
 
 template <typename TQ, typename TC, int HD>
@@ -54,7 +54,7 @@ __global__ void __launch_bounds__(NT, 1) attn_many_kernel(PagedArgs a, PagedQuer
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = warp_index();
     const uint32_t kvh = blockIdx.x % a.kv_heads, split = blockIdx.y;
 
     // the tile: tiles are counted over the sequences that are this kernel's
@@ -113,7 +113,8 @@ __global__ void __launch_bounds__(NT, 1) attn_many_kernel(PagedArgs a, PagedQuer
         for (int i = 0; i < 2; i++) {
             mbar_init(&bars.q_full[i], 128);
             mbar_init(&bars.s_full[i], 1);
-            mbar_init(&bars.p_full[i], 128);
+            mbar_init(&bars.p_full[i][0], 128);
+            mbar_init(&bars.p_full[i][1], 128);
             mbar_init(&bars.o_full[i], 1);
         }
         for (int i = 0; i < ST; i++) {
@@ -133,146 +134,172 @@ __global__ void __launch_bounds__(NT, 1) attn_many_kernel(PagedArgs a, PagedQuer
     const uint32_t tmem = tmem_slot;
     uint8_t *ring = smem + 2 * G::Q;
 
-    if (warp == 8) {
-        // ------------------------------------------------------ MMA issuer
-        if (lane == 0 && nt) {
-            const uint32_t id_s = idesc<TC>(128, KEYS, false), id_o = idesc<TC>(128, HD, true);
-            const uint32_t qa = smem_u32(smem), ra = smem_u32(ring);
-            const uint32_t ns = two ? 2 : 1;
-            auto stage = [&](uint32_t x) { return ra + (x % ST) * G::TILE; };
-            auto wait_kv = [&](uint32_t x) { return mbar_wait(&bars.kv_full[x % ST], (x / ST) & 1, &abort_flag); };
-            auto qk = [&](uint32_t s, uint32_t x) {  // S_s = Q_s K^T with K in stage x
-                const uint32_t kb = stage(x), qb = qa + s * G::Q;
+    // 384 threads of 168 registers: the softmax's 256 take 208, the others' 128 keep 88
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (warp == 8) {
+            // ------------------------------------------------------ MMA issuer
+            if (nt) {
+                const uint32_t leader = elect_one();
+                const uint32_t id_s = idesc<TC>(128, KEYS, false), id_o = idesc<TC>(128, HD, true);
+                const uint64_t qd = sdesc_sw128(smem_u32(smem), 16, 1024), kd = sdesc_sw128(smem_u32(ring), 16, 1024),
+                               vd = sdesc_sw128(smem_u32(ring), KEYS * 128, 1024);
+                const uint32_t ns = two ? 2 : 1;
+                auto wait_kv = [&](uint32_t x) { return mbar_wait(&bars.kv_full[x % ST], (x / ST) & 1, &abort_flag); };
+                auto qk = [&](uint32_t s, uint32_t x) {  // S_s = Q_s K^T with K in stage x
+                    const uint64_t kb = kd + (x % ST) * (G::TILE >> 4), qb = qd + s * (G::Q >> 4);
 #pragma unroll
-                for (int part = 0; part < (SPLIT ? 2 : 1); part++)
+                    for (int part = 0; part < (SPLIT ? 2 : 1); part++)
 #pragma unroll
-                    for (int ks = 0; ks < HD / 16; ks++) {
-                        const uint32_t off = (ks / 4) * (128 * 128) + (ks % 4) * 32;
-                        umma_ss(tmem + s * 128, sdesc_sw128(qb + part * (128 * HD * 2) + off, 16, 1024),
-                                sdesc_sw128(kb + off, 16, 1024), id_s, part | ks ? 1u : 0u);
-                    }
-            };
-            auto pv = [&](uint32_t s, uint32_t x, bool acc) {  // O_s += P_s V with V in stage x
-                const uint32_t vb = stage(x), d = tmem + 256 + s * 128;
+                        for (int ks = 0; ks < HD / 16; ks++) {
+                            const uint32_t off = ((ks / 4) * (128 * 128) + (ks % 4) * 32) >> 4;
+                            umma_ss(leader, tmem + s * 128, qb + part * (128 * HD * 2 >> 4) + off, kb + off, id_s, part | ks ? 1u : 0u);
+                        }
+                };
+                auto pv = [&](uint32_t s, uint32_t x, int half, bool acc) {  // O_s += P_s V, 64 keys of V in stage x
+                    const uint64_t vb = vd + (x % ST) * (G::TILE >> 4) + half * (KEYS * 64 >> 4);
+                    const uint32_t d = tmem + 256 + s * 128, pa = tmem + s * 128 + half * 32;
 #pragma unroll
-                for (int part = 0; part < (SPLIT ? 2 : 1); part++)
+                    for (int part = 0; part < (SPLIT ? 2 : 1); part++)
 #pragma unroll
-                    for (int ks = 0; ks < KEYS / 16; ks++)
-                        umma_ts(d, tmem + s * 128 + part * 64 + ks * 8,
-                                sdesc_sw128(vb + ks * 2048, KEYS * 128, 1024), id_o, (acc || part || ks) ? 1u : 0u);
-            };
-            // stage x may be loaded again; only where it will be, so that no arrival is left in flight at the end
-            auto freed = [&](uint32_t x) {
-                if (x + ST < 2 * nt) umma_commit(&bars.kv_empty[x % ST]);
-            };
-            const bool tail = j1 * KEYS > n;
-            bool ok = mbar_wait(&bars.q_full[0], 0, &abort_flag) && (!two || mbar_wait(&bars.q_full[1], 0, &abort_flag)) &&
-                      wait_kv(0);
-            if (ok) {
-                tc_fence_after();
-                for (uint32_t s = 0; s < ns; s++) {
-                    qk(s, 0);
-                    umma_commit(&bars.s_full[s]);
-                }
-                freed(0);
-            }
-            for (uint32_t j = 0; ok && j < nt; j++) {
-                const uint32_t xv = 2 * j + 1, xk = 2 * j + 2;
-                const bool more = j + 1 < nt;
-                ok = wait_kv(xv) && (!more || wait_kv(xk)) &&
-                     (more || !tail || mbar_wait(&bars.clean, 0, &abort_flag));
-                for (uint32_t s = 0; ok && s < ns; s++) {
-                    ok = mbar_wait(&bars.p_full[s], j & 1, &abort_flag);
-                    if (!ok) break;
-                    tc_fence_after();
-                    pv(s, xv, j > 0);
-                    if (more) {
-                        qk(s, xk);
-                        umma_commit(&bars.s_full[s]);
-                    } else {
-                        umma_commit(&bars.o_full[s]);
-                    }
-                }
+                        for (int i = 0; i < KEYS / 32; i++)
+                            umma_ts(leader, d, pa + part * 64 + i * 8, vb + (i * 2048 >> 4), id_o, (acc || part || i) ? 1u : 0u);
+                };
+                // stage x may be loaded again; only where it will be, so that no arrival is left in flight at the end
+                auto freed = [&](uint32_t x) {
+                    if (x + ST < 2 * nt) umma_commit(leader, &bars.kv_empty[x % ST]);
+                };
+                const bool tail = j1 * KEYS > n;
+                bool ok = mbar_wait(&bars.q_full[0], 0, &abort_flag) && (!two || mbar_wait(&bars.q_full[1], 0, &abort_flag)) &&
+                          wait_kv(0);
                 if (ok) {
-                    freed(xv);
-                    if (more) freed(xk);
+                    tc_fence_after();
+                    for (uint32_t s = 0; s < ns; s++) {
+                        qk(s, 0);
+                        umma_commit(leader, &bars.s_full[s]);
+                    }
+                    freed(0);
+                }
+                for (uint32_t j = 0; ok && j < nt; j++) {
+                    const uint32_t xv = 2 * j + 1, xk = 2 * j + 2;
+                    const bool more = j + 1 < nt;
+                    ok = wait_kv(xv) && (!more || wait_kv(xk)) &&
+                         (more || !tail || mbar_wait(&bars.clean, 0, &abort_flag));
+                    for (uint32_t s = 0; ok && s < ns; s++) {
+                        ok = mbar_wait(&bars.p_full[s][0], j & 1, &abort_flag);
+                        if (!ok) break;
+                        tc_fence_after();
+                        pv(s, xv, 0, j > 0);
+                        ok = mbar_wait(&bars.p_full[s][1], j & 1, &abort_flag);
+                        if (!ok) break;
+                        tc_fence_after();
+                        pv(s, xv, 1, true);
+                        if (more) {
+                            qk(s, xk);
+                            umma_commit(leader, &bars.s_full[s]);
+                        } else {
+                            umma_commit(leader, &bars.o_full[s]);
+                        }
+                    }
+                    if (ok) {
+                        freed(xv);
+                        if (more) freed(xk);
+                    }
                 }
             }
-        }
-    } else if (warp == 9) {
-        // ------------------------------------------------------ TMA: K and V pages
-        const uint32_t box = min(a.page_size, (uint32_t)KEYS), nbox = KEYS / box;
-        auto page_of = [&](uint32_t j) -> int {  // of this lane's box of tile j; past the end: a hole
-            const uint32_t slot = j * KEYS + lane * box;
-            if (lane >= nbox || slot >= n) return (int)a.n_pages;
-            const int pg = a.page(b, slot >> a.page_shift);
-            return pg < 0 ? (int)a.n_pages : pg;
-        };
-        int pg = page_of(j0);
-        bool ok = true;
-        for (uint32_t j = 0; ok && j < nt; j++) {
-            const int next = j + 1 < nt ? page_of(j0 + j + 1) : 0;
-            const int slot = (int)(((j0 + j) * KEYS + lane * box) & (a.page_size - 1));
+        } else if (warp == 9) {
+            // ------------------------------------------------------ TMA: K and V pages
+            const uint32_t box = min(a.page_size, (uint32_t)KEYS), nbox = KEYS / box;
+            auto page_of = [&](uint32_t j) -> int {  // of this lane's box of tile j; past the end: a hole
+                const uint32_t slot = j * KEYS + lane * box;
+                if (lane >= nbox || slot >= n) return (int)a.n_pages;
+                const int pg = a.page(b, slot >> a.page_shift);
+                return pg < 0 ? (int)a.n_pages : pg;
+            };
+            int pg = page_of(j0);
+            bool ok = true;
+            for (uint32_t j = 0; ok && j < nt; j++) {
+                const int next = j + 1 < nt ? page_of(j0 + j + 1) : 0;
+                const int slot = (int)(((j0 + j) * KEYS + lane * box) & (a.page_size - 1));
 #pragma unroll
-            for (int v = 0; v < 2; v++) {
-                const uint32_t x = 2 * j + v, st = x % ST;
-                if (x >= (uint32_t)ST && !mbar_wait(&bars.kv_empty[st], ((x / ST) - 1) & 1, &abort_flag)) {
-                    ok = false;
-                    break;
-                }
-                if (lane == 0) mbar_expect_tx(&bars.kv_full[st], G::TILE);
-                __syncwarp();
-                if (lane < nbox) {
-                    const uint32_t dst = smem_u32(ring + st * G::TILE) + lane * box * 128;
+                for (int v = 0; v < 2; v++) {
+                    const uint32_t x = 2 * j + v, st = x % ST;
+                    if (x >= (uint32_t)ST && !mbar_wait(&bars.kv_empty[st], ((x / ST) - 1) & 1, &abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    if (lane == 0) mbar_expect_tx(&bars.kv_full[st], G::TILE);
+                    __syncwarp();
+                    if (lane < nbox) {
+                        const uint32_t dst = smem_u32(ring + st * G::TILE) + lane * box * 128;
 #pragma unroll
-                    for (int cb = 0; cb < G::CB; cb++)
-                        tma_load_page(dst + cb * (KEYS * 128), v ? &mv : &mk, cb * 64, slot, (int)kvh, pg,
-                                      &bars.kv_full[st]);
+                        for (int cb = 0; cb < G::CB; cb++)
+                            tma_load_page(dst + cb * (KEYS * 128), v ? &mv : &mk, cb * 64, slot, (int)kvh, pg,
+                                          &bars.kv_full[st]);
+                    }
+                }
+                pg = next;
+            }
+            // V rows past the sequence's end may hold anything, and 0 * inf is not 0
+            if (ok && nt && j1 * KEYS > n) {
+                const uint32_t x = 2 * nt - 1, st = x % ST;
+                if (mbar_wait(&bars.kv_full[st], (x / ST) & 1, &abort_flag)) {
+                    const uint32_t r0 = n - (j1 - 1) * KEYS;
+                    for (uint32_t i = lane; i < (KEYS - r0) * (HD / 8); i += 32) {
+                        const uint32_t r = r0 + i / (HD / 8), c = i % (HD / 8);
+                        *reinterpret_cast<uint4 *>(ring + st * G::TILE + (c / 8) * (KEYS * 128) + sw128(r, c & 7)) =
+                            make_uint4(0, 0, 0, 0);
+                    }
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bars.clean);
                 }
             }
-            pg = next;
         }
-        // V rows past the sequence's end may hold anything, and 0 * inf is not 0
-        if (ok && nt && j1 * KEYS > n) {
-            const uint32_t x = 2 * nt - 1, st = x % ST;
-            if (mbar_wait(&bars.kv_full[st], (x / ST) & 1, &abort_flag)) {
-                const uint32_t r0 = n - (j1 - 1) * KEYS;
-                for (uint32_t i = lane; i < (KEYS - r0) * (HD / 8); i += 32) {
-                    const uint32_t r = r0 + i / (HD / 8), c = i % (HD / 8);
-                    *reinterpret_cast<uint4 *>(ring + st * G::TILE + (c / 8) * (KEYS * 128) + sw128(r, c & 7)) =
-                        make_uint4(0, 0, 0, 0);
-                }
-                fence_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bars.clean);
-            }
-        }
-    } else if (warp < 8) {
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         // ------------------------------------------------------ softmax
         const uint32_t s = warp >> 2, t = tid & 127;
         if (s == 0 || two) {
-            // queries: a negative scale goes into their sign, so that the largest score has the largest weight
+            // queries, eight 16-byte chunks of them in flight a thread; a negative scale
+            // goes into their sign, so that the largest score has the largest weight
             uint8_t *sq = smem + s * G::Q;
-            for (uint32_t i = t; i < 128 * HD / 8; i += 128) {
-                const uint32_t r = i / (HD / 8), c = i % (HD / 8);
-                float v[8];
+            constexpr int CH = HD / 8;  // chunks of 8 values a row
+            const uint32_t flip = q.scale < 0.f ? 0x80008000u : 0u;
+#pragma unroll 1
+            for (uint32_t i0 = t; i0 < 128 * CH; i0 += 128 * 8) {
+                uint4 raw[8][SPLIT ? 2 : 1];
 #pragma unroll
-                for (int e = 0; e < 8; e++) v[e] = 0.f;
-                if (s * 128 + r < my_rows) {
-                    const uint32_t rr = row0 + s * 128 + r;
-                    const uint32_t tok = first + rr / q.group, head = kvh * q.group + rr % q.group;
-                    load8(reinterpret_cast<const TQ *>(q.q) + (size_t)tok * q.q_stride + (size_t)head * HD + c * 8, v);
+                for (int e = 0; e < 8; e++) {
+                    const uint32_t i = i0 + e * 128, r = i / CH, c = i % CH;
+#pragma unroll
+                    for (int w = 0; w < (SPLIT ? 2 : 1); w++) raw[e][w] = make_uint4(0, 0, 0, 0);
+                    if (s * 128 + r < my_rows) {
+                        const uint32_t rr = row0 + s * 128 + r;
+                        const uint32_t tok = first + rr / q.group, head = kvh * q.group + rr % q.group;
+                        const uint4 *src = reinterpret_cast<const uint4 *>(
+                            reinterpret_cast<const TQ *>(q.q) + (size_t)tok * q.q_stride + (size_t)head * HD + c * 8);
+#pragma unroll
+                        for (int w = 0; w < (SPLIT ? 2 : 1); w++) raw[e][w] = __ldg(src + w);
+                    }
                 }
-                if (q.scale < 0.f)
 #pragma unroll
-                    for (int e = 0; e < 8; e++) v[e] = -v[e];
-                uint32_t hi[4], lo[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) split_pack<TC>(v[2 * e], v[2 * e + 1], hi[e], lo[e]);
-                const uint32_t at = (c / 8) * (128 * 128) + sw128(r, c & 7);
-                *reinterpret_cast<uint4 *>(sq + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                if (SPLIT)
-                    *reinterpret_cast<uint4 *>(sq + 128 * HD * 2 + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                for (int e = 0; e < 8; e++) {
+                    const uint32_t i = i0 + e * 128, r = i / CH, c = i % CH;
+                    const uint32_t at = (c / 8) * (128 * 128) + sw128(r, c & 7);
+                    uint4 h = raw[e][0];
+                    if (SPLIT) {
+                        const uint4 g = raw[e][SPLIT ? 1 : 0];
+                        uint32_t lo[4];
+                        split_pack<TC>(__uint_as_float(raw[e][0].x), __uint_as_float(raw[e][0].y), h.x, lo[0]);
+                        split_pack<TC>(__uint_as_float(raw[e][0].z), __uint_as_float(raw[e][0].w), h.y, lo[1]);
+                        split_pack<TC>(__uint_as_float(g.x), __uint_as_float(g.y), h.z, lo[2]);
+                        split_pack<TC>(__uint_as_float(g.z), __uint_as_float(g.w), h.w, lo[3]);
+                        *reinterpret_cast<uint4 *>(sq + 128 * HD * 2 + at) =
+                            make_uint4(lo[0] ^ flip, lo[1] ^ flip, lo[2] ^ flip, lo[3] ^ flip);
+                    }
+                    *reinterpret_cast<uint4 *>(sq + at) = make_uint4(h.x ^ flip, h.y ^ flip, h.z ^ flip, h.w ^ flip);
+                }
             }
             fence_async_smem();
             mbar_arrive(&bars.q_full[s]);
@@ -297,8 +324,18 @@ __global__ void __launch_bounds__(NT, 1) attn_many_kernel(PagedArgs a, PagedQuer
                 }
                 tc_fence_after();
                 float x[128];
+                tmem_ld32(ts, x);
+                tmem_ld32(ts + 32, x + 32);
+                tmem_wait_ld();
+                tmem_ld32(ts + 64, x + 64);
+                tmem_ld32(ts + 96, x + 96);
+                float mx[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-                for (int i = 0; i < 4; i++) tmem_ld32(ts + i * 32, x + i * 32);
+                for (int i = 4; i < 60; i += 8)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) mx[e] = max3(mx[e], x[i + e], x[i + 4 + e]);
+#pragma unroll
+                for (int e = 0; e < 4; e++) mx[e] = fmaxf(mx[e], x[60 + e]);
                 tmem_wait_ld();
                 const uint32_t k0 = (j0 + j) * KEYS;
                 if (hole || k0 < all_lo || k0 + KEYS > all_hi) {
@@ -311,13 +348,17 @@ __global__ void __launch_bounds__(NT, 1) attn_many_kernel(PagedArgs a, PagedQuer
 #pragma unroll
                     for (int i = 0; i < 128; i++)
                         if (i < rlo || i >= rhi || ((gone >> (i / 16)) & 1u)) x[i] = -INFINITY;
-                }
-                float mx[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-                for (int i = 4; i < 128; i += 4) {
+                    for (int e = 0; e < 4; e++) mx[e] = -INFINITY;  // over the visible ones only
 #pragma unroll
-                    for (int e = 0; e < 4; e++) mx[e] = fmaxf(mx[e], x[i + e]);
+                    for (int i = 0; i < 64; i += 8)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) mx[e] = max3(mx[e], x[i + e], x[i + 4 + e]);
                 }
+#pragma unroll
+                for (int i = 64; i < 128; i += 8)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) mx[e] = max3(mx[e], x[i + e], x[i + 4 + e]);
                 const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                 const bool up = mt > m + grow || (m == -INFINITY && mt > m);
                 if (__any_sync(~0u, up)) {
@@ -348,26 +389,30 @@ __global__ void __launch_bounds__(NT, 1) attn_many_kernel(PagedArgs a, PagedQuer
                 const f32x2 cc = pack2(c2, c2), nm = pack2(-mm * c2, -mm * c2);
                 f32x2 sum = pack2(0.f, 0.f);
 #pragma unroll
-                for (int i = 0; i < 128; i += 32) {
-                    uint32_t ph[16], pl[16];
+                for (int half = 0; half < 2; half++) {
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        float u, v;
-                        unpack2(fma2(pack2(x[i + e], x[i + e + 1]), cc, nm), u, v);
-                        u = ex2(u);
-                        v = ex2(v);
-                        sum = add2(sum, pack2(u, v));
-                        if (SPLIT)
-                            split_pack<TC>(u, v, ph[e / 2], pl[e / 2]);
-                        else
-                            ph[e / 2] = Pair<TC>::pack(u, v);
+                    for (int q16 = 0; q16 < 2; q16++) {
+                        uint32_t ph[16], pl[16];
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2) {
+                            const int i = half * 64 + q16 * 32 + e;
+                            float u, v;
+                            unpack2(fma2(pack2(x[i], x[i + 1]), cc, nm), u, v);
+                            u = ex2(u);
+                            v = ex2(v);
+                            sum = add2(sum, pack2(u, v));
+                            if (SPLIT)
+                                split_pack<TC>(u, v, ph[e / 2], pl[e / 2]);
+                            else
+                                ph[e / 2] = Pair<TC>::pack(u, v);
+                        }
+                        tmem_st16(ts + half * 32 + q16 * 16, ph);
+                        if (SPLIT) tmem_st16(ts + 64 + half * 32 + q16 * 16, pl);
                     }
-                    tmem_st16(ts + i / 2, ph);
-                    if (SPLIT) tmem_st16(ts + 64 + i / 2, pl);
+                    tmem_wait_st();
+                    tc_fence_before();
+                    mbar_arrive(&bars.p_full[s][half]);
                 }
-                tmem_wait_st();
-                tc_fence_before();
-                mbar_arrive(&bars.p_full[s]);
                 float u, v;
                 unpack2(sum, u, v);
                 l += u + v;

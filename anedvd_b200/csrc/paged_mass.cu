@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
     uint32_t *s_ends = reinterpret_cast<uint32_t *>(qring + QST * G::Q);  // items of sequences 0..i, per KV head
     const PagedArgs &a = p.a;
     const PagedQuery &q = p.q;
-    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = warp_index();
     uint32_t rank, ranks;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
@@ -169,7 +169,8 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
 
     if (warp == 8) {
         // ------------------------------------------------------ MMA issuer
-        if (lane == 0) {
+        {
+            const uint32_t leader = elect_one();
             const uint32_t ka = smem_u32(kring), qa = smem_u32(qring);
             uint32_t kx = 0, qx = 0, st = 0, ob = ~0u, oh = 0, oq = 0;
             bool ok = true, held = false;
@@ -182,7 +183,7 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
                     const uint32_t qt = t.qt0 + rank + e * ranks;
                     if (!held || t.b != ob || t.h != oh || qt != oq) {
                         if (held) {
-                            umma_commit(&q_empty[qx % QST]);
+                            umma_commit(leader, &q_empty[qx % QST]);
                             qx++;
                         }
                         held = true;
@@ -204,16 +205,16 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
 #pragma unroll
                             for (int ks = 0; ks < HD / 16; ks++) {
                                 const uint32_t off = (ks / 4) * (128 * 128) + (ks % 4) * 32;
-                                umma_ss(tmem + (s * 2 + buf) * 128, sdesc_sw128(kb + off, 16, 1024),
+                                umma_ss(leader, tmem + (s * 2 + buf) * 128, sdesc_sw128(kb + off, 16, 1024),
                                         sdesc_sw128(qb + part * G::TILE + off, 16, 1024), id, part | ks ? 1u : 0u);
                             }
-                        umma_commit(&s_full[s][buf]);
+                        umma_commit(leader, &s_full[s][buf]);
                     }
                 }
-                if (ok) umma_commit(&k_empty[kx & 1]);
+                if (ok) umma_commit(leader, &k_empty[kx & 1]);
                 kx++;
             }
-            if (ok && held) umma_commit(&q_empty[qx % QST]);
+            if (ok && held) umma_commit(leader, &q_empty[qx % QST]);
         }
     } else if (warp == 9) {
         // ------------------------------------------------------ TMA: K pages
