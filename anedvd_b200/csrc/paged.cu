@@ -561,7 +561,7 @@ int check_paged(const char *who, const cuq_paged_kv *kv, const cuq_batch *b, boo
 }
 
 int check_heads(const char *who, const cuq_paged_kv *kv, uint32_t heads) {
-    CUQ_CHECK_ARG(heads > 0 && heads <= 65535 && heads % kv->kv_heads == 0,
+    CUQ_CHECK_ARG(heads > 0 && heads <= 32768 && heads % kv->kv_heads == 0,
                   "%s: heads (%u) must be a positive multiple of kv_heads (%u)", who, heads, kv->kv_heads);
     return CUQ_OK;
 }
@@ -585,6 +585,7 @@ int check_query(const char *who, const cuq_paged_kv *kv, uint32_t n_tok, const v
     out.q_stride = q_stride;
     out.heads = heads;
     out.group = heads / kv->kv_heads;
+    out.group_inv = (uint32_t)((0x100000000ull + out.group - 1) / out.group);
     out.scale = scale;
     out.causal = causal ? 1 : 0;
     out.window = window < (1u << 30) ? window : (1u << 30);  // slots are below 2^30

@@ -44,10 +44,13 @@ struct PagedArgs {
 struct PagedQuery {
     const void *q;
     size_t q_stride;
-    uint32_t heads, group;
+    uint32_t heads, group, group_inv;  // group_inv: ceil(2^32 / group)
     float scale;
     int causal;
     uint32_t window;
+
+    // x / group for x below 2^16 + group (so that x * group stays below 2^32)
+    __device__ __forceinline__ uint32_t div_group(uint32_t x) const { return group == 1 ? x : __umulhi(x, group_inv); }
 
     // the slots [lo, hi) that the query at slot `pos` of a cache of n slots sees
     __device__ __forceinline__ void range(int pos, uint32_t n, uint32_t &lo, uint32_t &hi) const {

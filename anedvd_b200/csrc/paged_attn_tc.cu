@@ -38,6 +38,23 @@ struct ManyGeo {
     static constexpr int SMEM = 1024 + 2 * Q + ST * TILE;
 };
 
+// the 128 threads of softmax stream s
+__device__ __forceinline__ void wg_sync(uint32_t s) { asm volatile("bar.sync %0, 128;" ::"r"(s + 1) : "memory"); }
+
+// whether `ok` holds in all of them (a wait may have given up in some)
+__device__ __forceinline__ bool wg_all(uint32_t s, bool ok) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "barrier.cta.red.and.pred q, %2, 128, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"((uint32_t)ok), "r"(s + 1)
+        : "memory");
+    return r != 0;
+}
+
 struct ManyBars {
     uint64_t q_full[2], kv_full[6], kv_empty[6], s_full[2], p_full[2][2], o_full[2], clean;
 };
@@ -52,7 +69,7 @@ __global__ void __launch_bounds__(NT, 1) attn_many_kernel(PagedArgs a, PagedQuer
     extern __shared__ uint8_t smem_raw[];
     __shared__ ManyBars bars;
     __shared__ uint32_t tmem_slot;
-    __shared__ int abort_flag;
+    __shared__ int abort_flag, s_hole[2];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = warp_index();
     const uint32_t kvh = blockIdx.x % a.kv_heads, split = blockIdx.y;
@@ -109,7 +126,7 @@ __global__ void __launch_bounds__(NT, 1) attn_many_kernel(PagedArgs a, PagedQuer
 
     if (warp == 8) tmem_alloc512(&tmem_slot);
     if (tid == 0) {
-        abort_flag = 0;
+        abort_flag = s_hole[0] = s_hole[1] = 0;
         for (int i = 0; i < 2; i++) {
             mbar_init(&bars.q_full[i], 128);
             mbar_init(&bars.s_full[i], 1);
@@ -124,12 +141,8 @@ __global__ void __launch_bounds__(NT, 1) attn_many_kernel(PagedArgs a, PagedQuer
         mbar_init(&bars.clean, 1);
         mbar_init_fence();
     }
-    // are there holes among the slots?  (then the softmax looks each tile's pages up)
-    int hole = 0;
-    for (uint32_t s = (j0 * KEYS >> a.page_shift) + tid; ((uint64_t)s << a.page_shift) < min(n, j1 * KEYS); s += NT)
-        hole |= a.page(b, s) < 0;
     tc_fence_before();
-    hole = __syncthreads_or(hole);
+    __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
     uint8_t *ring = smem + 2 * G::Q;
@@ -261,35 +274,45 @@ __global__ void __launch_bounds__(NT, 1) attn_many_kernel(PagedArgs a, PagedQuer
         // ------------------------------------------------------ softmax
         const uint32_t s = warp >> 2, t = tid & 127;
         if (s == 0 || two) {
-            // queries, eight 16-byte chunks of them in flight a thread; a negative scale
-            // goes into their sign, so that the largest score has the largest weight
+            // are there holes among the slots?  (then the softmax looks each tile's pages up)
+            bool hole = false;
+            for (uint32_t x = (j0 * KEYS >> a.page_shift) + t; ((uint64_t)x << a.page_shift) < min(n, j1 * KEYS); x += 128)
+                hole |= a.page(b, x) < 0;
+            if (hole) s_hole[s] = 1;
+            // queries, all of a thread's 16-byte chunks in flight; a negative scale goes
+            // into their sign, so that the largest score has the largest weight
             uint8_t *sq = smem + s * G::Q;
-            constexpr int CH = HD / 8;  // chunks of 8 values a row
+            constexpr int CH = HD / 8, W = SPLIT ? 2 : 1, BATCH = SPLIT ? 8 : CH;  // chunks of 8 values a row
             const uint32_t flip = q.scale < 0.f ? 0x80008000u : 0u;
+            const uint32_t tok0 = row0 / q.group, rem0 = row0 - tok0 * q.group + s * 128;
+            const TQ *qb = reinterpret_cast<const TQ *>(q.q) + (size_t)(first + tok0) * q.q_stride +
+                           (size_t)kvh * q.group * HD;
+            // local row r: token tok0 + (rem0 + r) / group
+            auto row_of = [&](uint32_t r, uint32_t &tok, uint32_t &head) {
+                const uint32_t x = rem0 + r;
+                tok = q.div_group(x);
+                head = x - tok * q.group;
+            };
 #pragma unroll 1
-            for (uint32_t i0 = t; i0 < 128 * CH; i0 += 128 * 8) {
-                uint4 raw[8][SPLIT ? 2 : 1];
+            for (uint32_t i0 = t; i0 < 128 * CH; i0 += 128 * BATCH) {
+                uint4 raw[BATCH][W];
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
+                for (int e = 0; e < BATCH; e++) {
                     const uint32_t i = i0 + e * 128, r = i / CH, c = i % CH;
+                    uint32_t tok, head;
+                    row_of(r, tok, head);
+                    const bool in = s * 128 + r < my_rows;
+                    const uint4 *src = reinterpret_cast<const uint4 *>(qb + (size_t)tok * q.q_stride + head * HD + c * 8);
 #pragma unroll
-                    for (int w = 0; w < (SPLIT ? 2 : 1); w++) raw[e][w] = make_uint4(0, 0, 0, 0);
-                    if (s * 128 + r < my_rows) {
-                        const uint32_t rr = row0 + s * 128 + r;
-                        const uint32_t tok = first + rr / q.group, head = kvh * q.group + rr % q.group;
-                        const uint4 *src = reinterpret_cast<const uint4 *>(
-                            reinterpret_cast<const TQ *>(q.q) + (size_t)tok * q.q_stride + (size_t)head * HD + c * 8);
-#pragma unroll
-                        for (int w = 0; w < (SPLIT ? 2 : 1); w++) raw[e][w] = __ldg(src + w);
-                    }
+                    for (int w = 0; w < W; w++) raw[e][w] = in ? __ldg(src + w) : make_uint4(0, 0, 0, 0);
                 }
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
+                for (int e = 0; e < BATCH; e++) {
                     const uint32_t i = i0 + e * 128, r = i / CH, c = i % CH;
                     const uint32_t at = (c / 8) * (128 * 128) + sw128(r, c & 7);
                     uint4 h = raw[e][0];
                     if (SPLIT) {
-                        const uint4 g = raw[e][SPLIT ? 1 : 0];
+                        const uint4 g = raw[e][W - 1];
                         uint32_t lo[4];
                         split_pack<TC>(__uint_as_float(raw[e][0].x), __uint_as_float(raw[e][0].y), h.x, lo[0]);
                         split_pack<TC>(__uint_as_float(raw[e][0].z), __uint_as_float(raw[e][0].w), h.y, lo[1]);
@@ -303,6 +326,8 @@ __global__ void __launch_bounds__(NT, 1) attn_many_kernel(PagedArgs a, PagedQuer
             }
             fence_async_smem();
             mbar_arrive(&bars.q_full[s]);
+            wg_sync(s);
+            hole = s_hole[s];
 
             const uint32_t rr = row0 + s * 128 + t;
             const bool live = s * 128 + t < my_rows;
@@ -425,39 +450,59 @@ __global__ void __launch_bounds__(NT, 1) attn_many_kernel(PagedArgs a, PagedQuer
                 inv = l == 0.f ? 0.f : 1.f / l;
                 if (l != 0.f) lse2 = m * c2 + log2f(l);
             }
-            const uint32_t tok = first + rr / q.group, head = kvh * q.group + rr % q.group;
+            ok = wg_all(s, ok);
             const bool direct = o.plan.many_splits == 1;
-            const size_t prow = ((size_t)split * a.n_tok + tok) * q.heads + head;
-            if (ok) {
-                if (live) {
-                    if (direct && o.lse) o.lse[(size_t)tok * q.heads + head] = lse2 * 0.6931471805599453f;
-                    if (!direct) o.many_lse[prow] = lse2;
-                }
-                if (nt || direct) {
-                    TQ *dst = reinterpret_cast<TQ *>(o.out) + (size_t)tok * o.out_stride + (size_t)head * HD;
-                    float *part = o.many_o + prow * HD;
-#pragma unroll 1
-                    for (int i = 0; i < HD / 32; i++) {
-                        float ov[32];
-                        if (nt) {
-                            tmem_ld32(to + i * 32, ov);
-                            tmem_wait_ld();
-                        }
-#pragma unroll
-                        for (int e = 0; e < 32; e += 8) {
-                            float w[8];
-#pragma unroll
-                            for (int k = 0; k < 8; k++) w[k] = nt ? ov[e + k] * inv : 0.f;
-                            if (live) {
-                                if (direct)
-                                    store8(dst + i * 32 + e, w);
-                                else
-                                    store8(part + i * 32 + e, w);
-                            }
-                        }
-                    }
-                }
+            uint32_t tok, head;
+            row_of(t, tok, head);
+            tok += first + tok0;
+            head += kvh * q.group;
+            const size_t part0 = (size_t)split * a.n_tok * q.heads;
+            if (ok && live) {
+                if (direct && o.lse) o.lse[(size_t)tok * q.heads + head] = lse2 * 0.6931471805599453f;
+                if (!direct) o.many_lse[part0 + (size_t)tok * q.heads + head] = lse2;
             }
+            // rows leave through shared memory (this stream's queries are done with), 128
+            // bytes of each at a time, so that stores cover whole lines
+            auto leave = [&](auto *dst0, size_t stride, size_t row_step) {
+                using TO = typename std::remove_pointer<decltype(dst0)>::type;
+                constexpr int COLS = 128 / sizeof(TO);
+#pragma unroll 1
+                for (int c0 = 0; c0 < HD; c0 += COLS) {
+                    float ov[COLS];
+#pragma unroll
+                    for (int i = 0; i < COLS; i += 32) tmem_ld32(to + c0 + i, ov + i);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int c = 0; c < 8; c++) {
+                        uint4 u;
+                        if constexpr (sizeof(TO) == 4) {
+                            const float *w = ov + c * 4;
+                            u = make_uint4(__float_as_uint(nt ? w[0] * inv : 0.f), __float_as_uint(nt ? w[1] * inv : 0.f),
+                                           __float_as_uint(nt ? w[2] * inv : 0.f), __float_as_uint(nt ? w[3] * inv : 0.f));
+                        } else {
+                            const float *w = ov + c * 8;
+                            u = make_uint4(Pair<TO>::pack(w[0] * inv, w[1] * inv), Pair<TO>::pack(w[2] * inv, w[3] * inv),
+                                           Pair<TO>::pack(w[4] * inv, w[5] * inv), Pair<TO>::pack(w[6] * inv, w[7] * inv));
+                            if (!nt) u = make_uint4(0, 0, 0, 0);  // no tile: tensor memory holds anything
+                        }
+                        *reinterpret_cast<uint4 *>(sq + sw128(t, c)) = u;
+                    }
+                    wg_sync(s);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const uint32_t r = e * 16 + t / 8, c = t & 7;
+                        uint32_t tk, hd;
+                        row_of(r, tk, hd);
+                        if (s * 128 + r < my_rows)
+                            *reinterpret_cast<uint4 *>(dst0 + (size_t)(first + tok0 + tk) * stride +
+                                                       (size_t)(kvh * q.group + hd) * row_step + c0 + c * (16 / sizeof(TO))) =
+                                *reinterpret_cast<const uint4 *>(sq + sw128(r, c));
+                    }
+                    wg_sync(s);
+                }
+            };
+            if (ok && direct) leave(reinterpret_cast<TQ *>(o.out), o.out_stride, (size_t)HD);
+            if (ok && !direct && nt) leave(o.many_o + part0 * HD, (size_t)q.heads * HD, (size_t)HD);
         }
     }
     tc_fence_before();
