@@ -38,23 +38,6 @@ struct ManyGeo {
     static constexpr int SMEM = 1024 + 2 * Q + ST * TILE;
 };
 
-// the 128 threads of softmax stream s
-__device__ __forceinline__ void wg_sync(uint32_t s) { asm volatile("bar.sync %0, 128;" ::"r"(s + 1) : "memory"); }
-
-// whether `ok` holds in all of them (a wait may have given up in some)
-__device__ __forceinline__ bool wg_all(uint32_t s, bool ok) {
-    uint32_t r;
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\t"
-        "setp.ne.u32 p, %1, 0;\n\t"
-        "barrier.cta.red.and.pred q, %2, 128, p;\n\t"
-        "selp.u32 %0, 1, 0, q;\n\t}"
-        : "=r"(r)
-        : "r"((uint32_t)ok), "r"(s + 1)
-        : "memory");
-    return r != 0;
-}
-
 struct ManyBars {
     uint64_t q_full[2], kv_full[6], kv_empty[6], s_full[2], p_full[2][2], o_full[2], clean;
 };
@@ -326,7 +309,7 @@ __global__ void __launch_bounds__(NT, 1) attn_many_kernel(PagedArgs a, PagedQuer
             }
             fence_async_smem();
             mbar_arrive(&bars.q_full[s]);
-            wg_sync(s);
+            group_sync(s + 1);
             hole = s_hole[s];
 
             const uint32_t rr = row0 + s * 128 + t;
@@ -450,7 +433,7 @@ __global__ void __launch_bounds__(NT, 1) attn_many_kernel(PagedArgs a, PagedQuer
                 inv = l == 0.f ? 0.f : 1.f / l;
                 if (l != 0.f) lse2 = m * c2 + log2f(l);
             }
-            ok = wg_all(s, ok);
+            ok = group_all(s + 1, ok);
             const bool direct = o.plan.many_splits == 1;
             uint32_t tok, head;
             row_of(t, tok, head);
@@ -487,7 +470,7 @@ __global__ void __launch_bounds__(NT, 1) attn_many_kernel(PagedArgs a, PagedQuer
                         }
                         *reinterpret_cast<uint4 *>(sq + sw128(t, c)) = u;
                     }
-                    wg_sync(s);
+                    group_sync(s + 1);
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
                         const uint32_t r = e * 16 + t / 8, c = t & 7;
@@ -498,7 +481,7 @@ __global__ void __launch_bounds__(NT, 1) attn_many_kernel(PagedArgs a, PagedQuer
                                                        (size_t)(kvh * q.group + hd) * row_step + c0 + c * (16 / sizeof(TO))) =
                                 *reinterpret_cast<const uint4 *>(sq + sw128(r, c));
                     }
-                    wg_sync(s);
+                    group_sync(s + 1);
                 }
             };
             if (ok && direct) leave(reinterpret_cast<TQ *>(o.out), o.out_stride, (size_t)HD);

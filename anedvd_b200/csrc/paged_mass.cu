@@ -260,44 +260,60 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
                 if (qx && t.b == ob && t.h == oh && qt == oq) continue;
                 ob = t.b, oh = t.h, oq = qt;
                 const uint32_t st = qx % QST, nr = tile_rows(t, qt), r0 = t.i0 * q.group + qt * 128;
-                if (qx >= (uint32_t)QST && !mbar_wait(&q_empty[st], ((qx / QST) - 1) & 1, &abort_flag)) {
-                    ok = false;
-                    break;
-                }
-                // a row that saw nothing counts nothing; its products are kept finite
-                float ls = INFINITY;
+                const uint32_t tok0 = r0 / q.group, rem0 = r0 - tok0 * q.group;  // row r: (rem0 + r) / group tokens on
+                auto row_of = [&](uint32_t r, uint32_t &tok, uint32_t &head) {
+                    const uint32_t y = rem0 + r;
+                    tok = q.div_group(y);
+                    head = y - tok * q.group;
+                };
+                const TQ *qb = reinterpret_cast<const TQ *>(q.q) + (size_t)(t.first + tok0) * q.q_stride +
+                               (size_t)t.h * q.group * HD;
+                float ls = -INFINITY;
                 if (t128 < nr) {
-                    const uint32_t r = r0 + t128;
-                    ls = __ldg(p.lse + (size_t)(t.first + r / q.group) * q.heads + t.h * q.group + r % q.group);
-                    ls = ls == -INFINITY ? INFINITY : ls * 1.4426950408889634f;
+                    uint32_t tok, head;
+                    row_of(t128, tok, head);
+                    ls = __ldg(p.lse + (size_t)(t.first + tok0 + tok) * q.heads + t.h * q.group + head);
                 }
-                s_lse[st][t128] = ls;
+                // all of a thread's 16-byte chunks in flight, before the wait for the stage
+                constexpr int CH = HD / 8, W = SPLIT ? 2 : 1, BATCH = SPLIT ? CH / 2 : CH;
                 uint8_t *dst = qring + st * G::Q;
-                constexpr int CH = HD / 8;
-#pragma unroll 4
-                for (uint32_t i = t128; i < 128 * CH; i += 128) {
-                    const uint32_t r = i / CH, c = i % CH;
-                    const uint32_t at = (c / 8) * (128 * 128) + sw128(r, c & 7);
-                    const uint32_t rr = r0 + r, tok = t.first + rr / q.group, head = t.h * q.group + rr % q.group;
-                    const bool live =
-                        r < nr && __ldg(p.lse + (size_t)tok * q.heads + head) != -INFINITY;
-                    const TQ *src = reinterpret_cast<const TQ *>(q.q) + (size_t)tok * q.q_stride + (size_t)head * HD + c * 8;
-                    if (SPLIT) {
-                        float v[8];
+#pragma unroll 1
+                for (int part = 0; part < CH / BATCH; part++) {
+                    uint4 raw[BATCH][W];
 #pragma unroll
-                        for (int k = 0; k < 8; k++) v[k] = 0.f;
-                        if (live) load8(src, v);
-                        uint32_t hi[4], lo[4];
+                    for (int k = 0; k < BATCH; k++) {
+                        const uint32_t i = t128 + (part * BATCH + k) * 128, r = i / CH, c = i % CH;
+                        uint32_t tok, head;
+                        row_of(r, tok, head);
+                        const uint4 *src = reinterpret_cast<const uint4 *>(qb + (size_t)tok * q.q_stride + head * HD + c * 8);
 #pragma unroll
-                        for (int k = 0; k < 4; k++) split_pack<TC>(v[2 * k], v[2 * k + 1], hi[k], lo[k]);
-                        *reinterpret_cast<uint4 *>(dst + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                        *reinterpret_cast<uint4 *>(dst + G::TILE + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                    } else {
-                        uint4 v = make_uint4(0, 0, 0, 0);
-                        if (live) v = __ldg(reinterpret_cast<const uint4 *>(src));
-                        *reinterpret_cast<uint4 *>(dst + at) = v;
+                        for (int w = 0; w < W; w++) raw[k][w] = r < nr ? __ldg(src + w) : make_uint4(0, 0, 0, 0);
+                    }
+                    if (part == 0) {
+                        if (qx >= (uint32_t)QST) ok = mbar_wait(&q_empty[st], ((qx / QST) - 1) & 1, &abort_flag);
+                        // a row that saw nothing counts nothing
+                        s_lse[st][t128] = ls == -INFINITY ? INFINITY : ls * 1.4426950408889634f;
+                        ok = group_all(1, ok);
+                    }
+#pragma unroll
+                    for (int k = 0; k < BATCH; k++) {
+                        const uint32_t i = t128 + (part * BATCH + k) * 128, r = i / CH, c = i % CH;
+                        const uint32_t at = (c / 8) * (128 * 128) + sw128(r, c & 7);
+                        uint4 hi = raw[k][0], lo = make_uint4(0, 0, 0, 0);
+                        if (SPLIT) {
+                            const uint4 g = raw[k][W - 1];
+                            split_pack<TC>(__uint_as_float(raw[k][0].x), __uint_as_float(raw[k][0].y), hi.x, lo.x);
+                            split_pack<TC>(__uint_as_float(raw[k][0].z), __uint_as_float(raw[k][0].w), hi.y, lo.y);
+                            split_pack<TC>(__uint_as_float(g.x), __uint_as_float(g.y), hi.z, lo.z);
+                            split_pack<TC>(__uint_as_float(g.z), __uint_as_float(g.w), hi.w, lo.w);
+                        }
+                        // where nothing counts the products are kept finite
+                        if (s_lse[st][r] == INFINITY) hi = lo = make_uint4(0, 0, 0, 0);
+                        *reinterpret_cast<uint4 *>(dst + at) = hi;
+                        if (SPLIT) *reinterpret_cast<uint4 *>(dst + G::TILE + at) = lo;
                     }
                 }
+                if (!ok) break;
                 fence_async_smem();
                 mbar_arrive(&q_full[st]);
                 qx++;
@@ -352,16 +368,22 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
                 }
                 const float *ls = s_lse[qx % QST];
                 f32x2 acc = pack2(0.f, 0.f);
-                for (uint32_t c0 = 0; c0 < nr; c0 += 32) {
-                    float v[32];
-                    tmem_ld32(ts + buf * 128 + c0, v);
+                // 32 columns at a time, the next 32 on their way from tensor memory
+                float v[2][32];
+                tmem_ld32(ts + buf * 128, v[0]);
+#pragma unroll
+                for (int ch = 0; ch < 4; ch++) {
+                    const uint32_t c0 = ch * 32;
+                    if (c0 >= nr) break;
                     tmem_wait_ld();
+                    if (ch < 3 && c0 + 32 < nr) tmem_ld32(ts + buf * 128 + c0 + 32, v[(ch + 1) & 1]);
+                    const float *w = v[ch & 1];
 #pragma unroll
                     for (int i = 0; i < 32; i += 4) {
                         const float4 l4 = *reinterpret_cast<const float4 *>(ls + c0 + i);
                         float u0, u1, u2, u3;
-                        unpack2(fma2(pack2(v[i], v[i + 1]), cc, pack2(-l4.x, -l4.y)), u0, u1);
-                        unpack2(fma2(pack2(v[i + 2], v[i + 3]), cc, pack2(-l4.z, -l4.w)), u2, u3);
+                        unpack2(fma2(pack2(w[i], w[i + 1]), cc, pack2(-l4.x, -l4.y)), u0, u1);
+                        unpack2(fma2(pack2(w[i + 2], w[i + 3]), cc, pack2(-l4.z, -l4.w)), u2, u3);
                         if (masked) {
                             const int c = (int)c0 + i;
                             u0 = (c >= clo && c < chi) ? u0 : -INFINITY;
@@ -375,9 +397,9 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
                 }
                 tc_fence_before();
                 mbar_arrive(&s_empty[s][buf]);
-                float u, v;
-                unpack2(acc, u, v);
-                sum += u + v;
+                float even, odd;
+                unpack2(acc, even, odd);
+                sum += even + odd;
             }
             if (ok && k < t.n) {
                 if (a.page(t.b, k >> a.page_shift) < 0) sum = 0.f;  // a hole gathers nothing
