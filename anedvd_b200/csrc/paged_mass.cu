@@ -29,7 +29,7 @@ __device__ int g_timeout;
 
 constexpr int NT = 448;
 constexpr int ITEM = 256;         // slots
-constexpr int MAX_SEQS = 4096;    // sequences of one launch (the item table)
+constexpr int MAX_SEQS = 1024;    // sequences of one launch (the table in shared memory)
 
 template <int HD, bool SPLIT>
 struct MassGeo {
@@ -37,7 +37,7 @@ struct MassGeo {
     static constexpr int TILE = 128 * HD * 2;
     static constexpr int Q = TILE * (SPLIT ? 2 : 1);
     static constexpr int QST = (HD == 128 ? 2 : 4) / (SPLIT ? 2 : 1);
-    static constexpr int SMEM = 1024 + 4 * TILE + QST * Q + MAX_SEQS * 4;
+    static constexpr int SMEM = 1024 + 4 * TILE + QST * Q + MAX_SEQS * 16;
 };
 
 struct MassArgs {
@@ -66,13 +66,14 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
     constexpr int QST = G::QST;
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t k_full[2], k_empty[2], q_full[QST], q_empty[QST], s_full[2][2], s_empty[2][2];
-    __shared__ float s_lse[QST][128];
+    __shared__ float s_nlse[QST][128];  // -lse log2 e; -inf where a row counts nothing
     __shared__ float s_red[ITEM];
     __shared__ uint32_t s_scan[NT / 32], tmem_slot;
     __shared__ int abort_flag;
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t *kring = smem, *qring = smem + 4 * G::TILE;
-    uint32_t *s_ends = reinterpret_cast<uint32_t *>(qring + QST * G::Q);  // items of sequences 0..i, per KV head
+    // per sequence: items of the sequences up to it (per KV head), slots, first token row, tokens
+    uint4 *s_seq = reinterpret_cast<uint4 *>(qring + QST * G::Q);
     const PagedArgs &a = p.a;
     const PagedQuery &q = p.q;
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = warp_index();
@@ -101,7 +102,12 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
     uint32_t run = 0;
     for (uint32_t s0 = 0; s0 < p.seqs; s0 += NT) {
         const uint32_t i = s0 + tid;
-        uint32_t v = i < p.seqs ? (a.len(p.seq0 + i) + ITEM - 1) / ITEM : 0;
+        uint32_t len = 0, nq = 0, first = 0;
+        if (i < p.seqs) {
+            len = a.len(p.seq0 + i);
+            nq = a.tokens(p.seq0 + i, first);
+        }
+        uint32_t v = (len + ITEM - 1) / ITEM;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
             const uint32_t up = __shfl_up_sync(~0u, v, d);
@@ -114,7 +120,7 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
             if (w < warp) before += s_scan[w];
             run += s_scan[w];
         }
-        if (i < p.seqs) s_ends[i] = before + v;
+        if (i < p.seqs) s_seq[i] = make_uint4(before + v, len, first, nq);
         __syncthreads();
     }
     tc_fence_before();
@@ -135,17 +141,19 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
         uint32_t lo = 0, hi = p.seqs - 1;
         while (lo < hi) {
             const uint32_t mid = (lo + hi) / 2;
-            if ((uint64_t)s_ends[mid] * a.kv_heads > x)
+            if ((uint64_t)s_seq[mid].x * a.kv_heads > x)
                 hi = mid;
             else
                 lo = mid + 1;
         }
-        const uint32_t base = lo ? s_ends[lo - 1] : 0, cnt = s_ends[lo] - base, y = x - base * a.kv_heads;
+        const uint4 seq = s_seq[lo];
+        const uint32_t base = lo ? s_seq[lo - 1].x : 0, cnt = seq.x - base, y = x - base * a.kv_heads;
         t.b = p.seq0 + lo;
         t.h = y / cnt;
         t.k0 = (y % cnt) * ITEM;
-        t.n = a.len(t.b);
-        const uint32_t nq = a.tokens(t.b, t.first);
+        t.n = seq.y;
+        t.first = seq.z;
+        const uint32_t nq = seq.w;
         t.pos0 = (int)t.n - (int)nq;
         t.tq = min(nq, a.max_q);
         t.i0 = (p.last_q && nq > p.last_q) ? nq - p.last_q : 0;
@@ -292,7 +300,7 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
                     if (part == 0) {
                         if (qx >= (uint32_t)QST) ok = mbar_wait(&q_empty[st], ((qx / QST) - 1) & 1, &abort_flag);
                         // a row that saw nothing counts nothing
-                        s_lse[st][t128] = ls == -INFINITY ? INFINITY : ls * 1.4426950408889634f;
+                        s_nlse[st][t128] = ls == -INFINITY ? -INFINITY : -ls * 1.4426950408889634f;
                         ok = group_all(1, ok);
                     }
 #pragma unroll
@@ -308,7 +316,7 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
                             split_pack<TC>(__uint_as_float(g.z), __uint_as_float(g.w), hi.w, lo.w);
                         }
                         // where nothing counts the products are kept finite
-                        if (s_lse[st][r] == INFINITY) hi = lo = make_uint4(0, 0, 0, 0);
+                        if (s_nlse[st][r] == -INFINITY) hi = lo = make_uint4(0, 0, 0, 0);
                         *reinterpret_cast<uint4 *>(dst + at) = hi;
                         if (SPLIT) *reinterpret_cast<uint4 *>(dst + G::TILE + at) = lo;
                     }
@@ -334,6 +342,25 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
             item(x, t);
             const uint32_t k = t.k0 + s * 128 + t128;       // this thread's slot
             const uint32_t kw = k - lane;                   // its warp's first
+            // rows (of those that count) [vlo, vhi) see slot k; all the warp's slots are seen by [wlo, whi)
+            const int R = (int)((t.tq - min(t.i0, t.tq)) * q.group);
+            int vlo = 0, vhi = R, wlo = 0, whi = R;
+            if (q.causal) {
+                auto row = [&](long long i) { return (int)max(0ll, min((long long)R, (i - t.i0) * q.group)); };
+                vlo = row((long long)k - t.pos0);
+                wlo = row((long long)kw + 31 - t.pos0);
+                if (q.window) {
+                    vhi = row((long long)k + q.window - t.pos0);
+                    whi = row((long long)kw + q.window - t.pos0);
+                }
+            }
+            float *const m = p.mass + ((size_t)t.b * a.kv_heads + t.h) * p.mass_stride + k;
+            float old = 0.f;
+            bool there = false;  // a hole gathers nothing
+            if (k < t.n) {
+                there = a.page(t.b, k >> a.page_shift) >= 0;
+                if (ranks == 1 && p.decay != 0.f) old = p.decay * *m;
+            }
             float sum = 0.f;
             for (uint32_t e = 0; e < t.steps; e++, st++) {
                 const uint32_t qt = t.qt0 + rank + e * ranks;
@@ -351,63 +378,56 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
                 ok = mbar_wait(&s_full[s][buf], (st >> 1) & 1, &abort_flag);
                 if (!ok) break;
                 tc_fence_after();
-                // columns [clo, chi) see slot k; the warp's slots are kw .. kw + 31
-                int clo = 0, chi = (int)nr;
-                bool masked = false;
-                if (q.causal) {
-                    auto col = [&](long long i) {  // token i's first column, cut to the tile
-                        const long long v = i * q.group - (long long)r0;
-                        return (int)max(0ll, min((long long)nr, v));
-                    };
-                    clo = col((long long)k - t.pos0);
-                    masked = col((long long)kw + 31 - t.pos0) > 0;
-                    if (q.window) {
-                        chi = col((long long)k + q.window - t.pos0);
-                        masked |= col((long long)kw + q.window - t.pos0) < (int)nr;
-                    }
-                }
-                const float *ls = s_lse[qx % QST];
-                f32x2 acc = pack2(0.f, 0.f);
+                const int r_tile = (int)(qt * 128), clo = vlo - r_tile, chi = vhi - r_tile;
+                const bool masked = wlo > r_tile || whi < r_tile + (int)nr;
+                const float *nl = s_nlse[qx % QST];
+                f32x2 acc = pack2(0.f, 0.f), acc1 = acc;
                 // 32 columns at a time, the next 32 on their way from tensor memory
                 float v[2][32];
                 tmem_ld32(ts + buf * 128, v[0]);
 #pragma unroll
                 for (int ch = 0; ch < 4; ch++) {
-                    const uint32_t c0 = ch * 32;
-                    if (c0 >= nr) break;
+                    const int c0 = ch * 32;
+                    if (c0 >= (int)nr) break;
                     tmem_wait_ld();
-                    if (ch < 3 && c0 + 32 < nr) tmem_ld32(ts + buf * 128 + c0 + 32, v[(ch + 1) & 1]);
-                    const float *w = v[ch & 1];
+                    if (ch < 3 && c0 + 32 < (int)nr) tmem_ld32(ts + buf * 128 + c0 + 32, v[(ch + 1) & 1]);
+                    float *w = v[ch & 1];
+                    f32x2 n2[16];
 #pragma unroll
                     for (int i = 0; i < 32; i += 4) {
-                        const float4 l4 = *reinterpret_cast<const float4 *>(ls + c0 + i);
-                        float u0, u1, u2, u3;
-                        unpack2(fma2(pack2(w[i], w[i + 1]), cc, pack2(-l4.x, -l4.y)), u0, u1);
-                        unpack2(fma2(pack2(w[i + 2], w[i + 3]), cc, pack2(-l4.z, -l4.w)), u2, u3);
-                        if (masked) {
-                            const int c = (int)c0 + i;
-                            u0 = (c >= clo && c < chi) ? u0 : -INFINITY;
-                            u1 = (c + 1 >= clo && c + 1 < chi) ? u1 : -INFINITY;
-                            u2 = (c + 2 >= clo && c + 2 < chi) ? u2 : -INFINITY;
-                            u3 = (c + 3 >= clo && c + 3 < chi) ? u3 : -INFINITY;
+                        const float4 l4 = *reinterpret_cast<const float4 *>(nl + c0 + i);
+                        n2[i / 2] = pack2(l4.x, l4.y);
+                        n2[i / 2 + 1] = pack2(l4.z, l4.w);
+                    }
+                    if (masked) {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) {
+                            float u0, u1;
+                            unpack2(fma2(pack2(w[i], w[i + 1]), cc, n2[i / 2]), u0, u1);
+                            u0 = (c0 + i >= clo && c0 + i < chi) ? u0 : -INFINITY;
+                            u1 = (c0 + i + 1 >= clo && c0 + i + 1 < chi) ? u1 : -INFINITY;
+                            acc = add2(acc, pack2(ex2(u0), ex2(u1)));
                         }
-                        acc = add2(acc, pack2(ex2(u0), ex2(u1)));
-                        acc = add2(acc, pack2(ex2(u2), ex2(u3)));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            float u0, u1, u2, u3;
+                            unpack2(fma2(pack2(w[i], w[i + 1]), cc, n2[i / 2]), u0, u1);
+                            unpack2(fma2(pack2(w[i + 2], w[i + 3]), cc, n2[i / 2 + 1]), u2, u3);
+                            acc = add2(acc, pack2(ex2(u0), ex2(u1)));
+                            acc1 = add2(acc1, pack2(ex2(u2), ex2(u3)));
+                        }
                     }
                 }
+                acc = add2(acc, acc1);
                 tc_fence_before();
                 mbar_arrive(&s_empty[s][buf]);
                 float even, odd;
                 unpack2(acc, even, odd);
                 sum += even + odd;
             }
-            if (ok && k < t.n) {
-                if (a.page(t.b, k >> a.page_shift) < 0) sum = 0.f;  // a hole gathers nothing
-                if (ranks == 1) {
-                    float *m = p.mass + ((size_t)t.b * a.kv_heads + t.h) * p.mass_stride + k;
-                    *m = p.decay == 0.f ? sum : p.decay * *m + sum;
-                }
-            }
+            if (!there) sum = 0.f;
+            if (ok && ranks == 1 && k < t.n) *m = old + sum;
             if (ranks > 1) s_red[s * 128 + t128] = sum;
         }
         if (ok && held) mbar_arrive(&q_empty[qx % QST]);
