@@ -588,7 +588,7 @@ int check_query(const char *who, const cuq_paged_kv *kv, uint32_t n_tok, const v
     out.group_inv = (uint32_t)((0x100000000ull + out.group - 1) / out.group);
     out.scale = scale;
     out.causal = causal ? 1 : 0;
-    out.window = window < (1u << 30) ? window : (1u << 30);  // slots are below 2^30
+    out.window = window < (1u << 30) ? window : (1u << 30) - 1;  // slots are below 2^30
     return CUQ_OK;
 }
 

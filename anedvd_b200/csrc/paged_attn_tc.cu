@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(NT, 1) attn_many_kernel(PagedArgs a, PagedQuer
             }
             fence_async_smem();
             mbar_arrive(&bars.q_full[s]);
-            group_sync(s + 1);
+            group_sync<128>(s + 1);
             hole = s_hole[s];
 
             const uint32_t rr = row0 + s * 128 + t;
@@ -433,7 +433,7 @@ __global__ void __launch_bounds__(NT, 1) attn_many_kernel(PagedArgs a, PagedQuer
                 inv = l == 0.f ? 0.f : 1.f / l;
                 if (l != 0.f) lse2 = m * c2 + log2f(l);
             }
-            ok = group_all(s + 1, ok);
+            ok = group_all<128>(s + 1, ok);
             const bool direct = o.plan.many_splits == 1;
             uint32_t tok, head;
             row_of(t, tok, head);
@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(NT, 1) attn_many_kernel(PagedArgs a, PagedQuer
                         }
                         *reinterpret_cast<uint4 *>(sq + sw128(t, c)) = u;
                     }
-                    group_sync(s + 1);
+                    group_sync<128>(s + 1);
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
                         const uint32_t r = e * 16 + t / 8, c = t & 7;
@@ -481,7 +481,7 @@ __global__ void __launch_bounds__(NT, 1) attn_many_kernel(PagedArgs a, PagedQuer
                                                        (size_t)(kvh * q.group + hd) * row_step + c0 + c * (16 / sizeof(TO))) =
                                 *reinterpret_cast<const uint4 *>(sq + sw128(r, c));
                     }
-                    group_sync(s + 1);
+                    group_sync<128>(s + 1);
                 }
             };
             if (ok && direct) leave(reinterpret_cast<TQ *>(o.out), o.out_stride, (size_t)HD);

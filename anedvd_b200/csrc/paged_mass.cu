@@ -8,11 +8,12 @@
 //
 // An item is 256 slots of one KV head of one sequence, two 128-slot streams that
 // share the query tiles (128 (token, head) rows).  Persistent CTAs walk items:
-//   * warp 9 loads K pages by TMA (a ring of two items);
-//   * warps 10-13 gather query rows and their lse into a ring of query tiles; a
+//   * warp 17 loads K pages by TMA (a ring of two items);
+//   * warps 18-21 gather query rows and their lse into a ring of query tiles; a
 //     tile that the next item uses again stays where it is;
-//   * one lane of warp 8 issues S^T into two TMEM buffers per stream;
-//   * warps 0-3 and 4-7 sum 2^(S c - lse log2 e) over the columns.
+//   * warp 16 issues S^T into two TMEM buffers per stream;
+//   * warps 0-15 sum 2^(S c - lse log2 e) over the columns, two threads a slot, 64
+//     columns each: four warps a scheduler hide one another's waits.
 // Few queries: bound by the bytes of K, with only the columns that hold queries
 // computed.  Many: by the exponentials (16 a cycle and SM); then the query tiles of
 // an item are dealt out over a cluster, whose CTAs' sums are joined in rank order
@@ -27,8 +28,9 @@ namespace {
 
 __device__ int g_timeout;
 
-constexpr int NT = 448;
+constexpr int NT = 704;  // warps 0-15 sums, 16 MMA, 17 TMA, 18-21 query tiles
 constexpr int ITEM = 256;         // slots
+constexpr int LISTED = 64;        // items of a CTA that are worked out at its start
 constexpr int MAX_SEQS = 1024;    // sequences of one launch (the table in shared memory)
 
 template <int HD, bool SPLIT>
@@ -36,8 +38,21 @@ struct MassGeo {
     static constexpr int CB = HD / 64;
     static constexpr int TILE = 128 * HD * 2;
     static constexpr int Q = TILE * (SPLIT ? 2 : 1);
-    static constexpr int QST = (HD == 128 ? 2 : 4) / (SPLIT ? 2 : 1);
-    static constexpr int SMEM = 1024 + 4 * TILE + QST * Q + MAX_SEQS * 16;
+    static constexpr int UNITS = 6;  // tiles of shared memory, dealt out to keys and queries (see KQ)
+    static constexpr int SMEM = 1024 + UNITS * TILE + MAX_SEQS * 16;
+};
+
+// How the tiles are dealt out: few queries stay while keys stream, two items of
+// keys (4 tiles) and 2 of queries; many stream over one item's keys, 2 and 4.
+// A query tile of fp32 takes two.
+struct KQ {
+    uint32_t k_items, q_log;  // stages: items of keys, log2 of query tiles
+    __device__ __forceinline__ KQ(bool near, bool split) : k_items(near ? 2 : 1), q_log((near ? 1 : 2) - (split ? 1 : 0)) {}
+    __device__ __forceinline__ uint32_t k_stage(uint32_t x) const { return k_items == 2 ? x & 1 : 0; }
+    __device__ __forceinline__ uint32_t k_phase(uint32_t x) const { return (k_items == 2 ? x >> 1 : x) & 1; }
+    __device__ __forceinline__ uint32_t q_stage(uint32_t x) const { return x & ((1u << q_log) - 1); }
+    __device__ __forceinline__ uint32_t q_phase(uint32_t x) const { return (x >> q_log) & 1; }
+    __device__ __forceinline__ bool q_reused(uint32_t x) const { return x >= (1u << q_log); }
 };
 
 struct MassArgs {
@@ -63,17 +78,23 @@ template <typename TQ, typename TC, int HD>
 __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_constant__ CUtensorMap mk) {
     constexpr bool SPLIT = std::is_same<TQ, float>::value;
     using G = MassGeo<HD, SPLIT>;
-    constexpr int QST = G::QST;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t k_full[2], k_empty[2], q_full[QST], q_empty[QST], s_full[2][2], s_empty[2][2];
-    __shared__ float s_nlse[QST][128];  // -lse log2 e; -inf where a row counts nothing
-    __shared__ float s_red[ITEM];
-    __shared__ uint32_t s_scan[NT / 32], tmem_slot;
+    __shared__ uint64_t k_full[2], k_empty[2], q_full[4], q_empty[4], s_full[2][2], s_empty[2][2];
+    // -lse log2 e of the rows of query tile i at [i % 8]; -inf where a row counts
+    // nothing.  A tile is written once the products of the tile 4 (or fewer) before it
+    // are done, and those are at most two steps ahead of the sums: 4 + 2 < 8 tiles.
+    __shared__ float s_nlse[8][128];
+    __shared__ float s_red[2][ITEM];
+    __shared__ Item s_items[LISTED];
+    __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    uint8_t *kring = smem, *qring = smem + 4 * G::TILE;
+    const uint32_t most = p.last_q ? min(p.last_q, p.a.max_q) : p.a.max_q;
+    const bool near = (uint64_t)most * p.q.group <= 128;
+    const KQ ring(near, SPLIT);
+    uint8_t *kring = smem, *qring = smem + 2 * ring.k_items * G::TILE;
     // per sequence: items of the sequences up to it (per KV head), slots, first token row, tokens
-    uint4 *s_seq = reinterpret_cast<uint4 *>(qring + QST * G::Q);
+    uint4 *s_seq = reinterpret_cast<uint4 *>(smem + G::UNITS * G::TILE);
     const PagedArgs &a = p.a;
     const PagedQuery &q = p.q;
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = warp_index();
@@ -81,62 +102,53 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
 
-    if (warp == 8) tmem_alloc512(&tmem_slot);
+    if (warp == 16) tmem_alloc512(&tmem_slot);
     if (tid == 0) {
         abort_flag = 0;
         for (int i = 0; i < 2; i++) {
             mbar_init(&k_full[i], 1);
             mbar_init(&k_empty[i], 1);
             for (int s = 0; s < 2; s++) {
-                mbar_init(&s_full[s][i], 1);
-                mbar_init(&s_empty[s][i], 128);
+                mbar_init(&s_full[s][i], 2);
+                mbar_init(&s_empty[s][i], 256);
             }
         }
-        for (int i = 0; i < QST; i++) {
+        for (int i = 0; i < 4; i++) {
             mbar_init(&q_full[i], 128);
-            mbar_init(&q_empty[i], 1 + 256);
+            mbar_init(&q_empty[i], 1);
         }
         mbar_init_fence();
     }
-    // the item table: running sums of ceil(len / 256)
-    uint32_t run = 0;
-    for (uint32_t s0 = 0; s0 < p.seqs; s0 += NT) {
-        const uint32_t i = s0 + tid;
-        uint32_t len = 0, nq = 0, first = 0;
-        if (i < p.seqs) {
-            len = a.len(p.seq0 + i);
-            nq = a.tokens(p.seq0 + i, first);
-        }
-        uint32_t v = (len + ITEM - 1) / ITEM;
+    // the sequence table: running sums of ceil(len / 256)
+    if (warp == 0) {
+        uint32_t run = 0;
+        for (uint32_t s0 = 0; s0 < p.seqs; s0 += 32) {
+            const uint32_t i = s0 + lane;
+            uint32_t len = 0, nq = 0, first = 0;
+            if (i < p.seqs) {
+                len = a.len(p.seq0 + i);
+                nq = a.tokens(p.seq0 + i, first);
+            }
+            uint32_t v = (len + ITEM - 1) / ITEM;
 #pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const uint32_t up = __shfl_up_sync(~0u, v, d);
-            if (lane >= (uint32_t)d) v += up;
+            for (int d = 1; d < 32; d <<= 1) {
+                const uint32_t up = __shfl_up_sync(~0u, v, d);
+                if (lane >= (uint32_t)d) v += up;
+            }
+            if (i < p.seqs) s_seq[i] = make_uint4(run + v, len, first, nq);
+            run += __shfl_sync(~0u, v, 31);
         }
-        if (lane == 31) s_scan[warp] = v;
-        __syncthreads();
-        uint32_t before = run;
-        for (uint32_t w = 0; w < NT / 32; w++) {
-            if (w < warp) before += s_scan[w];
-            run += s_scan[w];
-        }
-        if (i < p.seqs) s_seq[i] = make_uint4(before + v, len, first, nq);
-        __syncthreads();
     }
-    tc_fence_before();
     __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = tmem_slot;
+    const uint32_t run = s_seq[p.seqs - 1].x;
     const uint32_t total = run * a.kv_heads;
     // few queries: neighbouring items, which share their query tile; else dealt out,
     // since a causal mask gives the first slots the most queries
     const uint32_t cluster = blockIdx.x / ranks, clusters = gridDim.x / ranks;
-    const uint32_t most = p.last_q ? min(p.last_q, a.max_q) : a.max_q;
-    const bool near = (uint64_t)most * q.group <= 128;
     const uint32_t per = near ? (total + clusters - 1) / clusters : 1;
     const uint32_t x0 = cluster * per, x1 = near ? min(total, x0 + per) : total, xs = near ? 1 : clusters;
 
-    auto item = [&](uint32_t x, Item &t) {
+    auto find = [&](uint32_t x, Item &t) {
         // sequence-major: find the sequence in the table, then its KV head and slots
         uint32_t lo = 0, hi = p.seqs - 1;
         while (lo < hi) {
@@ -172,10 +184,22 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
             }
         }
     };
+    for (uint32_t i = tid; i < (uint32_t)LISTED && x0 + (uint64_t)i * xs < x1; i += NT) find(x0 + i * xs, s_items[i]);
+    auto item = [&](uint32_t x, Item &t) {
+        const uint32_t i = near ? x - x0 : (x - x0) / xs;
+        if (i < (uint32_t)LISTED)
+            t = s_items[i];
+        else
+            find(x, t);
+    };
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
     // rows of query tile qt of item t
     auto tile_rows = [&](const Item &t, uint32_t qt) { return min(128u, (t.tq - t.i0) * q.group - qt * 128); };
 
-    if (warp == 8) {
+    if (warp == 16) {
         // ------------------------------------------------------ MMA issuer
         {
             const uint32_t leader = elect_one();
@@ -186,28 +210,28 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
                 Item t;
                 item(x, t);
                 if (!t.steps) continue;
-                ok = mbar_wait(&k_full[kx & 1], (kx >> 1) & 1, &abort_flag);
+                ok = mbar_wait(&k_full[ring.k_stage(kx)], ring.k_phase(kx), &abort_flag);
                 for (uint32_t e = 0; ok && e < t.steps; e++, st++) {
                     const uint32_t qt = t.qt0 + rank + e * ranks;
                     if (!held || t.b != ob || t.h != oh || qt != oq) {
                         if (held) {
-                            umma_commit(leader, &q_empty[qx % QST]);
+                            umma_commit(leader, &q_empty[ring.q_stage(qx)]);
                             qx++;
                         }
                         held = true;
                         ob = t.b, oh = t.h, oq = qt;
-                        ok = mbar_wait(&q_full[qx % QST], (qx / QST) & 1, &abort_flag);
+                        ok = mbar_wait(&q_full[ring.q_stage(qx)], ring.q_phase(qx), &abort_flag);
                         if (!ok) break;
                     }
                     const uint32_t nr = tile_rows(t, qt), id = idesc<TC>(128, (nr + 31) / 32 * 32, false);
-                    const uint32_t buf = st & 1, qb = qa + (qx % QST) * G::Q;
+                    const uint32_t buf = st & 1, qb = qa + ring.q_stage(qx) * G::Q;
                     for (uint32_t s = 0; s < 2; s++) {
                         if (st >= 2 && !mbar_wait(&s_empty[s][buf], ((st >> 1) - 1) & 1, &abort_flag)) {
                             ok = false;
                             break;
                         }
                         tc_fence_after();
-                        const uint32_t kb = ka + ((kx & 1) * 2 + s) * G::TILE;
+                        const uint32_t kb = ka + (ring.k_stage(kx) * 2 + s) * G::TILE;
 #pragma unroll
                         for (int part = 0; part < (SPLIT ? 2 : 1); part++)
 #pragma unroll
@@ -217,14 +241,15 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
                                         sdesc_sw128(qb + part * G::TILE + off, 16, 1024), id, part | ks ? 1u : 0u);
                             }
                         umma_commit(leader, &s_full[s][buf]);
+                        if (leader) mbar_arrive(&s_full[s][buf]);  // hands on what the query warps wrote to s_nlse
                     }
                 }
-                if (ok) umma_commit(leader, &k_empty[kx & 1]);
+                if (ok) umma_commit(leader, &k_empty[ring.k_stage(kx)]);
                 kx++;
             }
-            if (ok && held) umma_commit(leader, &q_empty[qx % QST]);
+            if (ok && held) umma_commit(leader, &q_empty[ring.q_stage(qx)]);
         }
-    } else if (warp == 9) {
+    } else if (warp == 17) {
         // ------------------------------------------------------ TMA: K pages
         const uint32_t box = min(a.page_size, 128u), nbox = ITEM / box;
         uint32_t kx = 0;
@@ -233,13 +258,13 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
             Item t;
             item(x, t);
             if (!t.steps) continue;
-            const uint32_t st = kx & 1, slot = t.k0 + lane * box;
+            const uint32_t st = ring.k_stage(kx), slot = t.k0 + lane * box;
             int pg = (int)a.n_pages;  // outside the pool: zeros
             if (lane < nbox && slot < t.n) {
                 pg = a.page(t.b, slot >> a.page_shift);
                 if (pg < 0) pg = (int)a.n_pages;
             }
-            if (kx >= 2) ok = mbar_wait(&k_empty[st], ((kx >> 1) - 1) & 1, &abort_flag);
+            if (kx >= ring.k_items) ok = mbar_wait(&k_empty[st], ring.k_phase(kx) ^ 1, &abort_flag);
             if (!ok) break;
             if (lane == 0) mbar_expect_tx(&k_full[st], 2 * G::TILE);
             __syncwarp();
@@ -253,13 +278,20 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
             }
             kx++;
         }
-        for (uint32_t i = kx > 2 ? kx - 2 : 0; ok && i < kx; i++)  // drain
-            ok = mbar_wait(&k_empty[i & 1], (i >> 1) & 1, &abort_flag);
-    } else if (warp >= 10) {
+        for (uint32_t i = kx > ring.k_items ? kx - ring.k_items : 0; ok && i < kx; i++)  // drain
+            ok = mbar_wait(&k_empty[ring.k_stage(i)], ring.k_phase(i), &abort_flag);
+    } else if (warp >= 18) {
         // ------------------------------------------------------ query tiles
-        const uint32_t t128 = tid - 320;
+        const uint32_t t128 = tid - 18 * 32;
         uint32_t qx = 0, ob = ~0u, oh = 0, oq = 0;
-        bool ok = true;
+        bool ok = true, pending = false;
+        auto send = [&]() {  // hand over the tile whose copies were issued last
+            if (!pending) return;
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            fence_async_smem();
+            mbar_arrive(&q_full[ring.q_stage(qx - 1)]);
+            pending = false;
+        };
         for (uint32_t x = x0; ok && x < x1; x += xs) {
             Item t;
             item(x, t);
@@ -267,7 +299,7 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
                 const uint32_t qt = t.qt0 + rank + e * ranks;
                 if (qx && t.b == ob && t.h == oh && qt == oq) continue;
                 ob = t.b, oh = t.h, oq = qt;
-                const uint32_t st = qx % QST, nr = tile_rows(t, qt), r0 = t.i0 * q.group + qt * 128;
+                const uint32_t st = ring.q_stage(qx), nr = tile_rows(t, qt), r0 = t.i0 * q.group + qt * 128;
                 const uint32_t tok0 = r0 / q.group, rem0 = r0 - tok0 * q.group;  // row r: (rem0 + r) / group tokens on
                 auto row_of = [&](uint32_t r, uint32_t &tok, uint32_t &head) {
                     const uint32_t y = rem0 + r;
@@ -282,138 +314,154 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
                     row_of(t128, tok, head);
                     ls = __ldg(p.lse + (size_t)(t.first + tok0 + tok) * q.heads + t.h * q.group + head);
                 }
-                // all of a thread's 16-byte chunks in flight, before the wait for the stage
-                constexpr int CH = HD / 8, W = SPLIT ? 2 : 1, BATCH = SPLIT ? CH / 2 : CH;
+                constexpr int CH = HD / 8, BATCH = 4;
                 uint8_t *dst = qring + st * G::Q;
-#pragma unroll 1
-                for (int part = 0; part < CH / BATCH; part++) {
-                    uint4 raw[BATCH][W];
+                if (ring.q_reused(qx) && !mbar_try_wait(&q_empty[st], ring.q_phase(qx) ^ 1)) {
+                    send();  // rather than hold the last tile back
+                    ok = mbar_wait(&q_empty[st], ring.q_phase(qx) ^ 1, &abort_flag);
+                }
+                // a row that saw nothing counts nothing, and its products are kept finite
+                s_nlse[qx & 7][t128] = ls == -INFINITY ? -INFINITY : -ls * 1.4426950408889634f;
+                ok = group_all<128>(1, ok);
+                if (!ok) break;
+                if constexpr (!SPLIT) {
 #pragma unroll
-                    for (int k = 0; k < BATCH; k++) {
-                        const uint32_t i = t128 + (part * BATCH + k) * 128, r = i / CH, c = i % CH;
+                    for (int k = 0; k < CH; k++) {
+                        const uint32_t i = t128 + k * 128, r = i / CH, c = i % CH;
                         uint32_t tok, head;
                         row_of(r, tok, head);
-                        const uint4 *src = reinterpret_cast<const uint4 *>(qb + (size_t)tok * q.q_stride + head * HD + c * 8);
-#pragma unroll
-                        for (int w = 0; w < W; w++) raw[k][w] = r < nr ? __ldg(src + w) : make_uint4(0, 0, 0, 0);
+                        const TQ *src = qb + (size_t)tok * q.q_stride + head * HD + c * 8;
+                        const bool in = s_nlse[qx & 7][r] != -INFINITY;
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                                         smem_u32(dst) + (c / 8) * (128 * 128) + sw128(r, c & 7)),
+                                     "l"(in ? src : qb), "r"(in ? 16 : 0)
+                                     : "memory");
                     }
-                    if (part == 0) {
-                        if (qx >= (uint32_t)QST) ok = mbar_wait(&q_empty[st], ((qx / QST) - 1) & 1, &abort_flag);
-                        // a row that saw nothing counts nothing
-                        s_nlse[st][t128] = ls == -INFINITY ? -INFINITY : -ls * 1.4426950408889634f;
-                        ok = group_all(1, ok);
+                    // the tile before this one goes out while this one is on its way
+                    asm volatile("cp.async.commit_group;" ::: "memory");
+                    if (pending) {
+                        asm volatile("cp.async.wait_group 1;" ::: "memory");
+                        fence_async_smem();
+                        mbar_arrive(&q_full[ring.q_stage(qx - 1)]);
                     }
+                    pending = true;
+                } else {
+#pragma unroll 1
+                    for (int part = 0; part < CH / BATCH; part++) {
+                        uint4 raw[BATCH][2];
 #pragma unroll
-                    for (int k = 0; k < BATCH; k++) {
-                        const uint32_t i = t128 + (part * BATCH + k) * 128, r = i / CH, c = i % CH;
-                        const uint32_t at = (c / 8) * (128 * 128) + sw128(r, c & 7);
-                        uint4 hi = raw[k][0], lo = make_uint4(0, 0, 0, 0);
-                        if (SPLIT) {
-                            const uint4 g = raw[k][W - 1];
-                            split_pack<TC>(__uint_as_float(raw[k][0].x), __uint_as_float(raw[k][0].y), hi.x, lo.x);
-                            split_pack<TC>(__uint_as_float(raw[k][0].z), __uint_as_float(raw[k][0].w), hi.y, lo.y);
+                        for (int k = 0; k < BATCH; k++) {
+                            const uint32_t i = t128 + (part * BATCH + k) * 128, r = i / CH, c = i % CH;
+                            uint32_t tok, head;
+                            row_of(r, tok, head);
+                            const uint4 *src =
+                                reinterpret_cast<const uint4 *>(qb + (size_t)tok * q.q_stride + head * HD + c * 8);
+                            const bool in = s_nlse[qx & 7][r] != -INFINITY;
+                            raw[k][0] = in ? __ldg(src) : make_uint4(0, 0, 0, 0);
+                            raw[k][1] = in ? __ldg(src + 1) : make_uint4(0, 0, 0, 0);
+                        }
+#pragma unroll
+                        for (int k = 0; k < BATCH; k++) {
+                            const uint32_t i = t128 + (part * BATCH + k) * 128, r = i / CH, c = i % CH;
+                            const uint32_t at = (c / 8) * (128 * 128) + sw128(r, c & 7);
+                            const uint4 f = raw[k][0], g = raw[k][1];
+                            uint4 hi, lo;
+                            split_pack<TC>(__uint_as_float(f.x), __uint_as_float(f.y), hi.x, lo.x);
+                            split_pack<TC>(__uint_as_float(f.z), __uint_as_float(f.w), hi.y, lo.y);
                             split_pack<TC>(__uint_as_float(g.x), __uint_as_float(g.y), hi.z, lo.z);
                             split_pack<TC>(__uint_as_float(g.z), __uint_as_float(g.w), hi.w, lo.w);
+                            *reinterpret_cast<uint4 *>(dst + at) = hi;
+                            *reinterpret_cast<uint4 *>(dst + G::TILE + at) = lo;
                         }
-                        // where nothing counts the products are kept finite
-                        if (s_nlse[st][r] == -INFINITY) hi = lo = make_uint4(0, 0, 0, 0);
-                        *reinterpret_cast<uint4 *>(dst + at) = hi;
-                        if (SPLIT) *reinterpret_cast<uint4 *>(dst + G::TILE + at) = lo;
                     }
                 }
-                if (!ok) break;
-                fence_async_smem();
-                mbar_arrive(&q_full[st]);
+                if constexpr (SPLIT) {
+                    fence_async_smem();
+                    mbar_arrive(&q_full[st]);
+                }
                 qx++;
             }
         }
-        for (uint32_t i = qx > (uint32_t)QST ? qx - QST : 0; ok && i < qx; i++)  // drain
-            ok = mbar_wait(&q_empty[i % QST], (i / QST) & 1, &abort_flag);
+        send();
+        const uint32_t q_tiles = 1u << ring.q_log;
+        for (uint32_t i = qx > q_tiles ? qx - q_tiles : 0; ok && i < qx; i++)  // drain
+            ok = mbar_wait(&q_empty[ring.q_stage(i)], ring.q_phase(i), &abort_flag);
     } else {
         // ------------------------------------------------------ column sums
-        const uint32_t s = warp >> 2, t128 = tid & 127;
-        const uint32_t ts = tmem + s * 256 + ((warp & 3) << 21);
+        const uint32_t s = warp >> 3, half = (warp >> 2) & 1, t128 = tid & 127;
+        const int col0 = (int)half * 64;  // this thread's columns
+        const uint32_t ts = tmem + s * 256 + col0 + ((warp & 3) << 21);
         const float c2 = q.scale * 1.4426950408889634f;
         const f32x2 cc = pack2(c2, c2);
-        uint32_t qx = 0, st = 0, ob = ~0u, oh = 0, oq = 0;
+        uint32_t qx = 0, st = 0, ob = ~0u, oh = 0, oq = 0, flip = 0;
         bool ok = true, held = false;
         for (uint32_t x = x0; ok && x < x1; x += xs) {
             Item t;
             item(x, t);
             const uint32_t k = t.k0 + s * 128 + t128;       // this thread's slot
-            const uint32_t kw = k - lane;                   // its warp's first
             // rows (of those that count) [vlo, vhi) see slot k; all the warp's slots are seen by [wlo, whi)
-            const int R = (int)((t.tq - min(t.i0, t.tq)) * q.group);
+            const int T = (int)t.tq - (int)t.i0, R = max(T, 0) * (int)q.group;
             int vlo = 0, vhi = R, wlo = 0, whi = R;
-            if (q.causal) {
-                auto row = [&](long long i) { return (int)max(0ll, min((long long)R, (i - t.i0) * q.group)); };
-                vlo = row((long long)k - t.pos0);
-                wlo = row((long long)kw + 31 - t.pos0);
+            if (q.causal && T > 0) {
+                const int at = (int)k - (t.pos0 + (int)t.i0), w0 = at - (int)lane;  // against the first one's slot
+                auto row = [&](int i) { return max(0, min(T, i)) * (int)q.group; };
+                vlo = row(at);
+                wlo = row(w0 + 31);
                 if (q.window) {
-                    vhi = row((long long)k + q.window - t.pos0);
-                    whi = row((long long)kw + q.window - t.pos0);
+                    vhi = row(at + (int)q.window);
+                    whi = row(w0 + (int)q.window);
                 }
             }
             float *const m = p.mass + ((size_t)t.b * a.kv_heads + t.h) * p.mass_stride + k;
-            float old = 0.f;
-            bool there = false;  // a hole gathers nothing
-            if (k < t.n) {
-                there = a.page(t.b, k >> a.page_shift) >= 0;
+            float old = 0.f, sum = 0.f;
+            int page_id = -1;  // looked at when the sums are there
+            if (half == 0 && k < t.n) {
+                page_id = __ldg(a.pages + (size_t)t.b * a.pages_stride + (k >> a.page_shift));
                 if (ranks == 1 && p.decay != 0.f) old = p.decay * *m;
             }
-            float sum = 0.f;
             for (uint32_t e = 0; e < t.steps; e++, st++) {
                 const uint32_t qt = t.qt0 + rank + e * ranks;
                 if (!held || t.b != ob || t.h != oh || qt != oq) {
-                    if (held) {
-                        mbar_arrive(&q_empty[qx % QST]);
-                        qx++;
-                    }
+                    if (held) qx++;
                     held = true;
                     ob = t.b, oh = t.h, oq = qt;
-                    ok = mbar_wait(&q_full[qx % QST], (qx / QST) & 1, &abort_flag);
-                    if (!ok) break;
                 }
-                const uint32_t buf = st & 1, nr = tile_rows(t, qt), r0 = t.i0 * q.group + qt * 128;
+                const uint32_t buf = st & 1, nr = tile_rows(t, qt);
                 ok = mbar_wait(&s_full[s][buf], (st >> 1) & 1, &abort_flag);
                 if (!ok) break;
                 tc_fence_after();
-                const int r_tile = (int)(qt * 128), clo = vlo - r_tile, chi = vhi - r_tile;
-                const bool masked = wlo > r_tile || whi < r_tile + (int)nr;
-                const float *nl = s_nlse[qx % QST];
+                const int r_tile = (int)(qt * 128) + col0, clo = vlo - r_tile, chi = vhi - r_tile;
+                const int cols = (int)nr - col0;  // may be none
+                const bool masked = wlo > r_tile || whi < r_tile + min(cols, 64);
+                const float *nl = s_nlse[qx & 7] + col0;
                 f32x2 acc = pack2(0.f, 0.f), acc1 = acc;
-                // 32 columns at a time, the next 32 on their way from tensor memory
-                float v[2][32];
-                tmem_ld32(ts + buf * 128, v[0]);
 #pragma unroll
-                for (int ch = 0; ch < 4; ch++) {
+                for (int ch = 0; ch < 2; ch++) {
                     const int c0 = ch * 32;
-                    if (c0 >= (int)nr) break;
+                    if (c0 >= cols) break;
+                    float w[32];
+                    tmem_ld32(ts + buf * 128 + c0, w);
                     tmem_wait_ld();
-                    if (ch < 3 && c0 + 32 < (int)nr) tmem_ld32(ts + buf * 128 + c0 + 32, v[(ch + 1) & 1]);
-                    float *w = v[ch & 1];
-                    f32x2 n2[16];
-#pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        const float4 l4 = *reinterpret_cast<const float4 *>(nl + c0 + i);
-                        n2[i / 2] = pack2(l4.x, l4.y);
-                        n2[i / 2 + 1] = pack2(l4.z, l4.w);
-                    }
                     if (masked) {
 #pragma unroll
-                        for (int i = 0; i < 32; i += 2) {
-                            float u0, u1;
-                            unpack2(fma2(pack2(w[i], w[i + 1]), cc, n2[i / 2]), u0, u1);
-                            u0 = (c0 + i >= clo && c0 + i < chi) ? u0 : -INFINITY;
-                            u1 = (c0 + i + 1 >= clo && c0 + i + 1 < chi) ? u1 : -INFINITY;
-                            acc = add2(acc, pack2(ex2(u0), ex2(u1)));
+                        for (int i = 0; i < 32; i += 4) {
+                            const float4 l4 = *reinterpret_cast<const float4 *>(nl + c0 + i);
+                            float u[4];
+                            unpack2(fma2(pack2(w[i], w[i + 1]), cc, pack2(l4.x, l4.y)), u[0], u[1]);
+                            unpack2(fma2(pack2(w[i + 2], w[i + 3]), cc, pack2(l4.z, l4.w)), u[2], u[3]);
+#pragma unroll
+                            for (int k4 = 0; k4 < 4; k4++)
+                                u[k4] = (c0 + i + k4 >= clo && c0 + i + k4 < chi) ? u[k4] : -INFINITY;
+                            acc = add2(acc, pack2(ex2(u[0]), ex2(u[1])));
+                            acc1 = add2(acc1, pack2(ex2(u[2]), ex2(u[3])));
                         }
                     } else {
 #pragma unroll
                         for (int i = 0; i < 32; i += 4) {
+                            const float4 l4 = *reinterpret_cast<const float4 *>(nl + c0 + i);
                             float u0, u1, u2, u3;
-                            unpack2(fma2(pack2(w[i], w[i + 1]), cc, n2[i / 2]), u0, u1);
-                            unpack2(fma2(pack2(w[i + 2], w[i + 3]), cc, n2[i / 2 + 1]), u2, u3);
+                            unpack2(fma2(pack2(w[i], w[i + 1]), cc, pack2(l4.x, l4.y)), u0, u1);
+                            unpack2(fma2(pack2(w[i + 2], w[i + 3]), cc, pack2(l4.z, l4.w)), u2, u3);
                             acc = add2(acc, pack2(ex2(u0), ex2(u1)));
                             acc1 = add2(acc1, pack2(ex2(u2), ex2(u3)));
                         }
@@ -426,11 +474,19 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
                 unpack2(acc, even, odd);
                 sum += even + odd;
             }
-            if (!there) sum = 0.f;
-            if (ok && ranks == 1 && k < t.n) *m = old + sum;
-            if (ranks > 1) s_red[s * 128 + t128] = sum;
+            // the second half's sum goes to the first half's thread
+            float *red = s_red[flip] + s * 128 + t128;  // the other buffer next time
+            flip ^= 1;
+            if (half) *red = sum;
+            ok = group_all<256>(s + 2, ok);  // the stream's threads go on or stop together
+            if (!half) {
+                sum = (uint32_t)page_id < a.n_pages ? sum + *red : 0.f;  // a hole gathers nothing
+                if (ranks > 1)
+                    s_red[1][s * 128 + t128] = sum;
+                else if (k < t.n && ok)
+                    *m = old + sum;
+            }
         }
-        if (ok && held) mbar_arrive(&q_empty[qx % QST]);
     }
     tc_fence_before();
     __syncthreads();
@@ -440,7 +496,7 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
         while (now_ns() - t0 < 1000000ull) {
         }
     }
-    if (warp == 8) {
+    if (warp == 16) {
         tc_fence_after();
         tmem_free512(tmem);
     }
@@ -455,7 +511,7 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
             for (uint32_t r = 0; r < ranks; r++) {
                 uint32_t at;
                 float v;
-                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(&s_red[tid])), "r"(r));
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(&s_red[1][tid])), "r"(r));
                 asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
                 sum += v;
             }

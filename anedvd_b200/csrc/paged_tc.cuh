@@ -65,18 +65,22 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, volati
     return mbar_wait_slow(bar, parity, abort_flag);
 }
 
-// 128 threads that share named barrier `id`
-__device__ __forceinline__ void group_sync(uint32_t id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
+// N threads that share named barrier `id`
+template <int N>
+__device__ __forceinline__ void group_sync(uint32_t id) {
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(N) : "memory");
+}
 // whether `ok` holds in all of them (a wait may have given up in some)
+template <int N>
 __device__ __forceinline__ bool group_all(uint32_t id, bool ok) {
     uint32_t r;
     asm volatile(
         "{\n\t.reg .pred p, q;\n\t"
         "setp.ne.u32 p, %1, 0;\n\t"
-        "barrier.cta.red.and.pred q, %2, 128, p;\n\t"
+        "barrier.cta.red.and.pred q, %2, %3, p;\n\t"
         "selp.u32 %0, 1, 0, q;\n\t}"
         : "=r"(r)
-        : "r"((uint32_t)ok), "r"(id)
+        : "r"((uint32_t)ok), "r"(id), "n"(N)
         : "memory");
     return r != 0;
 }
