@@ -85,6 +85,7 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
     // are done, and those are at most two steps ahead of the sums: 4 + 2 < 8 tiles.
     __shared__ float s_nlse[8][128];
     __shared__ float s_red[2][ITEM];
+    __shared__ const void *s_row[2][128];  // the rows of a query tile; null where a row counts nothing
     __shared__ Item s_items[LISTED];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
@@ -300,19 +301,14 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
                 if (qx && t.b == ob && t.h == oh && qt == oq) continue;
                 ob = t.b, oh = t.h, oq = qt;
                 const uint32_t st = ring.q_stage(qx), nr = tile_rows(t, qt), r0 = t.i0 * q.group + qt * 128;
-                const uint32_t tok0 = r0 / q.group, rem0 = r0 - tok0 * q.group;  // row r: (rem0 + r) / group tokens on
-                auto row_of = [&](uint32_t r, uint32_t &tok, uint32_t &head) {
-                    const uint32_t y = rem0 + r;
-                    tok = q.div_group(y);
-                    head = y - tok * q.group;
-                };
-                const TQ *qb = reinterpret_cast<const TQ *>(q.q) + (size_t)(t.first + tok0) * q.q_stride +
-                               (size_t)t.h * q.group * HD;
+                // thread r: where row r of the tile lies, and its lse
                 float ls = -INFINITY;
+                const TQ *src = nullptr;
                 if (t128 < nr) {
-                    uint32_t tok, head;
-                    row_of(t128, tok, head);
-                    ls = __ldg(p.lse + (size_t)(t.first + tok0 + tok) * q.heads + t.h * q.group + head);
+                    const uint32_t tok = t.first + (r0 + t128) / q.group;
+                    const uint32_t head = t.h * q.group + (r0 + t128) % q.group;
+                    ls = __ldg(p.lse + (size_t)tok * q.heads + head);
+                    src = reinterpret_cast<const TQ *>(q.q) + (size_t)tok * q.q_stride + (size_t)head * HD;
                 }
                 constexpr int CH = HD / 8, BATCH = 4;
                 uint8_t *dst = qring + st * G::Q;
@@ -322,19 +318,19 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
                 }
                 // a row that saw nothing counts nothing, and its products are kept finite
                 s_nlse[qx & 7][t128] = ls == -INFINITY ? -INFINITY : -ls * 1.4426950408889634f;
+                s_row[qx & 1][t128] = ls == -INFINITY ? nullptr : src;
                 ok = group_all<128>(1, ok);
                 if (!ok) break;
+                // this thread's chunk of rows r1, r1 + 128 / CH, ...
+                const uint32_t r1 = t128 / CH, c = t128 % CH;
                 if constexpr (!SPLIT) {
 #pragma unroll
                     for (int k = 0; k < CH; k++) {
-                        const uint32_t i = t128 + k * 128, r = i / CH, c = i % CH;
-                        uint32_t tok, head;
-                        row_of(r, tok, head);
-                        const TQ *src = qb + (size_t)tok * q.q_stride + head * HD + c * 8;
-                        const bool in = s_nlse[qx & 7][r] != -INFINITY;
+                        const uint32_t r = r1 + k * (128 / CH);
+                        const TQ *row = reinterpret_cast<const TQ *>(s_row[qx & 1][r]);
                         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
                                          smem_u32(dst) + (c / 8) * (128 * 128) + sw128(r, c & 7)),
-                                     "l"(in ? src : qb), "r"(in ? 16 : 0)
+                                     "l"(row ? row + c * 8 : reinterpret_cast<const TQ *>(q.q)), "r"(row ? 16 : 0)
                                      : "memory");
                     }
                     // the tile before this one goes out while this one is on its way
@@ -351,18 +347,15 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
                         uint4 raw[BATCH][2];
 #pragma unroll
                         for (int k = 0; k < BATCH; k++) {
-                            const uint32_t i = t128 + (part * BATCH + k) * 128, r = i / CH, c = i % CH;
-                            uint32_t tok, head;
-                            row_of(r, tok, head);
-                            const uint4 *src =
-                                reinterpret_cast<const uint4 *>(qb + (size_t)tok * q.q_stride + head * HD + c * 8);
-                            const bool in = s_nlse[qx & 7][r] != -INFINITY;
-                            raw[k][0] = in ? __ldg(src) : make_uint4(0, 0, 0, 0);
-                            raw[k][1] = in ? __ldg(src + 1) : make_uint4(0, 0, 0, 0);
+                            const uint32_t r = r1 + (part * BATCH + k) * (128 / CH);
+                            const TQ *row = reinterpret_cast<const TQ *>(s_row[qx & 1][r]);
+                            const uint4 *from = reinterpret_cast<const uint4 *>(row + c * 8);
+                            raw[k][0] = row ? __ldg(from) : make_uint4(0, 0, 0, 0);
+                            raw[k][1] = row ? __ldg(from + 1) : make_uint4(0, 0, 0, 0);
                         }
 #pragma unroll
                         for (int k = 0; k < BATCH; k++) {
-                            const uint32_t i = t128 + (part * BATCH + k) * 128, r = i / CH, c = i % CH;
+                            const uint32_t r = r1 + (part * BATCH + k) * (128 / CH);
                             const uint32_t at = (c / 8) * (128 * 128) + sw128(r, c & 7);
                             const uint4 f = raw[k][0], g = raw[k][1];
                             uint4 hi, lo;
