@@ -4,6 +4,7 @@
 // paged_mass.cu.
 #include <cmath>
 #include <new>
+#include <type_traits>
 
 #include "paged.cuh"
 
@@ -33,10 +34,11 @@ namespace {
 // ------------------------------------------------- rotary + append ----
 //
 // Bound by HBM for prompts (every value is read and written once) and by
-// latency for a few tokens.  A CTA takes T tokens: its threads first work out
-// the T * rot/2 cosines and sines, one each, into shared memory, then walk the
-// (token, head, unit) triples, a unit being the 16 values that hold 8 whole
-// pairs: two 16-byte vectors at j and j + rot/2, or 16 values in a row.
+// latency for a few tokens.  A CTA takes T tokens: a warp each finds its
+// sequence, slot and page, the threads work out the T * rot/2 cosines and sines,
+// one each, into shared memory, and then walk the rows (token, head) in units:
+// the 16 values that hold 8 whole pairs, two 16-byte vectors at j and j + rot/2,
+// or 16 values in a row.
 struct RopeArgs {
     PagedArgs a;
     const int32_t *positions;
@@ -57,43 +59,47 @@ __device__ __forceinline__ void store_as(int type, void *base, size_t at, const 
         store8(reinterpret_cast<__nv_bfloat16 *>(base) + at, v);
 }
 
+template <typename T>
+__device__ constexpr int in_type_of() {
+    return sizeof(T) == 4 ? CUQ_F32 : std::is_same<T, __half>::value ? CUQ_F16 : CUQ_BF16;
+}
+
 constexpr int ROPE_THREADS = 256;
 
 template <typename TI, int HD, int T>
 __global__ void __launch_bounds__(ROPE_THREADS) rope_append_kernel(RopeArgs p, RopeTable tab, int out_type,
                                                                     int cache_type) {
-    __shared__ float2 cs[T][ROPE_MAX_PAIRS];
+    __shared__ __align__(16) float cs[T][4][ROPE_MAX_PAIRS / 8][2][2];
     __shared__ int s_pos[T], s_slot[T], s_page[T];
     __shared__ int s_seq[T];
-    const uint32_t tok0 = blockIdx.x * T;
-    // the sequence of a token: how many sequences end at or before it
-    for (int i = 0; i < T; i++) {
-        const int tok = (int)(tok0 + i);
-        int n = 0;
-        for (uint32_t base = 0; base < p.a.n_seqs; base += ROPE_THREADS) {
-            const uint32_t b = base + threadIdx.x;
-            n += __syncthreads_count(b < p.a.n_seqs && __ldg(p.a.q_start + b + 1) <= tok);
-        }
-        if (threadIdx.x == 0) {
+    constexpr uint32_t UNITS = HD / 16, STEP = ROPE_THREADS / UNITS;
+    const uint32_t tok0 = blockIdx.x * T, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t half = tab.rot / 2, u = threadIdx.x % UNITS;
+    if (warp < T) {
+        // the sequence of a token: how many sequences end at or before it
+        const int tok = (int)(tok0 + warp);
+        uint32_t n = 0;
+        for (uint32_t s = 0; s < p.a.n_seqs; s += 32)
+            n += __popc(__ballot_sync(~0u, s + lane < p.a.n_seqs && __ldg(p.a.q_start + s + lane + 1) <= tok));
+        if (lane == 0) {
             int seq = -1, slot = -1, page = -1;
-            if (n < (int)p.a.n_seqs && tok < (int)p.a.n_tok) {
+            if (n < p.a.n_seqs && tok < (int)p.a.n_tok) {
                 uint32_t first;
                 const uint32_t nq = p.a.tokens(n, first);
+                const int len = (int)p.a.len(n);
                 if ((uint32_t)tok >= first && (uint32_t)tok < first + nq) {
-                    seq = n;
-                    const int len = (int)p.a.len(n);
+                    seq = (int)n;
                     slot = len - (int)nq + (tok - (int)first);
                     if (slot >= 0) page = p.a.page(n, (uint32_t)slot >> p.a.page_shift);
                 }
             }
-            s_seq[i] = seq;
-            s_slot[i] = slot;
-            s_page[i] = page;
-            s_pos[i] = seq < 0 ? 0 : p.positions ? __ldg(p.positions + tok) : slot;
+            s_seq[warp] = seq;
+            s_slot[warp] = slot;
+            s_page[warp] = page;
+            s_pos[warp] = seq < 0 ? 0 : p.positions ? __ldg(p.positions + tok) : slot;
         }
     }
     __syncthreads();
-    const uint32_t half = tab.rot / 2;
     for (uint32_t i = threadIdx.x; i < T * half; i += ROPE_THREADS) {
         const uint32_t t = i / half, j = i % half;
         const int64_t turn = (int64_t)((uint64_t)(int64_t)s_pos[t] * tab.turns[j]);
@@ -102,70 +108,99 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_append_kernel(RopeArgs p, R
         const float x = (float)(int32_t)(turn >> 32) * 0x1p-31f;  // in units of pi
         float si, co;
         sincospif(x, &si, &co);
-        cs[t][j] = make_float2(co * tab.mul, si * tab.mul);
+        // pairs 2 m, 2 m + 1 of unit j / 8 at [m][unit]: neighbouring units read without bank conflicts
+        cs[t][(j % 8) / 2][j / 8][0][j & 1] = co * tab.mul;
+        cs[t][(j % 8) / 2][j / 8][1][j & 1] = si * tab.mul;
     }
     __syncthreads();
-    constexpr uint32_t UNITS = HD / 16;
-    const uint32_t rows = p.heads + 2 * p.a.kv_heads, rot_units = tab.rot / 16;
-    for (uint32_t i = threadIdx.x; i < T * rows * UNITS; i += ROPE_THREADS) {
-        const uint32_t t = i / (rows * UNITS), r = (i / UNITS) % rows, u = i % UNITS;
+    const uint32_t rows = p.heads + 2 * p.a.kv_heads;
+    const bool rot_unit = u < tab.rot / 16;
+    uint32_t t = 0, r = threadIdx.x / UNITS;
+    for (;; r += STEP) {
+        while (r >= rows) {
+            r -= rows;
+            t++;
+        }
+        if (t >= (uint32_t)T) break;
         const uint32_t tok = tok0 + t;
-        if (s_seq[t] < 0) continue;
-        const bool is_q = r < p.heads, is_k = !is_q && r < p.heads + p.a.kv_heads;
-        if (!is_q && s_page[t] < 0) continue;
-        const bool turn = u < rot_units && (is_q || is_k);
-        const uint32_t h = is_q ? r : is_k ? r - p.heads : r - p.heads - p.a.kv_heads;
-        const TI *src = reinterpret_cast<const TI *>(is_q ? p.q : is_k ? p.k : p.v) +
-                        (size_t)tok * (is_q ? p.q_stride : p.kv_stride) + (size_t)h * HD;
+        const bool is_q = r < p.heads, is_v = r >= p.heads + p.a.kv_heads, turn = rot_unit && !is_v;
+        if (s_seq[t] < 0 || (!is_q && s_page[t] < 0)) continue;
         const bool apart = turn && !tab.adjacent;
         const uint32_t e0 = apart ? 8 * u : 16 * u, e1 = apart ? half + 8 * u : 16 * u + 8;
-        float a[8], b[8];
-        load8(src + e0, a);
-        load8(src + e1, b);
-        if (apart) {
+        const TI *src;
+        void *to;
+        size_t at;
+        if (is_q) {
+            src = reinterpret_cast<const TI *>(p.q) + (size_t)tok * p.q_stride + (size_t)r * HD;
+            to = p.q_out;
+            at = (size_t)tok * p.q_out_stride + (size_t)r * HD;
+        } else {
+            const uint32_t h = r - p.heads - (is_v ? p.a.kv_heads : 0);
+            src = reinterpret_cast<const TI *>(is_v ? p.v : p.k) + (size_t)tok * p.kv_stride + (size_t)h * HD;
+            to = is_v ? p.a.v : p.a.k;
+            at = p.a.row<HD>(s_page[t], h, (uint32_t)s_slot[t]);
+        }
+        constexpr int W = sizeof(TI) == 4 ? 2 : 1;  // vectors of 8 values
+        uint4 ra[W], rb[W];
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float2 c = cs[t][8 * u + j];
-                const float x = a[j], y = b[j];
-                a[j] = x * c.x - y * c.y;
-                b[j] = x * c.y + y * c.x;
+        for (int w = 0; w < W; w++) {
+            ra[w] = *(reinterpret_cast<const uint4 *>(src + e0) + w);
+            rb[w] = *(reinterpret_cast<const uint4 *>(src + e1) + w);
+        }
+        const int type = is_q ? out_type : cache_type;
+        if (!turn && type == in_type_of<TI>()) {  // as it is
+#pragma unroll
+            for (int w = 0; w < W; w++) {
+                *(reinterpret_cast<uint4 *>(reinterpret_cast<TI *>(to) + at + e0) + w) = ra[w];
+                *(reinterpret_cast<uint4 *>(reinterpret_cast<TI *>(to) + at + e1) + w) = rb[w];
+            }
+            continue;
+        }
+        float a[8], b[8];
+        unpack8<TI>(ra, a);
+        unpack8<TI>(rb, b);
+        if (turn && !tab.adjacent) {
+#pragma unroll
+            for (int m = 0; m < 4; m++) {
+                const float4 c = *reinterpret_cast<const float4 *>(cs[t][m][u]);  // co, co, si, si
+                float x = a[2 * m], y = b[2 * m];
+                a[2 * m] = x * c.x - y * c.z;
+                b[2 * m] = x * c.z + y * c.x;
+                x = a[2 * m + 1], y = b[2 * m + 1];
+                a[2 * m + 1] = x * c.y - y * c.w;
+                b[2 * m + 1] = x * c.w + y * c.y;
             }
         } else if (turn) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const float2 c = cs[t][8 * u + j], d = cs[t][8 * u + 4 + j];
-                float x = a[2 * j], y = a[2 * j + 1];
-                a[2 * j] = x * c.x - y * c.y;
-                a[2 * j + 1] = x * c.y + y * c.x;
-                x = b[2 * j], y = b[2 * j + 1];
-                b[2 * j] = x * d.x - y * d.y;
-                b[2 * j + 1] = x * d.y + y * d.x;
+            for (int m = 0; m < 4; m++) {
+                const float4 c = *reinterpret_cast<const float4 *>(cs[t][m][u]);
+                float *v = m < 2 ? a + 4 * m : b + 4 * (m - 2);  // pairs 2 m, 2 m + 1
+                float x = v[0], y = v[1];
+                v[0] = x * c.x - y * c.z;
+                v[1] = x * c.z + y * c.x;
+                x = v[2], y = v[3];
+                v[2] = x * c.y - y * c.w;
+                v[3] = x * c.w + y * c.y;
             }
         }
-        if (is_q) {
-            const size_t at = (size_t)tok * p.q_out_stride + (size_t)h * HD;
-            store_as<TI>(out_type, p.q_out, at + e0, a);
-            store_as<TI>(out_type, p.q_out, at + e1, b);
-        } else {
-            const size_t at = p.a.row<HD>(s_page[t], h, (uint32_t)s_slot[t]);
-            void *pool = is_k ? p.a.k : p.a.v;
-            store_as<TI>(cache_type, pool, at + e0, a);
-            store_as<TI>(cache_type, pool, at + e1, b);
-        }
+        store_as<TI>(type, to, at + e0, a);
+        store_as<TI>(type, to, at + e1, b);
     }
 }
 
 template <typename TI>
 int launch_rope_append(const RopeArgs &p, const RopeTable &t, int out_type, int cache_type, uint32_t hd,
                        cudaStream_t s) {
+    // two tokens a CTA once there are CTAs enough: 4096 tokens take 24.6 us, with one
+    // each 28.6 and with four 26.7; 16 tokens 9.3 us with one, 9.4 with two
     const bool many = p.a.n_tok >= 1024;
-    const uint32_t grid = many ? (p.a.n_tok + 3) / 4 : p.a.n_tok;
+    const uint32_t grid = many ? (p.a.n_tok + 1) / 2 : p.a.n_tok;
     if (hd == 64 && many)
-        rope_append_kernel<TI, 64, 4><<<grid, ROPE_THREADS, 0, s>>>(p, t, out_type, cache_type);
+        rope_append_kernel<TI, 64, 2><<<grid, ROPE_THREADS, 0, s>>>(p, t, out_type, cache_type);
     else if (hd == 64)
         rope_append_kernel<TI, 64, 1><<<grid, ROPE_THREADS, 0, s>>>(p, t, out_type, cache_type);
     else if (many)
-        rope_append_kernel<TI, 128, 4><<<grid, ROPE_THREADS, 0, s>>>(p, t, out_type, cache_type);
+        rope_append_kernel<TI, 128, 2><<<grid, ROPE_THREADS, 0, s>>>(p, t, out_type, cache_type);
     else
         rope_append_kernel<TI, 128, 1><<<grid, ROPE_THREADS, 0, s>>>(p, t, out_type, cache_type);
     CUQ_CUDA_TRY(cudaGetLastError());

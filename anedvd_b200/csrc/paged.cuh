@@ -90,22 +90,29 @@ struct Pair<__nv_bfloat16> {
     }
 };
 
-// eight values of any of the three types, as fp32
+// eight values of any of the three types, as fp32: one 16-byte vector, or two of fp32
 template <typename T>
-__device__ __forceinline__ void load8(const T *p, float (&v)[8]) {
-    const uint4 u = __ldg(reinterpret_cast<const uint4 *>(p));
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+__device__ __forceinline__ void unpack8(const uint4 (&u)[sizeof(T) == 4 ? 2 : 1], float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        v[0] = __uint_as_float(u[0].x), v[1] = __uint_as_float(u[0].y), v[2] = __uint_as_float(u[0].z);
+        v[3] = __uint_as_float(u[0].w), v[4] = __uint_as_float(u[1].x), v[5] = __uint_as_float(u[1].y);
+        v[6] = __uint_as_float(u[1].z), v[7] = __uint_as_float(u[1].w);
+    } else {
+        const uint32_t w[4] = {u[0].x, u[0].y, u[0].z, u[0].w};
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float2 f = Pair<T>::unpack(w[i]);
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
+        for (int i = 0; i < 4; i++) {
+            const float2 f = Pair<T>::unpack(w[i]);
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+        }
     }
 }
-template <>
-__device__ __forceinline__ void load8<float>(const float *p, float (&v)[8]) {
-    const float4 a = __ldg(reinterpret_cast<const float4 *>(p)), b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+template <typename T>
+__device__ __forceinline__ void load8(const T *p, float (&v)[8]) {
+    uint4 u[sizeof(T) == 4 ? 2 : 1];
+#pragma unroll
+    for (int w = 0; w < (sizeof(T) == 4 ? 2 : 1); w++) u[w] = __ldg(reinterpret_cast<const uint4 *>(p) + w);
+    unpack8<T>(u, v);
 }
 template <typename T>
 __device__ __forceinline__ void store8(T *p, const float (&v)[8]) {
