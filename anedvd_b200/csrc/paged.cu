@@ -571,6 +571,8 @@ int check_paged(const char *who, const cuq_paged_kv *kv, const cuq_batch *b, boo
     CUQ_CHECK_ARG(b->n_tok <= 0x3FFFFFFFu && b->max_kv <= 0x3FFFFFFFu && b->max_q <= 0x3FFFFFFFu &&
                       b->pages_stride <= 0x3FFFFFFFu,
                   "%s: batch sizes past 2^30", who);
+    CUQ_CHECK_ARG((uint64_t)b->n_seqs * kv->kv_heads <= (1u << 24), "%s: %u sequences of %u KV heads pass 2^24", who,
+                  b->n_seqs, kv->kv_heads);
     if (b->n_seqs) {
         CUQ_CHECK_ARG(b->kv_len && b->pages && aligned4(b->kv_len) && aligned4(b->pages),
                       "%s: kv_len and pages must be given", who);
@@ -592,6 +594,9 @@ int check_paged(const char *who, const cuq_paged_kv *kv, const cuq_batch *b, boo
     a.max_q = b->max_q < b->n_tok ? b->max_q : b->n_tok;
     const uint64_t slots = (uint64_t)b->pages_stride * ps;
     a.max_kv = slots < b->max_kv ? (uint32_t)slots : b->max_kv;
+    CUQ_CHECK_ARG((uint64_t)b->n_seqs * kv->kv_heads * ((a.max_kv + 15) / 16) <= 0x7FFFFFFFu,
+                  "%s: %u sequences of %u KV heads and %u slots pass 2^31 blocks of 16", who, b->n_seqs, kv->kv_heads,
+                  a.max_kv);
     return CUQ_OK;
 }
 

@@ -131,8 +131,8 @@ __device__ __forceinline__ void store8<float>(float *p, const float (&v)[8]) {
 // major.  Sequences of up to ATTN_FEW rows per KV head go to the mma.sync kernel
 // (paged_attn.cu), whose tile is 16 rows and whose time is the cache's bytes;
 // larger ones to the tcgen05 kernel (paged_attn_tc.cu), 2 x 128 rows.  Both may
-// split the slots over CTAs: partial results, out normalised and the log2 of the
-// sum of exponentials, go to the workspace and are joined by the merge kernel.
+// split the slots: parts, out normalised and the log2 of the sum of exponentials,
+// go to the workspace and are joined by the merge kernel.
 constexpr uint32_t ATTN_FEW = 16;
 
 struct AttnPagedCall {
@@ -149,8 +149,9 @@ struct AttnPagedCall {
 // How a call is split; a function of the call's host-side sizes alone.
 struct AttnPlan {
     bool few, many;        // which kernels run
-    uint32_t few_chunk;    // slots per CTA of the mma.sync kernel
-    uint32_t few_splits, many_splits;
+    uint32_t few_ctas;     // of the mma.sync kernel; its warps share the blocks out evenly
+    uint32_t few_rows;     // rows of a part
+    uint32_t many_splits;
     uint32_t many_tiles;   // bound of the 256-row tiles of all sequences
     // whether a sequence of `tokens` attended tokens is the mma.sync kernel's
     __device__ __forceinline__ bool is_few(uint32_t tokens, uint32_t group) const {
@@ -166,8 +167,8 @@ struct AttnOut {
     void *out;
     size_t out_stride;
     float *lse;
-    // parts: normalised outputs [splits][rows][hd] and log2 sums [splits][rows];
-    // rows are [n_seqs][kv_heads][ATTN_FEW] of the few, [n_tok][heads] of the many
+    // parts: normalised outputs [part][rows][hd] and log2 sums [part][rows]; rows are
+    // few_rows of the few, [n_tok][heads] of the many
     float *few_o, *few_lse, *many_o, *many_lse;
     AttnPlan plan;
 };

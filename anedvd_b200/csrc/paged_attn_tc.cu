@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(NT, 1) attn_many_kernel(PagedArgs a, PagedQuer
                         const uint32_t dst = smem_u32(ring + st * G::TILE) + lane * box * 128;
 #pragma unroll
                         for (int cb = 0; cb < G::CB; cb++)
-                            tma_load_page(dst + cb * (KEYS * 128), v ? &mv : &mk, cb * 64, slot, (int)kvh, pg,
+                            tma_load_page(dst + cb * (KEYS * 128), v ? &mv : &mk, cb, slot, (int)kvh, pg,
                                           &bars.kv_full[st]);
                     }
                 }
@@ -507,8 +507,8 @@ int launch_many(const AttnPagedCall &c, const AttnOut &o, cudaStream_t s) {
     using G = ManyGeo<HD, std::is_same<TQ, float>::value>;
     const uint32_t box = c.a.page_size < KEYS ? c.a.page_size : KEYS;
     CUtensorMap mk, mv;
-    int rc = make_page_map(&mk, c.a.k, c.a, HD, c.cache_type, box);
-    if (rc == CUQ_OK) rc = make_page_map(&mv, c.a.v, c.a, HD, c.cache_type, box);
+    int rc = make_page_map(&mk, c.a.k, c.a, HD, c.cache_type, box, 1);
+    if (rc == CUQ_OK) rc = make_page_map(&mv, c.a.v, c.a, HD, c.cache_type, box, 1);
     if (rc) return rc;
     auto kern = attn_many_kernel<TQ, TC, HD>;
     CUQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM));

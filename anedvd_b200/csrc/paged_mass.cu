@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
                 const uint32_t dst = smem_u32(kring) + (st * 2 + row / 128) * G::TILE + (row & 127) * 128;
 #pragma unroll
                 for (int cb = 0; cb < G::CB; cb++)
-                    tma_load_page(dst + cb * (128 * 128), &mk, cb * 64, (int)(slot & (a.page_size - 1)), (int)t.h, pg,
+                    tma_load_page(dst + cb * (128 * 128), &mk, cb, (int)(slot & (a.page_size - 1)), (int)t.h, pg,
                                   &k_full[st]);
             }
             kx++;
@@ -522,7 +522,7 @@ template <typename TQ, typename TC, int HD>
 int launch_mass(const MassPagedCall &c, int sm_count, cudaStream_t s) {
     using G = MassGeo<HD, std::is_same<TQ, float>::value>;
     CUtensorMap mk;
-    int rc = make_page_map(&mk, c.a.k, c.a, HD, c.cache_type, c.a.page_size < 128 ? c.a.page_size : 128);
+    int rc = make_page_map(&mk, c.a.k, c.a, HD, c.cache_type, c.a.page_size < 128 ? c.a.page_size : 128, 1);
     if (rc) return rc;
     auto kern = mass_kernel<TQ, TC, HD>;
     CUQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM));

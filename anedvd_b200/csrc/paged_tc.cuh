@@ -89,18 +89,23 @@ __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.a
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// A pool as a tensor [page][head][slot][dim]: one box is 64 dims of `rows`
-// slots of one head of one page, in the 128-byte swizzle.  A page coordinate of
-// n_pages lies outside and reads as zero, which is how holes are filled.
-__device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap *m, int dim, int slot, int head, int page,
+// A pool as a tensor [page][head][column block of 64 dims][slot][dim]: one box is
+// `rows` slots of one head of one page, one column block or all of them, block by
+// block in the 128-byte swizzle.  A page coordinate of n_pages lies outside and reads as zero,
+// which is how holes are filled.
+__device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap *m, int cb, int slot, int head, int page,
                                               uint64_t *bar) {
     asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
-        "[%6];" ::"r"(dst),
-        "l"(m), "r"(dim), "r"(slot), "r"(head), "r"(page), "r"(smem_u32(bar))
+        "cp.async.bulk.tensor.5d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], "
+        "[%7];" ::"r"(dst),
+        "l"(m), "r"(0), "r"(slot), "r"(cb), "r"(head), "r"(page), "r"(smem_u32(bar))
         : "memory");
 }
-int make_page_map(CUtensorMap *m, const void *pool, const PagedArgs &a, uint32_t hd, int type, uint32_t rows);
+__device__ __forceinline__ void prefetch_map(const CUtensorMap *m) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
+}
+int make_page_map(CUtensorMap *m, const void *pool, const PagedArgs &a, uint32_t hd, int type, uint32_t rows,
+                  uint32_t blocks);
 
 // Shared-memory descriptor, 128-byte swizzle: atoms of 8 rows of 128 B, `sbo`
 // bytes from one to the next along the rows; `lbo` from one 64-value column
