@@ -9,7 +9,20 @@
 #include "paged.cuh"
 
 namespace cuq {
+
 int sm_count_current();
+
+int paged_sm_count() {
+    static std::atomic<int> known[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return sm_count_current();
+    int n = known[dev].load(std::memory_order_relaxed);
+    if (!n) {
+        n = sm_count_current();
+        known[dev].store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
 
 constexpr int ROPE_MAX_PAIRS = 64;
 
@@ -750,7 +763,7 @@ size_t cuq_attention_paged_workspace(const cuq_paged_kv *kv, const cuq_batch *ba
     c.type = type;
     c.cache_type = kv->type;
     c.hd = kv->head_dim;
-    return attention_paged_workspace(c, sm_count_current());
+    return attention_paged_workspace(c, paged_sm_count());
 }
 
 int cuq_attention_paged(const cuq_paged_kv *kv, const cuq_batch *batch, void *out, size_t out_stride, const void *q,
@@ -773,7 +786,7 @@ int cuq_attention_paged(const cuq_paged_kv *kv, const cuq_batch *batch, void *ou
     c.cache_type = kv->type;
     c.hd = kv->head_dim;
     c.workspace = workspace;
-    const int sms = sm_count_current();
+    const int sms = paged_sm_count();
     const size_t need = attention_paged_workspace(c, sms);
     CUQ_CHECK_ARG(workspace_bytes >= need && (need == 0 || workspace),
                   "%s: workspace of %zu bytes, %zu needed (cuq_attention_paged_workspace)", who, workspace_bytes, need);
@@ -803,7 +816,7 @@ int cuq_attention_mass(const cuq_paged_kv *kv, const cuq_batch *batch, float *ma
     c.hd = kv->head_dim;
     c.last_q = last_q;
     c.decay = decay;
-    return launch_attention_mass(c, sm_count_current(), (cudaStream_t)stream);
+    return launch_attention_mass(c, paged_sm_count(), (cudaStream_t)stream);
 }
 
 int cuq_kv_evict(const cuq_paged_kv *kv, const cuq_batch *batch, const float *mass, size_t mass_stride,
@@ -832,7 +845,7 @@ int cuq_kv_evict(const cuq_paged_kv *kv, const cuq_batch *batch, const float *ma
     p.new_len = new_len;
     p.mass_out = mass_out;
     p.mass_out_stride = mass_out_stride;
-    return launch_evict(p, kv->head_dim, sm_count_current(), (cudaStream_t)stream);
+    return launch_evict(p, kv->head_dim, paged_sm_count(), (cudaStream_t)stream);
 }
 
 int cuq_paged_status(void *stream) {

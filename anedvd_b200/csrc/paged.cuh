@@ -4,9 +4,27 @@
 
 #include <cuda_bf16.h>
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace cuq {
+
+// SM count of the current device, asked for once per device.
+int paged_sm_count();
+// Let `kernel` use `bytes` of dynamic shared memory, set once per device (`done`
+// holds a bit for each of the first 64; others are set every time).
+template <typename K>
+cudaError_t allow_smem(K kernel, int bytes, std::atomic<uint64_t> &done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
 
 // The cache and the batch as a kernel sees them.  Every length and page id that
 // comes from device memory is cut or checked here, so no kernel reads past a

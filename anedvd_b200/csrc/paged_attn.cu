@@ -27,7 +27,7 @@ __device__ int g_timeout;  // a bounded wait of this file's kernels gave up
 // in the 128-byte swizzle, which ldmatrix reads without bank conflicts.  Scores and
 // outputs run on mma.sync.m16n8k16 (16 rows x 16 slots, fp32 accumulate); fp32
 // queries are two fp16 operands, hi and lo, and so are their probabilities.
-constexpr int FEW_WARPS = 4, FEW_ST = 3, FEW_KEYS = 16;
+constexpr int FEW_WARPS = 4, FEW_ST = 2, FEW_KEYS = 16;
 constexpr uint32_t FEW_RUN = 4;   // blocks a warp takes at least
 constexpr uint32_t FEW_ITEM = 3;  // blocks' worth of an item's own cost
 
@@ -456,7 +456,8 @@ int launch_few(const AttnPagedCall &c, const AttnOut &o, cudaStream_t s) {
     if (rc == CUQ_OK) rc = make_page_map(&mv, c.a.v, c.a, HD, c.cache_type, FEW_KEYS, HD / 64);
     if (rc) return rc;
     auto kern = attn_few_kernel<TQ, TC, HD>;
-    CUQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, FewGeo<HD>::SMEM));
+    static std::atomic<uint64_t> allowed;
+    CUQ_CUDA_TRY(allow_smem(kern, FewGeo<HD>::SMEM, allowed));
     kern<<<o.plan.few_ctas, FEW_WARPS * 32, FewGeo<HD>::SMEM, s>>>(c.a, c.q, o, mk, mv);
     CUQ_CUDA_TRY(cudaGetLastError());
     return CUQ_OK;

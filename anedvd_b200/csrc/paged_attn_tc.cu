@@ -511,7 +511,8 @@ int launch_many(const AttnPagedCall &c, const AttnOut &o, cudaStream_t s) {
     if (rc == CUQ_OK) rc = make_page_map(&mv, c.a.v, c.a, HD, c.cache_type, box, 1);
     if (rc) return rc;
     auto kern = attn_many_kernel<TQ, TC, HD>;
-    CUQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM));
+    static std::atomic<uint64_t> allowed;
+    CUQ_CUDA_TRY(allow_smem(kern, G::SMEM, allowed));
     kern<<<dim3(c.a.kv_heads * o.plan.many_tiles, o.plan.many_splits), NT, G::SMEM, s>>>(c.a, c.q, o, mk, mv);
     CUQ_CUDA_TRY(cudaGetLastError());
     return CUQ_OK;

@@ -525,7 +525,8 @@ int launch_mass(const MassPagedCall &c, int sm_count, cudaStream_t s) {
     int rc = make_page_map(&mk, c.a.k, c.a, HD, c.cache_type, c.a.page_size < 128 ? c.a.page_size : 128, 1);
     if (rc) return rc;
     auto kern = mass_kernel<TQ, TC, HD>;
-    CUQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM));
+    static std::atomic<uint64_t> allowed;
+    CUQ_CUDA_TRY(allow_smem(kern, G::SMEM, allowed));
     MassArgs p{};
     p.a = c.a;
     p.q = c.q;
