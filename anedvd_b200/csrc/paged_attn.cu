@@ -112,7 +112,10 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, FewGeo<HD>::CTAS)
         const uint64_t x0 = (uint64_t)gw * run, all = (uint64_t)total * a.kv_heads;
         left = x0 < all ? (uint32_t)min((uint64_t)run, all - x0) : 0;
     }
-    if (!left) return;
+    if (!left) {
+        if (gw == 0) griddep_wait();
+        return;
+    }
     // the run's first sequence, KV head and unit
     uint32_t b0 = 0, h0 = 0, k0 = 0;
     {
@@ -355,6 +358,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, FewGeo<HD>::CTAS)
             b++;
         }
     }
+    if (gw == 0) griddep_wait();  // behind the many-row kernel: this grid ends after that one, for the merge's sake
     if (!ok) {  // let the copies in flight land before this block's memory is given back
         if (lane == 0) g_timeout = 1;
         const unsigned long long t0 = now_ns();
@@ -458,8 +462,8 @@ int launch_few(const AttnPagedCall &c, const AttnOut &o, cudaStream_t s) {
     auto kern = attn_few_kernel<TQ, TC, HD>;
     static std::atomic<uint64_t> allowed;
     CUQ_CUDA_TRY(allow_smem(kern, FewGeo<HD>::SMEM, allowed));
-    kern<<<o.plan.few_ctas, FEW_WARPS * 32, FewGeo<HD>::SMEM, s>>>(c.a, c.q, o, mk, mv);
-    CUQ_CUDA_TRY(cudaGetLastError());
+    CUQ_CUDA_TRY(launch_maybe_pdl(kern, dim3(o.plan.few_ctas), dim3(FEW_WARPS * 32), FewGeo<HD>::SMEM, s, o.plan.many, c.a,
+                                  c.q, o, mk, mv));
     return CUQ_OK;
 }
 

@@ -56,6 +56,7 @@ __global__ void __launch_bounds__(NT, 1) attn_many_kernel(PagedArgs a, PagedQuer
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = warp_index();
     const uint32_t kvh = blockIdx.x % a.kv_heads, split = blockIdx.y;
+    griddep_launch();  // the few-row kernel and the merge may follow into free SMs; the merge waits for the end
 
     // the tile: tiles are counted over the sequences that are this kernel's
     uint32_t b = 0, tile = blockIdx.x / a.kv_heads, ntile = 0;
