@@ -224,12 +224,15 @@ int launch_rope_append(const RopeArgs &p, const RopeTable &t, int out_type, int 
 //
 // Selection, bound by latency: a cluster of CTAs takes one (sequence, KV head),
 // each a contiguous slice of its slots.  Masses become 32-bit keys in their order
-// (NaN lowest).  Three histogram passes (11, 11, 10 bits) find the key of the last
-// slot kept and how many of its equals are kept; every CTA counts its own slice and
-// adds the bins it hit into rank 0's through distributed shared memory, whose scan
-// tells all the digit.  A last pass writes the kept slots at their prefix sums.
-// Histogram atomics count whole numbers, so their order does not matter.
-constexpr int SEL_THREADS = 512, SEL_BINS = 2048, SEL_PER = 4;
+// (NaN lowest), eight a thread, kept in registers where the slice fits.
+// Three histogram passes (11, 11, 10 bits) find the key of the last slot kept and how
+// many of its equals are kept: every CTA counts its own slice, adds the bins it hit
+// into every CTA's sums through distributed shared memory, and works the digit out
+// for itself.  Then the slices' counts are exchanged and the kept slots written at
+// their prefix sums.  Histogram atomics count whole numbers, so their order does not
+// matter.  Five cluster barriers in all; with rank 0 finding the digits it was ten.
+constexpr int SEL_THREADS = 512, SEL_BINS = 2048, SEL_PER = 8;
+constexpr uint32_t SEL_TILE = SEL_THREADS * SEL_PER;
 
 __device__ __forceinline__ uint32_t mass_key(float m) {
     if (m != m) return 0u;
@@ -266,9 +269,10 @@ __device__ __forceinline__ void cluster_sync() {
 }
 
 __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(EvictArgs p) {
-    __shared__ uint32_t hist[SEL_BINS];  // this slice's counts
-    __shared__ uint32_t sums[SEL_BINS];  // rank 0: the cluster's
-    __shared__ uint32_t s_digit, s_need, s_above[16], s_equal[16], warp_a[SEL_THREADS / 32], warp_e[SEL_THREADS / 32];
+    __shared__ __align__(16) uint32_t hist[SEL_BINS];     // this slice's counts
+    __shared__ __align__(16) uint32_t sums[3][SEL_BINS];  // the cluster's, one set a pass
+    __shared__ uint32_t s_digit, s_need, s_above[8], s_equal[8], warp_a[SEL_THREADS / 32];
+    __shared__ uint2 s_run[SEL_PER * SEL_THREADS / 32];  // kept for sure and equal, by warps of slots
     uint32_t rank, ranks;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
@@ -282,249 +286,282 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(EvictArgs p) 
             kept[i] = i < n ? (int32_t)i : -1;
         return;
     }
+    auto sync = [&]() {
+        if (ranks > 1)
+            cluster_sync();
+        else
+            __syncthreads();
+    };
     // the slots in between, of which `need` are kept, and this CTA's slice of all slots
     const uint32_t lo = p.sink, hi = n - p.recent;
     const uint32_t per = (n + ranks - 1) / ranks, i0 = min(n, rank * per), i1 = min(n, i0 + per);
-    const uint32_t m0 = max(i0, lo), m1 = min(i1, hi);
+    const bool resident = per <= SEL_TILE;
+    uint32_t key[SEL_PER];
+    auto load = [&](uint32_t t0) {  // the thread's keys of the tile at t0; 0 past the slice
+#pragma unroll
+        for (int e = 0; e < SEL_PER; e++) {
+            const uint32_t i = t0 + e * SEL_THREADS + tid;
+            key[e] = i < i1 ? mass_key(__ldg(mass + i)) : 0u;
+        }
+    };
+    if (resident) load(i0);
+    for (uint32_t i = tid; i < SEL_BINS; i += SEL_THREADS) hist[i] = sums[0][i] = sums[1][i] = sums[2][i] = 0;
+    sync();  // the sums are clear everywhere
     uint32_t need = p.keep - p.sink - p.recent, prefix = 0;
     constexpr int SHIFT[3] = {21, 10, 0}, BITS[3] = {11, 11, 10};
-#pragma unroll
+#pragma unroll 1
     for (int pass = 0; pass < 3; pass++) {
         if (need == 0) break;  // nothing in between is kept
-        const int shift = SHIFT[pass], bins = 1 << BITS[pass];
-        for (uint32_t i = tid; i < SEL_BINS; i += SEL_THREADS) hist[i] = sums[i] = 0;
-        if (ranks > 1)
-            cluster_sync();  // rank 0's sums are clear
-        else
-            __syncthreads();
-        for (uint32_t i = m0 + tid; i < m1; i += SEL_THREADS * SEL_PER) {
-            float m[SEL_PER];
-#pragma unroll
-            for (int e = 0; e < SEL_PER; e++) m[e] = i + e * SEL_THREADS < m1 ? __ldg(mass + i + e * SEL_THREADS) : 0.f;
+        const int shift = SHIFT[pass], bits = BITS[pass], bins = 1 << bits;
+        for (uint32_t t0 = i0; t0 < i1; t0 += SEL_TILE) {
+            if (!resident) load(t0);
+            const uint32_t first = t0 + tid;
 #pragma unroll
             for (int e = 0; e < SEL_PER; e++) {
-                const uint32_t key = mass_key(m[e]);
-                if (i + e * SEL_THREADS < m1 && (pass == 0 || (key >> (shift + BITS[pass])) == prefix))
-                    atomicAdd(&hist[(key >> shift) & (bins - 1)], 1u);
+                const uint32_t i = first + e * SEL_THREADS;
+                if (i >= lo && i < hi && i < i1 && (pass == 0 || (key[e] >> (shift + bits)) == prefix))
+                    atomicAdd(&hist[(key[e] >> shift) & (bins - 1)], 1u);
             }
         }
         __syncthreads();
         if (ranks > 1) {
-            for (uint32_t i = tid; i < (uint32_t)bins; i += SEL_THREADS)
-                if (hist[i]) peer_add(peer_smem(&sums[i], 0), hist[i]);
+            for (uint32_t i = tid; i < (uint32_t)bins; i += SEL_THREADS) {
+                const uint32_t v = hist[i];
+                hist[i] = 0;
+                if (v)
+                    for (uint32_t r = 0; r < ranks; r++) peer_add(peer_smem(&sums[pass][i], r), v);
+            }
             cluster_sync();
         }
-        if (rank == 0) {  // the bin, from the top, in which the need-th key lies
-            const uint32_t *c = ranks > 1 ? sums : hist;
-            constexpr int PER = SEL_BINS / SEL_THREADS;
-            uint32_t v[PER], own = 0;  // thread t: bins [bins - PER (t + 1), bins - PER t), from the top
-#pragma unroll
-            for (int e = 0; e < PER; e++) {
-                const int bin = bins - 1 - (int)(tid * PER) - e;
-                v[e] = bin >= 0 ? c[bin] : 0u;
-                own += v[e];
-            }
-            uint32_t incl = own;
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const uint32_t up = __shfl_up_sync(~0u, incl, d);
-                if (lane >= (uint32_t)d) incl += up;
-            }
-            if (lane == 31) warp_a[warp] = incl;
-            __syncthreads();
-            uint32_t above = incl - own;
-            for (uint32_t w = 0; w < warp; w++) above += warp_a[w];
-#pragma unroll
-            for (int e = 0; e < PER; e++) {
-                if (above < need && above + v[e] >= need) {  // one thread only (need > 0)
-                    const uint32_t bin = (uint32_t)(bins - 1 - (int)(tid * PER) - e);
-                    for (uint32_t r = 0; r < ranks; r++) {
-                        peer_store(peer_smem(&s_digit, r), bin);
-                        peer_store(peer_smem(&s_need, r), need - above);
-                    }
-                }
-                above += v[e];
-            }
+        // the bin, from the top, in which the need-th key lies
+        uint32_t *c = ranks > 1 ? sums[pass] : hist;
+        constexpr int PER = SEL_BINS / SEL_THREADS;  // thread t: bins [bins - PER (t + 1), bins - PER t), from the top
+        static_assert(PER == 4, "a vector of bins a thread");
+        const int bin0 = bins - (int)((tid + 1) * PER);
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (bin0 >= 0) {
+            v = *reinterpret_cast<const uint4 *>(c + bin0);
+            *reinterpret_cast<uint4 *>(c + bin0) = make_uint4(0, 0, 0, 0);
         }
-        if (ranks > 1)
-            cluster_sync();
-        else
-            __syncthreads();
-        prefix = (prefix << BITS[pass]) | s_digit;
+        const uint32_t own = v.x + v.y + v.z + v.w;
+        uint32_t incl = own;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const uint32_t up = __shfl_up_sync(~0u, incl, d);
+            if (lane >= (uint32_t)d) incl += up;
+        }
+        if (lane == 31) warp_a[warp] = incl;
+        __syncthreads();
+        const uint32_t wv = lane < SEL_THREADS / 32 ? warp_a[lane] : 0;
+        uint32_t above = incl - own + __reduce_add_sync(~0u, lane < warp ? wv : 0u);
+        const uint32_t down[4] = {v.w, v.z, v.y, v.x};
+#pragma unroll
+        for (int e = 0; e < PER; e++) {
+            if (above < need && above + down[e] >= need) {  // one thread only (need > 0)
+                s_digit = (uint32_t)(bin0 + PER - 1 - e);
+                s_need = need - above;
+            }
+            above += down[e];
+        }
+        __syncthreads();
+        prefix = (prefix << bits) | s_digit;
         need = s_need;
     }
     // kept: keys above `prefix`, and the first `need` equal to it.  The key 2^32 - 1
     // stands for "none" when nothing in between is kept (no float has it).
     const uint32_t edge = need == 0 ? 0xFFFFFFFFu : prefix;
-    auto kind = [&](uint32_t i, float m, uint32_t &above, uint32_t &equal) {
-        const bool forced = i < lo || i >= hi;
-        const uint32_t key = mass_key(m);
-        above = forced || key > edge;
-        equal = !forced && key == edge;
-    };
-    uint32_t ca = 0, ce = 0;
-    for (uint32_t i = i0 + tid; i < i1; i += SEL_THREADS * SEL_PER) {
-        float m[SEL_PER];
-#pragma unroll
-        for (int e = 0; e < SEL_PER; e++) m[e] = i + e * SEL_THREADS < i1 ? __ldg(mass + i + e * SEL_THREADS) : 0.f;
+    // a tile's slots that are kept for sure and those equal to the edge, a bit a slot
+    // (this thread's), and the counts of them before each 32 slots of the tile (s_run)
+    auto kinds = [&](uint32_t t0, uint32_t &above, uint32_t &equal, uint32_t &na, uint32_t &ne) {
+        above = equal = 0;
+        __syncthreads();  // s_run may still be read
 #pragma unroll
         for (int e = 0; e < SEL_PER; e++) {
-            uint32_t u = 0, v = 0;
-            if (i + e * SEL_THREADS < i1) kind(i + e * SEL_THREADS, m[e], u, v);
-            ca += u;
-            ce += v;
+            const uint32_t i = t0 + e * SEL_THREADS + tid;
+            const bool in = i < i1, forced = i < lo || i >= hi;
+            const bool u = in && (forced || key[e] > edge), v = in && !forced && key[e] == edge;
+            above |= (uint32_t)u << e;
+            equal |= (uint32_t)v << e;
+            const uint32_t bu = __ballot_sync(~0u, u), bv = __ballot_sync(~0u, v);
+            if (lane == 0) s_run[e * (SEL_THREADS / 32) + warp] = make_uint2(__popc(bu), __popc(bv));
         }
-    }
-    ca = __reduce_add_sync(~0u, ca);
-    ce = __reduce_add_sync(~0u, ce);
-    __syncthreads();
-    if (lane == 0) warp_a[warp] = ca, warp_e[warp] = ce;
-    __syncthreads();
-    if (tid == 0) {
-        uint32_t u = 0, v = 0;
-        for (int w = 0; w < SEL_THREADS / 32; w++) u += warp_a[w], v += warp_e[w];
-        for (uint32_t r = 0; r < ranks; r++) {
-            peer_store(peer_smem(&s_above[rank], r), u);
-            peer_store(peer_smem(&s_equal[rank], r), v);
-        }
-    }
-    if (ranks > 1)
-        cluster_sync();
-    else
         __syncthreads();
-    uint32_t base_a = 0, base_e = 0;
-    for (uint32_t r = 0; r < rank; r++) base_a += s_above[r], base_e += s_equal[r];
-    // output: tiles of SEL_PER neighbouring slots a thread
-    for (uint32_t t0 = i0; t0 < i1; t0 += SEL_THREADS * SEL_PER) {
-        const uint32_t i = t0 + tid * SEL_PER;
-        uint32_t u[SEL_PER], v[SEL_PER], na = 0, ne = 0;
+        constexpr int RUNS = SEL_PER * SEL_THREADS / 32, EACH = RUNS / 32;  // a warp scans them, each in turn
+        uint2 r[EACH];
+        uint32_t su = 0, sv = 0;
 #pragma unroll
-        for (int e = 0; e < SEL_PER; e++) {
-            u[e] = v[e] = 0;
-            if (i + e < i1) kind(i + e, __ldg(mass + i + e), u[e], v[e]);
-            na += u[e];
-            ne += v[e];
+        for (int e = 0; e < EACH; e++) {
+            r[e] = s_run[lane * EACH + e];
+            su += r[e].x;
+            sv += r[e].y;
         }
-        uint32_t ia = na, ie = ne;
+        uint32_t iu = su, iv = sv;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
-            const uint32_t ua = __shfl_up_sync(~0u, ia, d), ue = __shfl_up_sync(~0u, ie, d);
-            if (lane >= (uint32_t)d) ia += ua, ie += ue;
+            const uint32_t uu = __shfl_up_sync(~0u, iu, d), uv = __shfl_up_sync(~0u, iv, d);
+            if (lane >= (uint32_t)d) iu += uu, iv += uv;
+        }
+        na = __shfl_sync(~0u, iu, 31);
+        ne = __shfl_sync(~0u, iv, 31);
+        __syncthreads();
+        if (warp == 0) {
+            iu -= su;
+            iv -= sv;
+#pragma unroll
+            for (int e = 0; e < EACH; e++) {
+                s_run[lane * EACH + e] = make_uint2(iu, iv);
+                iu += r[e].x;
+                iv += r[e].y;
+            }
         }
         __syncthreads();
-        if (lane == 31) warp_a[warp] = ia, warp_e[warp] = ie;
-        __syncthreads();
-        uint32_t at_a = base_a + ia - na, at_e = base_e + ie - ne;
-        for (uint32_t w = 0; w < SEL_THREADS / 32; w++) {
-            if (w < warp) at_a += warp_a[w], at_e += warp_e[w];
-            base_a += warp_a[w];
-            base_e += warp_e[w];
+    };
+    uint32_t ca = 0, ce = 0, above = 0, equal = 0;
+    for (uint32_t t0 = i0; t0 < i1; t0 += SEL_TILE) {
+        uint32_t na, ne;
+        if (!resident) load(t0);
+        kinds(t0, above, equal, na, ne);
+        ca += na;
+        ce += ne;
+    }
+    if (tid < ranks) {  // to rank tid
+        peer_store(peer_smem(&s_above[rank], tid), ca);
+        peer_store(peer_smem(&s_equal[rank], tid), ce);
+    }
+    sync();
+    uint32_t base_a = 0, base_e = 0;
+    for (uint32_t r = 0; r < rank; r++) base_a += s_above[r], base_e += s_equal[r];
+    for (uint32_t t0 = i0; t0 < i1; t0 += SEL_TILE) {
+        uint32_t na = 0, ne = 0;
+        if (!resident) {
+            load(t0);
+            kinds(t0, above, equal, na, ne);
         }
 #pragma unroll
         for (int e = 0; e < SEL_PER; e++) {
-            if (u[e] || (v[e] && at_e < need)) {
-                const uint32_t at = at_a + min(at_e, need);
-                if (at < p.keep) kept[at] = (int32_t)(i + e);
+            const uint32_t u = (above >> e) & 1u, v = (equal >> e) & 1u, low = (1u << lane) - 1u;
+            const uint32_t bu = __ballot_sync(~0u, u), bv = __ballot_sync(~0u, v);
+            const uint2 run = s_run[e * (SEL_THREADS / 32) + warp];
+            const uint32_t at_e = base_e + run.y + __popc(bv & low);
+            if (u || (v && at_e < need)) {
+                const uint32_t at = base_a + run.x + __popc(bu & low) + min(at_e, need);
+                if (at < p.keep) kept[at] = (int32_t)(t0 + e * SEL_THREADS + tid);
             }
-            at_a += u[e];
-            at_e += v[e];
         }
+        base_a += na;
+        base_e += ne;
     }
 }
 
-// Compaction, in place: a CTA owns one slice of SLICE bytes of every row of one
-// (sequence, KV head, pool), so no other CTA reads or writes what it does; one CTA
-// more per (sequence, KV head) moves the mass.  New slot j takes old slot kept[j] >=
-// j, in order: a chunk of rows is read whole before it is written, and no later
-// chunk reads what an earlier one wrote, so the next chunk's reads are under way
-// while this one is written.
-constexpr int MOVE_THREADS = 256;
-constexpr int MOVE_VECS = 8;  // vectors per thread in one chunk
+// Compaction, in place: a cluster of CTAs takes one (sequence, KV head, pool), and one
+// CTA more per (sequence, KV head) moves the mass.  New slot j takes old slot
+// kept[j] >= j, in order: a chunk of MOVE_ROWS rows a CTA is read whole, by cp.async
+// into shared memory, before any CTA of the cluster writes it, and no later chunk reads
+// what an earlier one wrote.  Whole rows, because each instruction costs a cycle for
+// every line that it touches: with 32-byte slices of all rows a CTA, which needs no
+// cluster, the move of 16 sequences (4001 of up to 32768 slots) took 24.3 us instead of 19.8.
+constexpr int MOVE_THREADS = 256, MOVE_ROWS = 192;
 
-template <int HD, int SLICE>
+template <int HD>
 __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(EvictArgs p) {
-    constexpr uint32_t VPR = SLICE / 16;                      // vectors per row
-    constexpr uint32_t ROWS = MOVE_THREADS * MOVE_VECS / VPR;  // rows per chunk
-    constexpr uint32_t SLICES = HD * 2 / SLICE, STEP = MOVE_THREADS / VPR;
-    griddep_wait();
-    uint32_t x = blockIdx.x;
-    const uint32_t part = x % (2 * SLICES + 1);
-    x /= 2 * SLICES + 1;
+    constexpr uint32_t LANES = HD * 2 / 16, STEP = MOVE_THREADS / LANES, PER = MOVE_ROWS / STEP;  // lanes a row
+    extern __shared__ __align__(16) uint8_t stage[];
+    __shared__ int64_t s_from[MOVE_ROWS], s_to[MOVE_ROWS];  // offsets of a chunk's rows; -1: does not move
+    uint32_t rank, ranks;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
+    uint32_t x = blockIdx.x / ranks;
+    const uint32_t part = x % 3;  // K, V, mass
+    x /= 3;
     const uint32_t h = x % p.a.kv_heads, b = x / p.a.kv_heads;
     const uint32_t n = p.a.len(b);
     const int32_t *kept = p.kept + ((size_t)b * p.a.kv_heads + h) * p.keep;
-    if (part == 2 * SLICES) {
+    if (part == 2) {
         if (!p.mass_out) return;
+        griddep_wait();
         const float *src = p.mass + ((size_t)b * p.a.kv_heads + h) * p.mass_stride;
         float *dst = p.mass_out + ((size_t)b * p.a.kv_heads + h) * p.mass_out_stride;
         const uint32_t live = min(n, p.keep);
-        for (uint32_t c = 0; c < live; c += MOVE_THREADS * MOVE_VECS) {
-            float v[MOVE_VECS];
+        constexpr uint32_t V = 16;
+        for (uint32_t c = 0; c < live && rank == 0; c += MOVE_THREADS * V) {
+            float v[V];
 #pragma unroll
-            for (int i = 0; i < MOVE_VECS; i++) {
+            for (uint32_t i = 0; i < V; i++) {
                 const uint32_t j = c + i * MOVE_THREADS + threadIdx.x;
                 v[i] = j < live ? src[kept[j]] : 0.f;
             }
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < MOVE_VECS; i++) {
+            for (uint32_t i = 0; i < V; i++) {
                 const uint32_t j = c + i * MOVE_THREADS + threadIdx.x;
                 if (j < live) dst[j] = v[i];
             }
             __syncthreads();
         }
-        for (uint32_t i = live + threadIdx.x; i < n; i += MOVE_THREADS) dst[i] = 0.f;
+        // (in place, slots past `live` may still have to be read)
+        if (ranks > 1) cluster_sync();
+        for (uint32_t i = live + rank * MOVE_THREADS + threadIdx.x; i < n; i += ranks * MOVE_THREADS) dst[i] = 0.f;
         return;
     }
-    if (n <= p.keep) return;  // every slot stays where it is
-    const bool is_v = part >= SLICES;
-    uint8_t *pool = reinterpret_cast<uint8_t *>(is_v ? p.a.v : p.a.k) + (part % SLICES) * SLICE;
-    const uint32_t r0 = threadIdx.x / VPR, off = (threadIdx.x % VPR) * 16;
-    uint4 val[MOVE_VECS];
-    uint32_t ok = 0;  // a bit for each vector that moves
-    auto read = [&](uint32_t c) {
-        uint32_t src[MOVE_VECS];
-        int pg[MOVE_VECS];
-#pragma unroll
-        for (int i = 0; i < MOVE_VECS; i++) {
-            const uint32_t j = c + r0 + i * STEP;
-            src[i] = j < p.keep ? (uint32_t)__ldg(kept + j) : j;
-            if (src[i] >= n) src[i] = j;
-        }
-#pragma unroll
-        for (int i = 0; i < MOVE_VECS; i++)
-            pg[i] = src[i] != c + r0 + i * STEP ? p.a.page(b, src[i] >> p.a.page_shift) : -1;
-        ok = 0;
-#pragma unroll
-        for (int i = 0; i < MOVE_VECS; i++)
-            if (pg[i] >= 0) {
-                ok |= 1u << i;
-                val[i] = *reinterpret_cast<const uint4 *>(pool + p.a.row<HD>(pg[i], h, src[i]) * 2 + off);
-            }
+    if (n <= p.keep) return;  // every slot stays where it is: the same for the whole cluster
+    uint8_t *pool = reinterpret_cast<uint8_t *>(part ? p.a.v : p.a.k);
+    auto place = [&](uint32_t slot) -> int64_t {  // offset of its row, below 0 on a hole
+        const int pg = p.a.page(b, slot >> p.a.page_shift);
+        return pg < 0 ? -1 : (int64_t)(p.a.row<HD>(pg, h, slot) * 2);
     };
-    read(0);
-    for (uint32_t c = 0; c < p.keep; c += ROWS) {
-        uint4 out[MOVE_VECS];
-        const uint32_t move = ok;
-#pragma unroll
-        for (int i = 0; i < MOVE_VECS; i++) out[i] = val[i];
-        __syncthreads();  // chunk c is read by every thread
-        if (c + ROWS < p.keep) read(c + ROWS);
-#pragma unroll
-        for (int i = 0; i < MOVE_VECS; i++) {
-            const uint32_t j = c + r0 + i * STEP;
-            if (!((move >> i) & 1u)) continue;
-            const int pg = p.a.page(b, j >> p.a.page_shift);
-            if (pg >= 0) *reinterpret_cast<uint4 *>(pool + p.a.row<HD>(pg, h, j) * 2 + off) = out[i];
+    griddep_wait();  // what is above reads the batch alone
+    const uint32_t r0 = threadIdx.x / LANES, off = (threadIdx.x % LANES) * 16;
+    int64_t from_next, to_next;  // this thread's row of the next chunk, looked up while a chunk is read
+    auto look = [&](uint32_t c) {
+        const uint32_t j = c + rank * MOVE_ROWS + threadIdx.x;
+        from_next = to_next = -1;
+        if (threadIdx.x >= MOVE_ROWS || j >= p.keep) return;
+        const uint32_t src = (uint32_t)__ldg(kept + j);
+        if (src == j || src >= n) return;
+        to_next = place(j);
+        from_next = to_next < 0 ? -1 : place(src);
+    };
+    look(0);
+    for (uint32_t c = 0; c < p.keep; c += ranks * MOVE_ROWS) {
+        if (threadIdx.x < MOVE_ROWS) {
+            s_from[threadIdx.x] = from_next;
+            s_to[threadIdx.x] = to_next;
         }
+        __syncthreads();
+#pragma unroll
+        for (uint32_t i = 0; i < PER; i++) {
+            const uint32_t r = i * STEP + r0;
+            const int64_t from = s_from[r];
+            if (from >= 0)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                                 (uint32_t)__cvta_generic_to_shared(stage + r * (HD * 2) + off)),
+                             "l"(pool + from + off)
+                             : "memory");
+        }
+        look(c + ranks * MOVE_ROWS);
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        if (ranks > 1)  // the chunk is read by every thread of the cluster
+            cluster_sync();
+        else
+            __syncthreads();
+#pragma unroll
+        for (uint32_t i = 0; i < PER; i++) {
+            const uint32_t r = i * STEP + r0;
+            if (s_from[r] >= 0)
+                *reinterpret_cast<uint4 *>(pool + s_to[r] + off) =
+                    *reinterpret_cast<const uint4 *>(stage + r * (HD * 2) + off);
+        }
+        __syncthreads();  // the offsets and the stage may be written again
     }
 }
 
+// slots of one CTA's slice, beyond which another joins its cluster
+constexpr uint32_t SEL_SLICE = 4096;
+
 int launch_evict(const EvictArgs &p, uint32_t hd, int sm_count, cudaStream_t s) {
     const uint32_t rows = p.a.n_seqs * p.a.kv_heads;
-    // a slice of 4096 slots a CTA keeps its passes short; clusters of up to 8
     uint32_t ranks = 1;
-    while (ranks < 8 && (uint64_t)ranks * 4096 < p.a.max_kv && (uint64_t)rows * ranks * 2 <= 4u * sm_count) ranks *= 2;
+    while (ranks < 8 && (uint64_t)ranks * SEL_SLICE < p.a.max_kv && (uint64_t)rows * ranks * 2 <= 4u * sm_count) ranks *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(rows * ranks);
     cfg.blockDim = dim3(SEL_THREADS);
@@ -537,18 +574,26 @@ int launch_evict(const EvictArgs &p, uint32_t hd, int sm_count, cudaStream_t s) 
     cfg.numAttrs = 1;
     CUQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, evict_select_kernel, p));
     if (p.a.max_kv <= p.keep && !p.mass_out) return CUQ_OK;  // nothing can move
-    // slices of 32 bytes (a DRAM sector) while that leaves SMs idle otherwise, else of 64
-    const bool wide = (uint64_t)rows * (2 * (hd * 2 / 32)) > 4u * (uint64_t)sm_count;
-    const uint32_t parts = 2 * (hd * 2 / (wide ? 64 : 32)) + 1;
-    const dim3 grid(rows * parts), block(MOVE_THREADS);
-    cudaError_t e;
-    if (hd == 64)
-        e = wide ? launch_maybe_pdl(evict_move_kernel<64, 64>, grid, block, 0, s, true, p)
-                 : launch_maybe_pdl(evict_move_kernel<64, 32>, grid, block, 0, s, true, p);
-    else
-        e = wide ? launch_maybe_pdl(evict_move_kernel<128, 64>, grid, block, 0, s, true, p)
-                 : launch_maybe_pdl(evict_move_kernel<128, 32>, grid, block, 0, s, true, p);
-    CUQ_CUDA_TRY(e);
+    // as many CTAs a cluster as have rows to move, so that most calls take one or two rounds
+    uint32_t movers = 1;
+    while (movers < 8 && movers * MOVE_ROWS < p.keep) movers *= 2;
+    const int bytes = MOVE_ROWS * (int)hd * 2;
+    static std::atomic<uint64_t> allowed64, allowed128;
+    CUQ_CUDA_TRY(hd == 64 ? allow_smem(evict_move_kernel<64>, bytes, allowed64)
+                          : allow_smem(evict_move_kernel<128>, bytes, allowed128));
+    cudaLaunchAttribute attrs[2];
+    attrs[0].id = cudaLaunchAttributeClusterDimension;
+    attrs[0].val.clusterDim.x = movers;
+    attrs[0].val.clusterDim.y = attrs[0].val.clusterDim.z = 1;
+    attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(rows * 3 * movers);
+    cfg.blockDim = dim3(MOVE_THREADS);
+    cfg.dynamicSmemBytes = (size_t)bytes;
+    cfg.attrs = attrs;
+    cfg.numAttrs = 2;
+    CUQ_CUDA_TRY(hd == 64 ? cudaLaunchKernelEx(&cfg, evict_move_kernel<64>, p)
+                          : cudaLaunchKernelEx(&cfg, evict_move_kernel<128>, p));
     return CUQ_OK;
 }
 
