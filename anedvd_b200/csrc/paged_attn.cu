@@ -85,6 +85,9 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, FewGeo<HD>::CTAS)
                     const __grid_constant__ CUtensorMap mv) {
     using G = FewGeo<HD>;
     constexpr bool SPLIT = std::is_same<TQ, float>::value;
+    // probabilities of fp32 queries are 2^12 larger, so that their low fp16 parts keep
+    // clear of subnormals
+    constexpr float LIFT = SPLIT ? 12.f : 0.f;
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t full[FEW_WARPS][FEW_ST];
     __shared__ int abort_flag;
@@ -299,7 +302,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, FewGeo<HD>::CTAS)
                     float sum = 0.f;
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        p[h][e] = ex2(x[e] - ms);
+                        p[h][e] = ex2(x[e] - ms + LIFT);
                         sum += p[h][e];
                     }
                     l[h] = l[h] * f + sum;
@@ -345,7 +348,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, FewGeo<HD>::CTAS)
             if (r >= rows) continue;
             const size_t row = part * o.plan.few_rows + r;
             const float inv = l[h] == 0.f ? 0.f : 1.f / l[h];  // NaN stays NaN
-            if (t4 == 0) o.few_lse[row] = l[h] == 0.f ? -INFINITY : m[h] + log2f(l[h]);
+            if (t4 == 0) o.few_lse[row] = l[h] == 0.f ? -INFINITY : m[h] - LIFT + log2f(l[h]);
 #pragma unroll
             for (int d = 0; d < HD / 8; d++)
                 *reinterpret_cast<float2 *>(o.few_o + row * HD + d * 8 + t4 * 2) =

@@ -13,7 +13,10 @@
 // issued behind O += P V of tile j, so when S is there, O is complete: the softmax
 // threads rescale O themselves, and only when a row's maximum has grown by more
 // than 2^8 (until then P stays below 2^8 and the sum takes it as it is).
-// fp32 queries are two fp16 operands, and P is then two, which together fill S.
+// fp32 queries are two fp16 operands, and P is then two, which together fill S.  The
+// tensor cores cut off what falls below the accumulator's last place, always towards
+// zero: over a long context that is 2e-6 of an fp32 output.  So with fp32 queries O is
+// of one tile only and the softmax threads sum the tiles in registers (4e-7).
 // What bounds it: per 128 x 128 tile the two products take 1024 cycles of the
 // tensor pipe at head_dim 128 (512 at 64) and the exponentials 1024 of the MUFU.
 #include "paged_tc.cuh"
@@ -48,6 +51,9 @@ __global__ void __launch_bounds__(NT, 1) attn_many_kernel(PagedArgs a, PagedQuer
                                                            const __grid_constant__ CUtensorMap mv) {
     constexpr bool SPLIT = std::is_same<TQ, float>::value;
     using G = ManyGeo<HD, SPLIT>;
+    // probabilities of fp32 queries are 2^7 larger (below 2^15 with the 2^8 that a
+    // maximum may lag), so that their low fp16 parts keep clear of subnormals
+    constexpr float LIFT = SPLIT ? 7.f : 0.f;
     constexpr int ST = G::ST;
     extern __shared__ uint8_t smem_raw[];
     __shared__ ManyBars bars;
@@ -131,9 +137,12 @@ __global__ void __launch_bounds__(NT, 1) attn_many_kernel(PagedArgs a, PagedQuer
     const uint32_t tmem = tmem_slot;
     uint8_t *ring = smem + 2 * G::Q;
 
-    // 384 threads of 168 registers: the softmax's 256 take 208, the others' 128 keep 88
+    // 384 threads of 168 registers: the softmax's 256 take 208 (224), the others' 128 keep 88 (56)
     if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if constexpr (SPLIT)
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        else
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         if (warp == 8) {
             // ------------------------------------------------------ MMA issuer
             if (nt) {
@@ -150,17 +159,19 @@ __global__ void __launch_bounds__(NT, 1) attn_many_kernel(PagedArgs a, PagedQuer
 #pragma unroll
                         for (int ks = 0; ks < HD / 16; ks++) {
                             const uint32_t off = ((ks / 4) * (128 * 128) + (ks % 4) * 32) >> 4;
-                            umma_ss(leader, tmem + s * 128, qb + part * (128 * HD * 2 >> 4) + off, kb + off, id_s, part | ks ? 1u : 0u);
+                            // (the low parts first: what the accumulator cuts off is then small against the sum)
+                        umma_ss(leader, tmem + s * 128, qb + (SPLIT ? 1 - part : 0) * (128 * HD * 2 >> 4) + off, kb + off, id_s,
+                                part | ks ? 1u : 0u);
                         }
                 };
                 auto pv = [&](uint32_t s, uint32_t x, int half, bool acc) {  // O_s += P_s V, 64 keys of V in stage x
                     const uint64_t vb = vd + (x % ST) * (G::TILE >> 4) + half * (KEYS * 64 >> 4);
-                    const uint32_t d = tmem + 256 + s * 128, pa = tmem + s * 128 + half * 32;
+                    const uint32_t d = tmem + 256 + s * 128, pa = tmem + s * 128 + half * (SPLIT ? 64 : 32);
 #pragma unroll
                     for (int part = 0; part < (SPLIT ? 2 : 1); part++)
 #pragma unroll
                         for (int i = 0; i < KEYS / 32; i++)
-                            umma_ts(leader, d, pa + part * 64 + i * 8, vb + (i * 2048 >> 4), id_o, (acc || part || i) ? 1u : 0u);
+                            umma_ts(leader, d, SPLIT ? pa + (i / 2) * 32 + (1 - part) * 16 + (i & 1) * 8 : pa + i * 8, vb + (i * 2048 >> 4), id_o, (acc || part || i) ? 1u : 0u);
                 };
                 // stage x may be loaded again; only where it will be, so that no arrival is left in flight at the end
                 auto freed = [&](uint32_t x) {
@@ -186,7 +197,7 @@ __global__ void __launch_bounds__(NT, 1) attn_many_kernel(PagedArgs a, PagedQuer
                         ok = mbar_wait(&bars.p_full[s][0], j & 1, &abort_flag);
                         if (!ok) break;
                         tc_fence_after();
-                        pv(s, xv, 0, j > 0);
+                        pv(s, xv, 0, !SPLIT && j > 0);
                         ok = mbar_wait(&bars.p_full[s][1], j & 1, &abort_flag);
                         if (!ok) break;
                         tc_fence_after();
@@ -254,7 +265,10 @@ __global__ void __launch_bounds__(NT, 1) attn_many_kernel(PagedArgs a, PagedQuer
             }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        if constexpr (SPLIT)
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        else
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         // ------------------------------------------------------ softmax
         const uint32_t s = warp >> 2, t = tid & 127;
         if (s == 0 || two) {
@@ -325,6 +339,9 @@ __global__ void __launch_bounds__(NT, 1) attn_many_kernel(PagedArgs a, PagedQuer
             const uint32_t lane_base = (warp & 3) << 21;  // this warp's TMEM lanes
             const uint32_t ts = tmem + s * 128 + lane_base, to = tmem + 256 + s * 128 + lane_base;
             float m = -INFINITY, l = 0.f;
+            float osum[SPLIT ? HD : 1];  // fp32 queries: the output so far
+#pragma unroll
+            for (int i = 0; i < (SPLIT ? HD : 1); i++) osum[i] = 0.f;
             bool ok = true;
             for (uint32_t j = 0; j < nt; j++) {
                 if (!mbar_wait(&bars.s_full[s], j & 1, &abort_flag)) {
@@ -332,95 +349,154 @@ __global__ void __launch_bounds__(NT, 1) attn_many_kernel(PagedArgs a, PagedQuer
                     break;
                 }
                 tc_fence_after();
-                float x[128];
-                tmem_ld32(ts, x);
-                tmem_ld32(ts + 32, x + 32);
-                tmem_wait_ld();
-                tmem_ld32(ts + 64, x + 64);
-                tmem_ld32(ts + 96, x + 96);
-                float mx[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-                for (int i = 4; i < 60; i += 8)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) mx[e] = max3(mx[e], x[i + e], x[i + 4 + e]);
-#pragma unroll
-                for (int e = 0; e < 4; e++) mx[e] = fmaxf(mx[e], x[60 + e]);
-                tmem_wait_ld();
                 const uint32_t k0 = (j0 + j) * KEYS;
-                if (hole || k0 < all_lo || k0 + KEYS > all_hi) {
-                    uint32_t gone = 0;  // 16-slot units on a hole
-                    if (hole) {
-                        const uint32_t slot = k0 + (lane & 7) * 16;
-                        gone = __ballot_sync(~0u, lane < 8 && slot < n && a.page(b, slot >> a.page_shift) < 0);
-                    }
-                    const int rlo = (int)lo - (int)k0, rhi = (int)hi - (int)k0;
-#pragma unroll
-                    for (int i = 0; i < 128; i++)
-                        if (i < rlo || i >= rhi || ((gone >> (i / 16)) & 1u)) x[i] = -INFINITY;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) mx[e] = -INFINITY;  // over the visible ones only
-#pragma unroll
-                    for (int i = 0; i < 64; i += 8)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) mx[e] = max3(mx[e], x[i + e], x[i + 4 + e]);
+                const bool masked = hole || k0 < all_lo || k0 + KEYS > all_hi;
+                uint32_t gone = 0;  // 16-slot units on a hole
+                if (hole) {
+                    const uint32_t slot = k0 + (lane & 7) * 16;
+                    gone = __ballot_sync(~0u, lane < 8 && slot < n && a.page(b, slot >> a.page_shift) < 0);
                 }
+                const int rlo = (int)lo - (int)k0, rhi = (int)hi - (int)k0;
+                f32x2 sum = pack2(0.f, 0.f);
+                if constexpr (SPLIT) {
+                    float x[32], mt = -INFINITY;
+                    auto scores = [&](int ch) {  // 32 scores, masked
+                        tmem_ld32(ts + ch * 32, x);
+                        tmem_wait_ld();
+                        if (masked) {
 #pragma unroll
-                for (int i = 64; i < 128; i += 8)
+                            for (int i = 0; i < 32; i++) {
+                                const int c = ch * 32 + i;
+                                if (c < rlo || c >= rhi || ((gone >> (c / 16)) & 1u)) x[i] = -INFINITY;
+                            }
+                        }
+                    };
 #pragma unroll
-                    for (int e = 0; e < 4; e++) mx[e] = max3(mx[e], x[i + e], x[i + 4 + e]);
-                const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                const bool up = mt > m + grow || (m == -INFINITY && mt > m);
-                if (__any_sync(~0u, up)) {
-                    const float mn = up ? mt : m;
-                    const float f = up ? ex2((m - mn) * c2) : 1.f;  // 0 from -inf
-                    m = mn;
-                    l *= f;
-                    if (j > 0) {  // O is complete: S was issued behind it
-#pragma unroll 1
-                        for (int i = 0; i < HD / 16; i++) {
-                            float ov[16];
-                            asm volatile(
-                                "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
-                                "%14,%15}, [%16];"
-                                : "=f"(ov[0]), "=f"(ov[1]), "=f"(ov[2]), "=f"(ov[3]), "=f"(ov[4]), "=f"(ov[5]),
-                                  "=f"(ov[6]), "=f"(ov[7]), "=f"(ov[8]), "=f"(ov[9]), "=f"(ov[10]), "=f"(ov[11]),
-                                  "=f"(ov[12]), "=f"(ov[13]), "=f"(ov[14]), "=f"(ov[15])
-                                : "r"(to + i * 16));
+                    for (int ch = 0; ch < 4; ch++) {
+                        scores(ch);
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) mt = max3(mt, x[i], x[i + 1]);
+                    }
+                    if (j > 0) {  // the last tile's O is complete: S was issued behind it
+#pragma unroll
+                        for (int ch = 0; ch < HD / 32; ch++) {
+                            tmem_ld32(to + ch * 32, x);
                             tmem_wait_ld();
-                            uint32_t r[16];
 #pragma unroll
-                            for (int e = 0; e < 16; e++) r[e] = __float_as_uint(ov[e] * f);
-                            tmem_st16(to + i * 16, r);
+                            for (int i = 0; i < 32; i++) osum[ch * 32 + i] += x[i];
                         }
                     }
-                }
-                const float mm = m == -INFINITY ? 0.f : m;
-                const f32x2 cc = pack2(c2, c2), nm = pack2(-mm * c2, -mm * c2);
-                f32x2 sum = pack2(0.f, 0.f);
+                    if (mt > m + grow) {
+                        const float f = ex2((m - mt) * c2);  // 0 from -inf
+                        m = mt;
+                        l *= f;
 #pragma unroll
-                for (int half = 0; half < 2; half++) {
+                        for (int i = 0; i < HD; i++) osum[i] *= f;
+                    }
+                    const float mc = LIFT - (m == -INFINITY ? 0.f : m) * c2;
+                    const f32x2 cc = pack2(c2, c2), nm = pack2(mc, mc);
+                    // P takes the place of its own 32 scores: 16 columns hi, 16 lo
 #pragma unroll
-                    for (int q16 = 0; q16 < 2; q16++) {
+                    for (int ch = 0; ch < 4; ch++) {
+                        scores(ch);
                         uint32_t ph[16], pl[16];
 #pragma unroll
                         for (int e = 0; e < 32; e += 2) {
-                            const int i = half * 64 + q16 * 32 + e;
                             float u, v;
-                            unpack2(fma2(pack2(x[i], x[i + 1]), cc, nm), u, v);
+                            unpack2(fma2(pack2(x[e], x[e + 1]), cc, nm), u, v);
                             u = ex2(u);
                             v = ex2(v);
                             sum = add2(sum, pack2(u, v));
-                            if (SPLIT)
-                                split_pack<TC>(u, v, ph[e / 2], pl[e / 2]);
-                            else
-                                ph[e / 2] = Pair<TC>::pack(u, v);
+                            split_pack<TC>(u, v, ph[e / 2], pl[e / 2]);
                         }
-                        tmem_st16(ts + half * 32 + q16 * 16, ph);
-                        if (SPLIT) tmem_st16(ts + 64 + half * 32 + q16 * 16, pl);
+                        tmem_st16(ts + ch * 32, ph);
+                        tmem_st16(ts + ch * 32 + 16, pl);
+                        if (ch & 1) {
+                            tmem_wait_st();
+                            tc_fence_before();
+                            mbar_arrive(&bars.p_full[s][ch / 2]);
+                        }
                     }
-                    tmem_wait_st();
-                    tc_fence_before();
-                    mbar_arrive(&bars.p_full[s][half]);
+                } else {
+                    float x[128];
+                    tmem_ld32(ts, x);
+                    tmem_ld32(ts + 32, x + 32);
+                    tmem_wait_ld();
+                    tmem_ld32(ts + 64, x + 64);
+                    tmem_ld32(ts + 96, x + 96);
+                    float mx[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+                    for (int i = 4; i < 60; i += 8)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) mx[e] = max3(mx[e], x[i + e], x[i + 4 + e]);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) mx[e] = fmaxf(mx[e], x[60 + e]);
+                    tmem_wait_ld();
+                    if (masked) {
+#pragma unroll
+                        for (int i = 0; i < 128; i++)
+                            if (i < rlo || i >= rhi || ((gone >> (i / 16)) & 1u)) x[i] = -INFINITY;
+#pragma unroll
+                        for (int e = 0; e < 4; e++) mx[e] = -INFINITY;  // over the visible ones only
+#pragma unroll
+                        for (int i = 0; i < 64; i += 8)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) mx[e] = max3(mx[e], x[i + e], x[i + 4 + e]);
+                    }
+#pragma unroll
+                    for (int i = 64; i < 128; i += 8)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) mx[e] = max3(mx[e], x[i + e], x[i + 4 + e]);
+                    const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                    const bool up = mt > m + grow || (m == -INFINITY && mt > m);
+                    if (__any_sync(~0u, up)) {
+                        const float mn = up ? mt : m;
+                        const float f = up ? ex2((m - mn) * c2) : 1.f;  // 0 from -inf
+                        m = mn;
+                        l *= f;
+                        if (j > 0) {  // O is complete: S was issued behind it
+#pragma unroll 1
+                            for (int i = 0; i < HD / 16; i++) {
+                                float ov[16];
+                                asm volatile(
+                                    "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
+                                    "%14,%15}, [%16];"
+                                    : "=f"(ov[0]), "=f"(ov[1]), "=f"(ov[2]), "=f"(ov[3]), "=f"(ov[4]), "=f"(ov[5]),
+                                      "=f"(ov[6]), "=f"(ov[7]), "=f"(ov[8]), "=f"(ov[9]), "=f"(ov[10]), "=f"(ov[11]),
+                                      "=f"(ov[12]), "=f"(ov[13]), "=f"(ov[14]), "=f"(ov[15])
+                                    : "r"(to + i * 16));
+                                tmem_wait_ld();
+                                uint32_t r[16];
+#pragma unroll
+                                for (int e = 0; e < 16; e++) r[e] = __float_as_uint(ov[e] * f);
+                                tmem_st16(to + i * 16, r);
+                            }
+                        }
+                    }
+                    const float mm = m == -INFINITY ? 0.f : m;
+                    const float mc = -mm * c2;
+                    const f32x2 cc = pack2(c2, c2), nm = pack2(mc, mc);
+#pragma unroll
+                    for (int half = 0; half < 2; half++) {
+#pragma unroll
+                        for (int q16 = 0; q16 < 2; q16++) {
+                            uint32_t ph[16];
+#pragma unroll
+                            for (int e = 0; e < 32; e += 2) {
+                                const int i = half * 64 + q16 * 32 + e;
+                                float u, v;
+                                unpack2(fma2(pack2(x[i], x[i + 1]), cc, nm), u, v);
+                                u = ex2(u);
+                                v = ex2(v);
+                                sum = add2(sum, pack2(u, v));
+                                ph[e / 2] = Pair<TC>::pack(u, v);
+                            }
+                            tmem_st16(ts + half * 32 + q16 * 16, ph);
+                        }
+                        tmem_wait_st();
+                        tc_fence_before();
+                        mbar_arrive(&bars.p_full[s][half]);
+                    }
                 }
                 float u, v;
                 unpack2(sum, u, v);
@@ -432,7 +508,7 @@ __global__ void __launch_bounds__(NT, 1) attn_many_kernel(PagedArgs a, PagedQuer
                 ok = mbar_wait(&bars.o_full[s], 0, &abort_flag);
                 tc_fence_after();
                 inv = l == 0.f ? 0.f : 1.f / l;
-                if (l != 0.f) lse2 = m * c2 + log2f(l);
+                if (l != 0.f) lse2 = m * c2 - LIFT + log2f(l);
             }
             ok = group_all<128>(s + 1, ok);
             const bool direct = o.plan.many_splits == 1;
@@ -450,12 +526,16 @@ __global__ void __launch_bounds__(NT, 1) attn_many_kernel(PagedArgs a, PagedQuer
             auto leave = [&](auto *dst0, size_t stride, size_t row_step) {
                 using TO = typename std::remove_pointer<decltype(dst0)>::type;
                 constexpr int COLS = 128 / sizeof(TO);
-#pragma unroll 1
+#pragma unroll(SPLIT ? HD : 1)
                 for (int c0 = 0; c0 < HD; c0 += COLS) {
                     float ov[COLS];
 #pragma unroll
                     for (int i = 0; i < COLS; i += 32) tmem_ld32(to + c0 + i, ov + i);
                     tmem_wait_ld();
+                    if constexpr (SPLIT) {
+#pragma unroll
+                        for (int i = 0; i < COLS; i++) ov[i] += osum[c0 + i];
+                    }
 #pragma unroll
                     for (int c = 0; c < 8; c++) {
                         uint4 u;
