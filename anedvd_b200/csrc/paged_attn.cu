@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, FewGeo<HD>::CTAS)
                     }
                     __syncwarp();
                 }
-                float sc[2][4] = {};
+                float sc[2][4] = {}, slo[2][4] = {};
 #pragma unroll
                 for (int ks = 0; ks < HD / 16; ks++) {
                     // keys 0-7 | 8-15 x dims 0-7 | 8-15 of this k step
@@ -278,10 +278,13 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, FewGeo<HD>::CTAS)
                     mma16816<TC>(sc[0], qf[ks], kf[0], kf[1]);
                     mma16816<TC>(sc[1], qf[ks], kf[2], kf[3]);
                     if constexpr (SPLIT) {
-                        mma16816<TC>(sc[0], ql[ks], kf[0], kf[1]);
-                        mma16816<TC>(sc[1], ql[ks], kf[2], kf[3]);
+                        mma16816<TC>(slo[0], ql[ks], kf[0], kf[1]);
+                        mma16816<TC>(slo[1], ql[ks], kf[2], kf[3]);
                     }
                 }
+                if constexpr (SPLIT)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) sc[0][e] += slo[0][e], sc[1][e] += slo[1][e];
                 uint32_t phi[4], plo[4];
                 float p[2][4];
 #pragma unroll
@@ -324,12 +327,12 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, FewGeo<HD>::CTAS)
                     uint32_t vf[4];
                     const uint32_t r = lane & 15, c = d * 2 + (lane >> 4);
                     ldsm4t(vf, va + (c / 8) * 2048 + sw128(r, c & 7));
-                    mma16816<TC>(acc[2 * d], phi, vf[0], vf[1]);
-                    mma16816<TC>(acc[2 * d + 1], phi, vf[2], vf[3]);
                     if (SPLIT) {
                         mma16816<TC>(acc[2 * d], plo, vf[0], vf[1]);
                         mma16816<TC>(acc[2 * d + 1], plo, vf[2], vf[3]);
                     }
+                    mma16816<TC>(acc[2 * d], phi, vf[0], vf[1]);
+                    mma16816<TC>(acc[2 * d + 1], phi, vf[2], vf[3]);
                 }
                 if (tail) fence_async_smem();  // the zeros are written before the stage is loaded again
             }

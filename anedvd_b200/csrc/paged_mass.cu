@@ -239,7 +239,8 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
                             for (int ks = 0; ks < HD / 16; ks++) {
                                 const uint32_t off = (ks / 4) * (128 * 128) + (ks % 4) * 32;
                                 umma_ss(leader, tmem + (s * 2 + buf) * 128, sdesc_sw128(kb + off, 16, 1024),
-                                        sdesc_sw128(qb + part * G::TILE + off, 16, 1024), id, part | ks ? 1u : 0u);
+                                        sdesc_sw128(qb + (SPLIT ? 1 - part : 0) * G::TILE + off, 16, 1024), id,
+                                        part | ks ? 1u : 0u);  // the low parts first
                             }
                         umma_commit(leader, &s_full[s][buf]);
                         if (leader) mbar_arrive(&s_full[s][buf]);  // hands on what the query warps wrote to s_nlse
