@@ -274,6 +274,7 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(EvictArgs p) 
     __shared__ uint32_t s_digit, s_need, s_above[8], s_equal[8], warp_a[SEL_THREADS / 32];
     __shared__ uint2 s_run[SEL_PER * SEL_THREADS / 32];  // kept for sure and equal, by warps of slots
     uint32_t rank, ranks;
+    griddep_launch();  // the move may take its place; it waits for this grid's end
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
     const uint32_t x = blockIdx.x / ranks, b = x / p.a.kv_heads, h = x % p.a.kv_heads;
