@@ -89,11 +89,8 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_append_kernel(RopeArgs p, R
     const uint32_t tok0 = blockIdx.x * T, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t half = tab.rot / 2, u = threadIdx.x % UNITS;
     if (warp < T) {
-        // the sequence of a token: how many sequences end at or before it
         const int tok = (int)(tok0 + warp);
-        uint32_t n = 0;
-        for (uint32_t s = 0; s < p.a.n_seqs; s += 32)
-            n += __popc(__ballot_sync(~0u, s + lane < p.a.n_seqs && __ldg(p.a.q_start + s + lane + 1) <= tok));
+        const uint32_t n = p.a.sequence_of(tok);
         if (lane == 0) {
             int seq = -1, slot = -1, page = -1;
             if (n < p.a.n_seqs && tok < (int)p.a.n_tok) {
@@ -478,8 +475,8 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(EvictArgs p) {
     const uint32_t n = p.a.len(b);
     const int32_t *kept = p.kept + ((size_t)b * p.a.kv_heads + h) * p.keep;
     if (part == 2) {
-        if (!p.mass_out) return;
         griddep_wait();
+        if (!p.mass_out) return;
         const float *src = p.mass + ((size_t)b * p.a.kv_heads + h) * p.mass_stride;
         float *dst = p.mass_out + ((size_t)b * p.a.kv_heads + h) * p.mass_out_stride;
         const uint32_t live = min(n, p.keep);
@@ -504,7 +501,10 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(EvictArgs p) {
         for (uint32_t i = live + rank * MOVE_THREADS + threadIdx.x; i < n; i += ranks * MOVE_THREADS) dst[i] = 0.f;
         return;
     }
-    if (n <= p.keep) return;  // every slot stays where it is: the same for the whole cluster
+    if (n <= p.keep) {  // every slot stays where it is: the same for the whole cluster
+        griddep_wait();  // every CTA waits, so this grid ends after the selection
+        return;
+    }
     uint8_t *pool = reinterpret_cast<uint8_t *>(part ? p.a.v : p.a.k);
     auto place = [&](uint32_t slot) -> int64_t {  // offset of its row, below 0 on a hole
         const int pg = p.a.page(b, slot >> p.a.page_shift);

@@ -47,6 +47,18 @@ struct PagedArgs {
         const uint32_t end = e <= 0 ? 0u : min((uint32_t)e, n_tok);
         return end > first ? end - first : 0u;
     }
+    // the sequence of token row `tok`, by a whole warp: how many sequences end at or before
+    // it (q_start ascends), 32 probes at a time; n_seqs for a row of no sequence
+    __device__ __forceinline__ uint32_t sequence_of(int tok) const {
+        const uint32_t lane = threadIdx.x & 31;
+        uint32_t lo = 0, size = n_seqs;
+        while (size) {
+            const uint32_t step = (size + 31) / 32, end = lo + size, last = lo + (lane + 1) * step - 1;
+            lo += step * __popc(__ballot_sync(~0u, last < end && __ldg(q_start + last + 1) <= tok));
+            size = lo < end ? min(step - 1, end - lo) : 0;
+        }
+        return min(lo, n_seqs);
+    }
     __device__ __forceinline__ int page(uint32_t b, uint32_t col) const {
         const int id = __ldg(pages + (size_t)b * pages_stride + col);
         return (id >= 0 && (uint32_t)id < n_pages) ? id : -1;
@@ -188,6 +200,7 @@ struct AttnOut {
     // parts: normalised outputs [part][rows][hd] and log2 sums [part][rows]; rows are
     // few_rows of the few, [n_tok][heads] of the many
     float *few_o, *few_lse, *many_o, *many_lse;
+    uint32_t *few_units;  // [n_seqs + 1]: units of the few's sequences before each (per KV head)
     AttnPlan plan;
 };
 int launch_attention_many(const AttnPagedCall &c, const AttnOut &o, cudaStream_t s);

@@ -30,6 +30,7 @@ __device__ int g_timeout;  // a bounded wait of this file's kernels gave up
 constexpr int FEW_WARPS = 4, FEW_ST = 2, FEW_KEYS = 16;
 constexpr uint32_t FEW_RUN = 4;   // blocks a warp takes at least
 constexpr uint32_t FEW_ITEM = 3;  // blocks' worth of an item's own cost
+constexpr uint32_t FEW_COUNTED = 32;  // sequences whose units the merge counts for itself
 
 template <int HD>
 struct FewGeo {
@@ -59,20 +60,6 @@ struct FewSeq {
     }
 };
 
-// Units per KV head of all sequences, and of those before sequence `upto`, counted
-// by a whole warp.
-__device__ __forceinline__ uint32_t few_total(const PagedArgs &a, const PagedQuery &q, const AttnPlan &plan, uint32_t upto,
-                                              uint32_t &before) {
-    const uint32_t lane = threadIdx.x & 31;
-    uint32_t sum = 0, part = 0;
-    for (uint32_t b = lane; b < a.n_seqs; b += 32) {
-        const uint32_t v = FewSeq(a, q, plan, b).units();
-        sum += v;
-        part += b < upto ? v : 0;
-    }
-    before = __reduce_add_sync(~0u, part);
-    return __reduce_add_sync(~0u, sum);
-}
 // Units of one warp's run.
 __device__ __forceinline__ uint32_t few_run(uint32_t total, uint32_t kv_heads, uint32_t ctas) {
     const uint32_t warps = ctas * FEW_WARPS;
@@ -109,6 +96,21 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, FewGeo<HD>::CTAS)
     total = __reduce_add_sync(~0u, total);
     __syncthreads();
     const uint32_t gw = blockIdx.x * FEW_WARPS + warp;
+    if (a.n_seqs > FEW_COUNTED && gw == gridDim.x * FEW_WARPS - 1) {  // the last warp, which has the least to do: the table for the merge
+        uint32_t before = 0;
+        for (uint32_t s0 = 0; s0 < a.n_seqs; s0 += 32) {
+            const uint32_t v = s0 + lane < a.n_seqs ? FewSeq(a, q, o.plan, s0 + lane).units() : 0;
+            uint32_t upto = v;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const uint32_t up = __shfl_up_sync(~0u, upto, d);
+                if (lane >= (uint32_t)d) upto += up;
+            }
+            if (s0 + lane < a.n_seqs) o.few_units[s0 + lane] = before + upto - v;
+            before += __shfl_sync(~0u, upto, 31);
+        }
+        if (lane == 0) o.few_units[a.n_seqs] = total;
+    }
     const uint32_t run = few_run(total, a.kv_heads, gridDim.x);
     uint32_t left = 0;  // units of this warp's run
     {
@@ -385,23 +387,34 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) attn_merge_kernel(PagedArgs 
     const uint32_t lane = threadIdx.x & 31;
     const uint32_t row = blockIdx.x * MERGE_WARPS + (threadIdx.x >> 5);
     const uint32_t tok = row / q.heads, head = row % q.heads;
-    if (tok >= a.n_tok) return;
-    uint32_t b = 0;  // sequences that end at or before the token
-    for (uint32_t s = 0; s < a.n_seqs; s += 32)
-        b += __popc(__ballot_sync(~0u, s + lane < a.n_seqs && __ldg(a.q_start + s + lane + 1) <= (int)tok));
-    if (b >= a.n_seqs) return;
-    uint32_t first;
-    const uint32_t nq = a.tokens(b, first), n = a.len(b);
-    if (tok < first || tok - first >= min(nq, a.max_q)) return;
+    const uint32_t b = tok < a.n_tok ? a.sequence_of((int)tok) : a.n_seqs;
+    uint32_t first = 0, nq = 0;
+    if (b < a.n_seqs) nq = a.tokens(b, first);
     const uint32_t tq = min(nq, a.max_q), i = tok - first;
     const bool few = o.plan.is_few(tq, q.group);
+    // a row of no sequence, past max_q, or written by its kernel
+    const bool none = b >= a.n_seqs || tok < first || i >= tq || (!few && o.plan.many_splits == 1);
+    const FewSeq sq(a, q, o.plan, none ? 0 : b);
+    // units before the sequence, and of all: up to 32 sequences are counted here, before
+    // the wait (decode of 32 requests 39.8 us; 41.1 with the table, which more need: a
+    // count over 1000 sequences in each of the merge's warps would take longer than it)
+    uint32_t before = 0, total_units = 0;
+    if (a.n_seqs <= FEW_COUNTED) {
+        const uint32_t v = lane < a.n_seqs ? FewSeq(a, q, o.plan, lane).units() : 0;
+        total_units = __reduce_add_sync(~0u, v);
+        before = __reduce_add_sync(~0u, lane < b ? v : 0);
+    }
+    griddep_wait();  // what is above reads the batch alone; every warp waits, so this grid ends last
+    if (none) return;
     uint32_t parts = o.plan.many_splits;
     size_t step = (size_t)a.n_tok * q.heads, at = (size_t)tok * q.heads + head;
     const float *part_o = o.many_o, *part_lse = o.many_lse;
     if (few) {  // the warps whose runs hold blocks of this item
-        uint32_t before;
-        const uint32_t total = few_total(a, q, o.plan, b, before), run = few_run(total, a.kv_heads, o.plan.few_ctas);
-        const FewSeq sq(a, q, o.plan, b);
+        if (a.n_seqs > FEW_COUNTED) {
+            before = o.few_units[b];
+            total_units = o.few_units[a.n_seqs];
+        }
+        const uint32_t run = few_run(total_units, a.kv_heads, o.plan.few_ctas);
         const uint32_t kvh = head / q.group;
         const uint64_t x0 = (uint64_t)before * a.kv_heads + (uint64_t)kvh * sq.units();
         const uint32_t w0 = (uint32_t)(x0 / run), w1 = (uint32_t)((x0 + sq.nblk + run - 1) / run);
@@ -410,10 +423,7 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) attn_merge_kernel(PagedArgs 
         at = (w0 + (size_t)b * a.kv_heads + kvh) * step + i * q.group + head % q.group;
         part_o = o.few_o;
         part_lse = o.few_lse;
-    } else if (o.plan.many_splits == 1) {
-        return;  // written by its kernel
     }
-    griddep_wait();  // what is above reads the batch alone
     float v[E], total = 0.f, top = -INFINITY;
 #pragma unroll
     for (int e = 0; e < E; e++) v[e] = 0.f;
@@ -500,17 +510,17 @@ int make_page_map(CUtensorMap *m, const void *pool, const PagedArgs &a, uint32_t
     typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-    static EncodeFn encode = nullptr;
-    if (!encode) {
+    static const EncodeFn encode = []() -> EncodeFn {  // the driver's, looked up through the runtime
         void *fn = nullptr;
         cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &q) !=
-                cudaSuccess ||
-            q != cudaDriverEntryPointSuccess || !fn) {
-            set_error("paged cache: cuTensorMapEncodeTiled is not available from the driver");
-            return CUQ_ECUDA;
-        }
-        encode = reinterpret_cast<EncodeFn>(fn);
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            return nullptr;
+        return reinterpret_cast<EncodeFn>(fn);
+    }();
+    if (!encode) {
+        set_error("paged cache: cuTensorMapEncodeTiled is not available from the driver");
+        return CUQ_ECUDA;
     }
     const CUresult r = encode(m, type == CUQ_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5,
                               const_cast<void *>(pool), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -553,21 +563,22 @@ AttnPlan attention_paged_plan(const AttnPagedCall &c, int sm_count) {
 }
 
 namespace {
-// floats of the few's outputs, the many's outputs, the few's sums, the many's sums
-void part_sizes(const AttnPagedCall &c, const AttnPlan &p, size_t (&n)[4]) {
+// floats of the few's outputs, the many's outputs, the few's sums, the many's sums, and the few's table
+void part_sizes(const AttnPagedCall &c, const AttnPlan &p, size_t (&n)[5]) {
     const size_t few = p.few ? ((size_t)p.few_ctas * FEW_WARPS + (size_t)c.a.n_seqs * c.a.kv_heads) * p.few_rows : 0;
     const size_t many = p.many_splits > 1 ? (size_t)p.many_splits * c.a.n_tok * c.q.heads : 0;
     n[0] = few * c.hd;
     n[1] = many * c.hd;
     n[2] = few;
     n[3] = many;
+    n[4] = p.few && c.a.n_seqs > FEW_COUNTED ? (size_t)c.a.n_seqs + 1 : 0;
 }
 }  // namespace
 
 size_t attention_paged_workspace(const AttnPagedCall &c, int sm_count) {
-    size_t n[4];
+    size_t n[5];
     part_sizes(c, attention_paged_plan(c, sm_count), n);
-    return (n[0] + n[1] + n[2] + n[3]) * sizeof(float);
+    return (n[0] + n[1] + n[2] + n[3] + n[4]) * sizeof(float);
 }
 
 int launch_attention_paged(const AttnPagedCall &c, int sm_count, cudaStream_t s) {
@@ -576,12 +587,13 @@ int launch_attention_paged(const AttnPagedCall &c, int sm_count, cudaStream_t s)
     o.out_stride = c.out_stride;
     o.lse = c.lse;
     o.plan = attention_paged_plan(c, sm_count);
-    size_t n[4];
+    size_t n[5];
     part_sizes(c, o.plan, n);
     o.few_o = reinterpret_cast<float *>(c.workspace);
     o.many_o = o.few_o + n[0];
     o.few_lse = o.many_o + n[1];
     o.many_lse = o.few_lse + n[2];
+    o.few_units = reinterpret_cast<uint32_t *>(o.many_lse + n[3]);
     if (c.type == CUQ_F32) return launch_all<float, __half>(c, o, s);
     if (c.type == CUQ_F16) return launch_all<__half, __half>(c, o, s);
     return launch_all<__nv_bfloat16, __nv_bfloat16>(c, o, s);

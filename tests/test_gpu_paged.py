@@ -199,6 +199,112 @@ def test_bad_batch_arrays_touch_nothing():
         assert not out.isnan().any()
 
 
+@pytest.mark.parametrize("pair", PAIRS)
+def test_wide_groups(pair):
+    """More query heads a KV head than a tile has rows."""
+    run_attention([(1, 40), (3, 130), (2, 2)], 300, 1, 64, pair, page=32)
+    run_attention([(1, 300), (5, 77)], 17, 1, 128, pair, page=32)
+
+
+@pytest.mark.parametrize("pair", PAIRS)
+def test_many_sequences(pair):
+    """Hundreds of sequences: single tokens alone, and mixed with chunks and empty ones."""
+    run_attention([(1, 1 + (37 * i) % 90) for i in range(1100)], 4, 2, 64, pair, tail=1)
+    run_attention([((0, 1, 1, 9, 1)[i % 5], (i * 29) % 120 if i % 5 else 40) for i in range(300)], 6, 2, 64, pair, window=50)
+
+
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-3])
+def test_scales(scale):
+    for pair in PAIRS:
+        t, cache = pair
+        b = pu.Batch([(1, 70), (40, 90), (150, 150)], 2, 64, cache, 16)
+        q, row, qh = queries(b, 4, t)
+        out, lse = attend(b, 4, t, q, row, scale)
+        check_attention(b, 4, t, out, lse, qh, scale)
+
+
+def test_offsets_past_32_bits():
+    """Pools of more than 2^32 elements, with the pages at their far end."""
+    stride, n_pages = 1 << 28, 18                       # 4.8e9 elements, 9.7 GB a pool
+    b = pu.Batch([(1, 70), (33, 60)], 1, 64, "f16", 16)
+    far = {n: torch.empty(n_pages, stride, dtype=torch.float16, device="cuda") for n in ("k", "v")}
+    ids = list(range(n_pages - b.n_pages, n_pages)) if b.n_pages <= n_pages else None
+    assert ids
+    for i, p in enumerate(ids):
+        far["k"][p, : b.stride] = b.k[i]
+        far["v"][p, : b.stride] = b.v[i]
+    b.table = torch.where(b.table < b.n_pages, b.table + ids[0], torch.tensor(1 << 30, dtype=torch.int32))
+    b.d_table.copy_(b.table)
+    near_k, near_v, first = b.k_host, b.v_host, ids[0]
+    b.kv_desc.k, b.kv_desc.v = far["k"].data_ptr(), far["v"].data_ptr()
+    b.kv_desc.page_stride, b.kv_desc.n_pages = stride, n_pages
+    L = lib()
+    row = (4 + 2) * 64
+    x = torch.randn(b.n_tok, row, device="cuda").half()
+    q = torch.empty(b.n_tok, 4 * 64, dtype=torch.float16, device="cuda")
+    plan = rt.RopePlan(rt.CuqRopeParams(rot_dim=64, theta=1e4))
+    rt.check(L.cuq_rope_append(plan.handle, b.kvp, b.bp, None, ptr(q), 256, 1, ptr(x), row,
+                               ctypes.c_void_p(x.data_ptr() + 512), ctypes.c_void_p(x.data_ptr() + 640), row, 1, 4, None))
+    out, lse = attend(b, 4, "f16", q, 256, 0.125)
+    mass = torch.zeros(2, 1, b.max_kv, device="cuda")
+    rt.check(L.cuq_attention_mass(b.kvp, b.bp, ptr(mass), b.max_kv, ptr(q), 256, 1, ptr(lse), 4, 0.125, 1, 0, 0, 1.0, None))
+    rt.check(L.cuq_paged_status(None))
+    # the model sees the same rows in small pools
+    b.k_host = torch.stack([far["k"][p, : b.stride].cpu() for p in ids])
+    b.v_host = torch.stack([far["v"][p, : b.stride].cpu() for p in ids])
+    assert not torch.equal(b.k_host, near_k) and not torch.equal(b.v_host, near_v)
+    b.table = torch.where(b.table < n_pages, b.table - first, b.table)
+    check_attention(b, 4, "f16", out, lse, q.view(b.n_tok, 4, 64).cpu(), 0.125)
+    for i, (_, n) in enumerate(b.seqs):
+        want = 4.0 * b.seqs[i][0]
+        assert abs(float(mass[i, :, :n].sum()) - want) < 2.0 ** -10 * want
+    m0 = mass.cpu()
+    kept = torch.empty(2, 1, 20, dtype=torch.int32, device="cuda")
+    new = torch.empty(2, dtype=torch.int32, device="cuda")
+    rt.check(L.cuq_kv_evict(b.kvp, b.bp, ptr(mass), b.max_kv, 20, 2, 4, ptr(kept), ptr(new), None, b.max_kv, None))
+    torch.cuda.synchronize()
+    for i, (_, n) in enumerate(b.seqs):
+        keep = pu.evict(m0[i, 0], n, 20, 2, 4)
+        assert kept[i, 0].tolist() == keep
+        rows, _ = b.rows(b.k_host, i, n)
+        for j, s in enumerate(keep):
+            page = int(b.table[i, j // 16]) + first
+            assert torch.equal(far["k"][page, (j % 16) * 64:(j % 16 + 1) * 64].cpu().double(), rows[s, 0])
+
+
+def test_captured_before_any_other_call():
+    """A process whose first call of each op is made while a graph is captured."""
+    import subprocess
+    import sys
+
+    code = """
+import ctypes, torch
+from tests import paged_util as pu
+from tests.test_gpu_paged import *
+L = rt.load(); rt.init(0)
+b = pu.Batch([(1, 40), (40, 300), (1, 7)], 2, 128, "bf16", 16)
+q, row, qh = queries(b, 8, "bf16")
+need = L.cuq_attention_paged_workspace(b.kvp, b.bp, 8, 30)
+ws = torch.empty(max(1, need), dtype=torch.uint8, device="cuda")
+out, lse = torch.full((b.n_tok, 1024), 7.0, dtype=torch.bfloat16, device="cuda"), torch.full((b.n_tok, 8), 7.0, device="cuda")
+mass = torch.zeros(3, 2, b.max_kv, device="cuda")
+kept = torch.empty(3, 2, 30, dtype=torch.int32, device="cuda"); new = torch.empty(3, dtype=torch.int32, device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    s = torch.cuda.current_stream().cuda_stream
+    rt.check(L.cuq_attention_paged(b.kvp, b.bp, ptr(out), 1024, ptr(q), row, 30, ptr(lse), 8, 0.1, 1, 0, ptr(ws), need, s))
+    rt.check(L.cuq_attention_mass(b.kvp, b.bp, ptr(mass), b.max_kv, ptr(q), row, 30, ptr(lse), 8, 0.1, 1, 0, 0, 1.0, s))
+    rt.check(L.cuq_kv_evict(b.kvp, b.bp, ptr(mass), b.max_kv, 30, 2, 4, ptr(kept), ptr(new), None, b.max_kv, s))
+g.replay(); torch.cuda.synchronize()
+check_attention(b, 8, "bf16", out, lse, qh, 0.1)
+assert new.tolist() == [30, 30, 7]
+print("captured")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=240)
+    assert "captured" in r.stdout, r.stdout[-2000:] + r.stderr[-2000:]
+
+
 # ------------------------------------------------------------------ rotary + append ----
 
 ROPES = [dict(rot_dim=64), dict(rot_dim=64, adjacent=1, theta=5e5), dict(rot_dim=32, scaling=rt.ROPE_LINEAR, factor=4.0),
@@ -337,6 +443,12 @@ def test_mass_masks(pair):
     run_mass([(1, 900), (40, 500), (150, 400)], 12, 2, 128, pair, page=32, window=100, holes=holes, decay=0.5)
     run_mass([(1, 900), (40, 500), (150, 400)], 9, 3, 64, pair, page=32, causal=False, holes=holes, decay=-0.5)
     run_mass([(700, 900)], 4, 2, 64, pair, page=16, decay=0.9)
+
+
+@pytest.mark.parametrize("pair", PAIRS)
+def test_mass_of_many_sequences(pair):
+    run_mass([((i % 4), (i * 17) % 70) for i in range(1500)], 4, 2, 64, pair)
+    run_mass([(40, 90), (3, 300)], 160, 1, 64, pair, page=32)
 
 
 def test_mass_repeats_bit_for_bit():
