@@ -30,7 +30,6 @@ __device__ int g_timeout;  // a bounded wait of this file's kernels gave up
 constexpr int FEW_WARPS = 4, FEW_ST = 2, FEW_KEYS = 16;
 constexpr uint32_t FEW_RUN = 4;   // blocks a warp takes at least
 constexpr uint32_t FEW_ITEM = 3;  // blocks' worth of an item's own cost
-constexpr uint32_t FEW_COUNTED = 32;  // sequences whose units the merge counts for itself
 
 template <int HD>
 struct FewGeo {
@@ -96,7 +95,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, FewGeo<HD>::CTAS)
     total = __reduce_add_sync(~0u, total);
     __syncthreads();
     const uint32_t gw = blockIdx.x * FEW_WARPS + warp;
-    if (a.n_seqs > FEW_COUNTED && gw == gridDim.x * FEW_WARPS - 1) {  // the last warp, which has the least to do: the table for the merge
+    if (gw == gridDim.x * FEW_WARPS - 1) {  // the last warp, which has the least to do: the table for the merge
         uint32_t before = 0;
         for (uint32_t s0 = 0; s0 < a.n_seqs; s0 += 32) {
             const uint32_t v = s0 + lane < a.n_seqs ? FewSeq(a, q, o.plan, s0 + lane).units() : 0;
@@ -395,26 +394,13 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) attn_merge_kernel(PagedArgs 
     // a row of no sequence, past max_q, or written by its kernel
     const bool none = b >= a.n_seqs || tok < first || i >= tq || (!few && o.plan.many_splits == 1);
     const FewSeq sq(a, q, o.plan, none ? 0 : b);
-    // units before the sequence, and of all: up to 32 sequences are counted here, before
-    // the wait (decode of 32 requests 39.8 us; 41.1 with the table, which more need: a
-    // count over 1000 sequences in each of the merge's warps would take longer than it)
-    uint32_t before = 0, total_units = 0;
-    if (a.n_seqs <= FEW_COUNTED) {
-        const uint32_t v = lane < a.n_seqs ? FewSeq(a, q, o.plan, lane).units() : 0;
-        total_units = __reduce_add_sync(~0u, v);
-        before = __reduce_add_sync(~0u, lane < b ? v : 0);
-    }
     griddep_wait();  // what is above reads the batch alone; every warp waits, so this grid ends last
     if (none) return;
     uint32_t parts = o.plan.many_splits;
     size_t step = (size_t)a.n_tok * q.heads, at = (size_t)tok * q.heads + head;
     const float *part_o = o.many_o, *part_lse = o.many_lse;
     if (few) {  // the warps whose runs hold blocks of this item
-        if (a.n_seqs > FEW_COUNTED) {
-            before = o.few_units[b];
-            total_units = o.few_units[a.n_seqs];
-        }
-        const uint32_t run = few_run(total_units, a.kv_heads, o.plan.few_ctas);
+        const uint32_t before = o.few_units[b], run = few_run(o.few_units[a.n_seqs], a.kv_heads, o.plan.few_ctas);
         const uint32_t kvh = head / q.group;
         const uint64_t x0 = (uint64_t)before * a.kv_heads + (uint64_t)kvh * sq.units();
         const uint32_t w0 = (uint32_t)(x0 / run), w1 = (uint32_t)((x0 + sq.nblk + run - 1) / run);
@@ -571,7 +557,7 @@ void part_sizes(const AttnPagedCall &c, const AttnPlan &p, size_t (&n)[5]) {
     n[1] = many * c.hd;
     n[2] = few;
     n[3] = many;
-    n[4] = p.few && c.a.n_seqs > FEW_COUNTED ? (size_t)c.a.n_seqs + 1 : 0;
+    n[4] = p.few ? (size_t)c.a.n_seqs + 1 : 0;
 }
 }  // namespace
 
