@@ -18,7 +18,14 @@
 // zero: over a long context that is 2e-6 of an fp32 output.  So with fp32 queries O is
 // of one tile only and the softmax threads sum the tiles in registers (4e-7).
 // What bounds it: per 128 x 128 tile the two products take 1024 cycles of the
-// tensor pipe at head_dim 128 (512 at 64) and the exponentials 1024 of the MUFU.
+// tensor pipe at head_dim 128 (512 at 64) and the exponentials 1024 of the MUFU; but
+// Q K^T reads both operands from shared memory, 8 KB a product of 64 cycles, and runs
+// at 86, so that a pair of tiles takes at least 2400 cycles and is measured at 2900.
+// Start and end of a CTA cost 11 000 more.  4096 tokens of 32 heads (8 KV heads,
+// head_dim 128, fp16, causal) take 153 us, 895 TFLOP/s, 52 % of the measured product
+// rate; 512 tokens over 32768 slots (12 heads, 2 KV heads, bf16) 101 us, 1.01 PFLOP/s.
+// Tried and not kept: a quarter of the exponentials as polynomials on the FMA pipe
+// (155 us), queries and first tile loaded before the first barrier (162 us).
 #include "paged_tc.cuh"
 
 namespace cuq {

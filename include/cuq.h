@@ -278,7 +278,9 @@ int cuq_rope_append(const cuq_rope_plan *rope, const cuq_paged_kv *kv, const cuq
  * with an fp16 cache (q and the probabilities then run as fp16 hi + lo pairs).
  * causal: a token sees the slots up to its own; window > 0 (causal only): and
  * of those the last `window`.  A token that sees nothing gets out 0 and lse
- * -inf.  lse [n_tok][heads] (may be NULL): the natural log of the sum of
+ * -inf.  Slots at or past kv_len and slots on a hole may hold anything; a NaN or
+ * infinity in a V row before kv_len can reach tokens of its tile that do not see
+ * it.  lse [n_tok][heads] (may be NULL): the natural log of the sum of
  * exponentials.  workspace: cuq_attention_paged_workspace bytes, 256-byte
  * aligned (may be NULL when that is 0); two calls that may run at the same
  * time need one each. */
