@@ -159,8 +159,16 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, FewGeo<HD>::CTAS)
     // ---- the loading cursor, FEW_ST blocks ahead of the computing one
     uint32_t lb = b0, lh = h0, lk = k0, to_load = left, ist = 0;
     FewSeq ls(a, q, o.plan, lb);
-    uint32_t ids_at = ~0u;  // lane i: page of block ids_at + i of sequence lb
+    // lane i: page id, as the table holds it, of block ids_at + i of sequence lb
+    uint32_t ids_at = ~0u;
     int ids = 0;
+    auto look = [&]() {
+        ids_at = lk;
+        ids = lk + lane < ls.nblk ? __ldg(a.pages + (size_t)lb * a.pages_stride +
+                                          (((ls.blk0 + lk + lane) * FEW_KEYS) >> a.page_shift))
+                                  : -1;
+    };
+    if (lk < ls.nblk) look();  // on its way while the queries are loaded
     auto issue = [&]() -> int {  // the next block into its stage; its page, or -1
         while (to_load && lk >= ls.nblk) {  // past the item's blocks: on to the next one
             const uint32_t skip = min(to_load, ls.nblk + FEW_ITEM - lk);
@@ -176,11 +184,9 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, FewGeo<HD>::CTAS)
         }
         if (!to_load) return -1;
         to_load--;
-        if (lk < ids_at || lk >= ids_at + 32) {
-            ids_at = lk;
-            ids = lk + lane < ls.nblk ? a.page(lb, ((ls.blk0 + lk + lane) * FEW_KEYS) >> a.page_shift) : -1;
-        }
-        const int pg = __shfl_sync(~0u, ids, lk - ids_at);
+        if (lk < ids_at || lk >= ids_at + 32) look();
+        int pg = __shfl_sync(~0u, ids, lk - ids_at);
+        if ((uint32_t)pg >= a.n_pages) pg = -1;
         if (lane == 0) {
             const uint32_t dst = smem_u32(ring + ist * 2 * G::ROWS);
             const int slot = (int)(((ls.blk0 + lk) * FEW_KEYS) & (a.page_size - 1)), p = pg < 0 ? (int)a.n_pages : pg;
