@@ -90,6 +90,7 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_append_kernel(RopeArgs p, R
     constexpr uint32_t UNITS = HD / 16, STEP = ROPE_THREADS / UNITS;
     const uint32_t tok0 = blockIdx.x * T, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t half = tab.rot / 2, u = threadIdx.x % UNITS, rows = p.heads + 2 * p.a.kv_heads;
+    griddep_wait();
     // row r (q heads, k heads, v heads) of a token
     auto source = [&](uint32_t tok, uint32_t r) -> const TI * {
         if (r < p.heads) return reinterpret_cast<const TI *>(p.q) + (size_t)tok * p.q_stride + (size_t)r * HD;
@@ -219,15 +220,11 @@ int launch_rope_append(const RopeArgs &p, const RopeTable &t, int out_type, int 
     // each 28.6 and with four 26.7; 16 tokens 9.3 us with one, 9.4 with two
     const bool many = p.a.n_tok >= 1024;
     const uint32_t grid = many ? (p.a.n_tok + 1) / 2 : p.a.n_tok;
-    if (hd == 64 && many)
-        rope_append_kernel<TI, 64, 2><<<grid, ROPE_THREADS, 0, s>>>(p, t, out_type, cache_type);
-    else if (hd == 64)
-        rope_append_kernel<TI, 64, 1><<<grid, ROPE_THREADS, 0, s>>>(p, t, out_type, cache_type);
-    else if (many)
-        rope_append_kernel<TI, 128, 2><<<grid, ROPE_THREADS, 0, s>>>(p, t, out_type, cache_type);
-    else
-        rope_append_kernel<TI, 128, 1><<<grid, ROPE_THREADS, 0, s>>>(p, t, out_type, cache_type);
-    CUQ_CUDA_TRY(cudaGetLastError());
+    auto launch = [&](auto kernel) {
+        return launch_maybe_pdl(kernel, dim3(grid), dim3(ROPE_THREADS), 0, s, true, p, t, out_type, cache_type);
+    };
+    CUQ_CUDA_TRY(hd == 64 ? (many ? launch(rope_append_kernel<TI, 64, 2>) : launch(rope_append_kernel<TI, 64, 1>))
+                          : (many ? launch(rope_append_kernel<TI, 128, 2>) : launch(rope_append_kernel<TI, 128, 1>)));
     return CUQ_OK;
 }
 
@@ -287,6 +284,7 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(EvictArgs p) 
     __shared__ uint32_t s_digit, s_need, s_above[8], s_equal[8], warp_a[SEL_THREADS / 32];
     __shared__ uint2 s_run[SEL_PER * SEL_THREADS / 32];  // kept for sure and equal, by warps of slots
     uint32_t rank, ranks;
+    griddep_wait();
     griddep_launch();  // the move may take its place; it waits for this grid's end
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
@@ -585,12 +583,14 @@ int launch_evict(const EvictArgs &p, uint32_t hd, int sm_count, cudaStream_t s) 
     cfg.gridDim = dim3(rows * ranks);
     cfg.blockDim = dim3(SEL_THREADS);
     cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = ranks;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cudaLaunchAttribute attrs[2];
+    attrs[0].id = cudaLaunchAttributeClusterDimension;
+    attrs[0].val.clusterDim.x = ranks;
+    attrs[0].val.clusterDim.y = attrs[0].val.clusterDim.z = 1;
+    attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attrs;
+    cfg.numAttrs = 2;
     CUQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, evict_select_kernel, p));
     if (p.a.max_kv <= p.keep && !p.mass_out) return CUQ_OK;  // nothing can move
     // as many CTAs a cluster as have rows to move, so that most calls take one or two rounds
@@ -600,17 +600,10 @@ int launch_evict(const EvictArgs &p, uint32_t hd, int sm_count, cudaStream_t s) 
     static std::atomic<uint64_t> allowed64, allowed128;
     CUQ_CUDA_TRY(hd == 64 ? allow_smem(evict_move_kernel<64>, bytes, allowed64)
                           : allow_smem(evict_move_kernel<128>, bytes, allowed128));
-    cudaLaunchAttribute attrs[2];
-    attrs[0].id = cudaLaunchAttributeClusterDimension;
     attrs[0].val.clusterDim.x = movers;
-    attrs[0].val.clusterDim.y = attrs[0].val.clusterDim.z = 1;
-    attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attrs[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.gridDim = dim3(rows * 3 * movers);
     cfg.blockDim = dim3(MOVE_THREADS);
     cfg.dynamicSmemBytes = (size_t)bytes;
-    cfg.attrs = attrs;
-    cfg.numAttrs = 2;
     CUQ_CUDA_TRY(hd == 64 ? cudaLaunchKernelEx(&cfg, evict_move_kernel<64>, p)
                           : cudaLaunchKernelEx(&cfg, evict_move_kernel<128>, p));
     return CUQ_OK;

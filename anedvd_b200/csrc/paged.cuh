@@ -10,6 +10,11 @@
 
 namespace cuq {
 
+// Every kernel of these ops is launched as a programmatic dependent of what the
+// stream holds before it, and waits (griddepcontrol.wait) before it reads anything
+// that may come from there: the order is the stream's, and a launch costs 1 to 2 us
+// less than one that waits for the stream to run dry.
+
 // SM count of the current device, asked for once per device.
 int paged_sm_count();
 // Let `kernel` use `bytes` of dynamic shared memory, set once per device (`done`

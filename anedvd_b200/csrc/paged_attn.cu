@@ -86,6 +86,9 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, FewGeo<HD>::CTAS)
     __shared__ int abort_flag;
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = warp_index();
+    // alone: wait for what came before.  Behind the many-row kernel, which has waited
+    // for it, run beside that one's tail and end after it, for the merge's sake.
+    if (!o.plan.many) griddep_wait();
     griddep_launch();  // the merge may take its place; it waits for this grid's end
     // units of the sequences [0, 32), one a lane, and of all
     const uint32_t v0 = lane < a.n_seqs ? FewSeq(a, q, o.plan, lane).units() : 0;
@@ -378,7 +381,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, FewGeo<HD>::CTAS)
             b++;
         }
     }
-    if (gw == 0) griddep_wait();  // behind the many-row kernel: this grid ends after that one, for the merge's sake
+    if (gw == 0) griddep_wait();
     if (!ok) {  // let the copies in flight land before this block's memory is given back
         if (lane == 0) g_timeout = 1;
         const unsigned long long t0 = now_ns();
@@ -479,7 +482,7 @@ int launch_few(const AttnPagedCall &c, const AttnOut &o, cudaStream_t s) {
     auto kern = attn_few_kernel<TQ, TC, HD>;
     static std::atomic<uint64_t> allowed;
     CUQ_CUDA_TRY(allow_smem(kern, FewGeo<HD>::SMEM, allowed));
-    CUQ_CUDA_TRY(launch_maybe_pdl(kern, dim3(o.plan.few_ctas), dim3(FEW_WARPS * 32), FewGeo<HD>::SMEM, s, o.plan.many, c.a,
+    CUQ_CUDA_TRY(launch_maybe_pdl(kern, dim3(o.plan.few_ctas), dim3(FEW_WARPS * 32), FewGeo<HD>::SMEM, s, true, c.a,
                                   c.q, o, mk, mv));
     return CUQ_OK;
 }

@@ -69,6 +69,7 @@ __global__ void __launch_bounds__(NT, 1) attn_many_kernel(PagedArgs a, PagedQuer
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = warp_index();
     const uint32_t kvh = blockIdx.x % a.kv_heads, split = blockIdx.y;
+    griddep_wait();
     griddep_launch();  // the few-row kernel and the merge may follow into free SMs; the merge waits for the end
 
     // the tile: tiles are counted over the sequences that are this kernel's
@@ -601,8 +602,8 @@ int launch_many(const AttnPagedCall &c, const AttnOut &o, cudaStream_t s) {
     auto kern = attn_many_kernel<TQ, TC, HD>;
     static std::atomic<uint64_t> allowed;
     CUQ_CUDA_TRY(allow_smem(kern, G::SMEM, allowed));
-    kern<<<dim3(c.a.kv_heads * o.plan.many_tiles, o.plan.many_splits), NT, G::SMEM, s>>>(c.a, c.q, o, mk, mv);
-    CUQ_CUDA_TRY(cudaGetLastError());
+    CUQ_CUDA_TRY(launch_maybe_pdl(kern, dim3(c.a.kv_heads * o.plan.many_tiles, o.plan.many_splits), dim3(NT), G::SMEM, s,
+                                  true, c.a, c.q, o, mk, mv));
     return CUQ_OK;
 }
 

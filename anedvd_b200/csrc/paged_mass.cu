@@ -108,6 +108,7 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
 
+    griddep_wait();
     if (warp == 16) tmem_alloc512(&tmem_slot);
     if (tid == 0) {
         abort_flag = 0;
@@ -555,12 +556,14 @@ int launch_mass(const MassPagedCall &c, int sm_count, cudaStream_t s) {
         cfg.blockDim = dim3(NT);
         cfg.dynamicSmemBytes = G::SMEM;
         cfg.stream = s;
-        cudaLaunchAttribute attr[1];
+        cudaLaunchAttribute attr[2];
         attr[0].id = cudaLaunchAttributeClusterDimension;
         attr[0].val.clusterDim.x = ranks;
         attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
         cfg.attrs = attr;
-        cfg.numAttrs = 1;
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
+        cfg.numAttrs = 2;
         CUQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, p, mk));
     }
     return CUQ_OK;
