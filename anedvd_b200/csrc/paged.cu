@@ -52,7 +52,7 @@ namespace {
 // one each, into shared memory, and then walk the rows (token, head) in units:
 // the 16 values that hold 8 whole pairs, two 16-byte vectors at j and j + rot/2,
 // or 16 values in a row.  4096 tokens (32 heads, 8 KV heads, head_dim 128, fp16, 101 MB)
-// take 23.1 us, 4.4 TB/s, 67 % of a copy's rate; more loads in flight a thread cost
+// take 21.3 us, 4.7 TB/s, 73 % of a copy's rate; more loads in flight a thread cost
 // occupancy and made it slower (31 us).
 struct RopeArgs {
     PagedArgs a;
@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_append_kernel(RopeArgs p, R
         return reinterpret_cast<const TI *>(is_v ? p.v : p.k) + (size_t)tok * p.kv_stride +
                (size_t)(r - p.heads - (is_v ? p.a.kv_heads : 0)) * HD;
     };
-    // into L2 while the tokens are found: 4096 tokens 24.6 -> 23.1 us (a few tokens gain nothing by it)
+    // into L2 while the tokens are found: 4096 tokens 23.1 us instead of 24.6 (a few tokens gain nothing by it)
     constexpr uint32_t LINES = T > 1 ? HD * sizeof(TI) / 128 : 0;
     for (uint32_t i = threadIdx.x; i < T * rows * LINES; i += ROPE_THREADS) {
         const uint32_t row = i / max(1u, LINES), t = row / rows;

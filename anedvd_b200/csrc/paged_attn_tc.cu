@@ -22,10 +22,11 @@
 // Q K^T reads both operands from shared memory, 8 KB a product of 64 cycles, and runs
 // at 86, so that a pair of tiles takes at least 2400 cycles and is measured at 2900.
 // Start and end of a CTA cost 11 000 more.  4096 tokens of 32 heads (8 KV heads,
-// head_dim 128, fp16, causal) take 153 us, 895 TFLOP/s, 52 % of the measured product
+// head_dim 128, fp16, causal) take 151 us, 912 TFLOP/s, 53 % of the measured product
 // rate; 512 tokens over 32768 slots (12 heads, 2 KV heads, bf16) 101 us, 1.01 PFLOP/s.
 // Tried and not kept: a quarter of the exponentials as polynomials on the FMA pipe
-// (155 us), queries and first tile loaded before the first barrier (162 us).
+// (155 us), queries and first tile loaded before the first barrier (162 us), P handed
+// over as 96 + 32 keys (158 us), two softmax threads a row (166 us).
 #include "paged_tc.cuh"
 
 namespace cuq {

@@ -18,11 +18,12 @@
 // computed.  Many: by the exponentials (16 a cycle and SM); then the query tiles of
 // an item are dealt out over a cluster, whose CTAs' sums are joined in rank order
 // through distributed shared memory.  The last 32 queries of 4 sequences up to 16384
-// slots (32 heads, 8 KV heads, head_dim 128) take 20.5 us, 2.8 TB/s: six items a CTA of
+// slots (32 heads, 8 KV heads, head_dim 128) take 18.4 us, 3.15 TB/s: six items a CTA of
 // 2450 cycles (2048 of them exponentials) and 1200 between two items, after 8700 to
-// the first.  2048 queries over 4096 slots (12 heads, 2 KV heads) take 45 us, 2700
+// the first.  2048 queries over 4096 slots (12 heads, 2 KV heads) take 43 us, 2700
 // cycles a step of 256 slots x 128 rows.  Six of 16 exponential pairs as polynomials on
-// the FMA pipe made it slower (51 us); eight summing warps instead of sixteen, 53 us.
+// the FMA pipe made it slower (51 us); eight summing warps instead of sixteen, 53 us;
+// two items a cluster, one of many queries and one of few, no faster (43 us).
 #include "paged_tc.cuh"
 
 namespace cuq {
