@@ -260,22 +260,11 @@ struct EvictArgs {
     size_t mass_out_stride;
 };
 
-__device__ __forceinline__ uint32_t peer_smem(const void *p, uint32_t rank) {
-    uint32_t at;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
-                 : "=r"(at)
-                 : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
-    return at;
-}
 __device__ __forceinline__ void peer_add(uint32_t at, uint32_t v) {
     asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
 }
 __device__ __forceinline__ void peer_store(uint32_t at, uint32_t v) {
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
-}
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(EvictArgs p) {

@@ -31,6 +31,24 @@ cudaError_t allow_smem(K kernel, int bytes, std::atomic<uint64_t> &done) {
     return e;
 }
 
+// Shared memory of the cluster's CTA `rank`, and the barrier over all of its CTAs.
+__device__ __forceinline__ uint32_t peer_smem(const void *p, uint32_t rank) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+                 : "=r"(at)
+                 : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    return at;
+}
+__device__ __forceinline__ float peer_load(uint32_t at) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 // The cache and the batch as a kernel sees them.  Every length and page id that
 // comes from device memory is cut or checked here, so no kernel reads past a
 // pool, a table or a token tensor whatever the arrays hold.
@@ -186,6 +204,7 @@ struct AttnPlan {
     bool few, many;        // which kernels run
     uint32_t few_ctas;     // of the mma.sync kernel; its warps share the blocks out evenly
     uint32_t few_rows;     // rows of a part
+    uint32_t few_cluster;  // CTAs that take one (sequence, KV head) between them and join its parts; 0: runs and a merge
     uint32_t many_splits;
     uint32_t many_tiles;   // bound of the 256-row tiles of all sequences
     // whether a sequence of `tokens` attended tokens is the mma.sync kernel's

@@ -34,9 +34,13 @@ __device__ int g_timeout;  // a bounded wait of this file's kernels gave up
 // step took 42.4 us and with four 48.6, since queries and page ids then wait behind
 // 28 MB of copies.  With a CTA for each part of 256 to 1024 slots instead of equal runs
 // it took 51 to 67 us.
+// Where all items are short, a cluster of CTAs takes each instead and joins its parts
+// through distributed shared memory: one launch, no workspace (attention_paged_plan has
+// the rule and what both forms measured).
 constexpr int FEW_WARPS = 4, FEW_ST = 2, FEW_KEYS = 16;
 constexpr uint32_t FEW_RUN = 4;   // blocks a warp takes at least
 constexpr uint32_t FEW_ITEM = 3;  // blocks' worth of an item's own cost
+constexpr uint32_t FEW_NEAR = 8;  // blocks a warp at most where a cluster takes an item
 
 template <int HD>
 struct FewGeo {
@@ -72,7 +76,10 @@ __device__ __forceinline__ uint32_t few_run(uint32_t total, uint32_t kv_heads, u
     return max(FEW_RUN, (uint32_t)(((uint64_t)total * kv_heads + warps - 1) / warps));
 }
 
-template <typename TQ, typename TC, int HD>
+// NEAR: few short items.  A cluster of CTAs takes one item and every warp an equal
+// part of its blocks; the parts stay in shared memory and are joined there, so that
+// the call is one launch.
+template <typename TQ, typename TC, int HD, bool NEAR>
 __global__ void __launch_bounds__(FEW_WARPS * 32, FewGeo<HD>::CTAS)
     attn_few_kernel(PagedArgs a, PagedQuery q, AttnOut o, const __grid_constant__ CUtensorMap mk,
                     const __grid_constant__ CUtensorMap mv) {
@@ -84,14 +91,20 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, FewGeo<HD>::CTAS)
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t full[FEW_WARPS][FEW_ST];
     __shared__ int abort_flag;
+    __shared__ float s_lse[NEAR ? FEW_WARPS : 1][ATTN_FEW];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = warp_index();
+    uint32_t rank = 0, ranks = 1;
+    if constexpr (NEAR) {
+        asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+        asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
+    }
     // alone: wait for what came before.  Behind the many-row kernel, which has waited
     // for it, run beside that one's tail and end after it, for the merge's sake.
-    if (!o.plan.many) griddep_wait();
-    griddep_launch();  // the merge may take its place; it waits for this grid's end
+    if (NEAR || !o.plan.many) griddep_wait();
+    if (!NEAR) griddep_launch();  // the merge may take its place; it waits for this grid's end
     // units of the sequences [0, 32), one a lane, and of all
-    const uint32_t v0 = lane < a.n_seqs ? FewSeq(a, q, o.plan, lane).units() : 0;
+    const uint32_t v0 = !NEAR && lane < a.n_seqs ? FewSeq(a, q, o.plan, lane).units() : 0;
     if (tid == 0) {
         prefetch_map(&mk);
         prefetch_map(&mv);
@@ -100,61 +113,70 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, FewGeo<HD>::CTAS)
             for (int s = 0; s < FEW_ST; s++) mbar_init(&full[w][s], 1);
         mbar_init_fence();
     }
-    uint32_t total = v0;
-    for (uint32_t b = lane + 32; b < a.n_seqs; b += 32) total += FewSeq(a, q, o.plan, b).units();
-    total = __reduce_add_sync(~0u, total);
-    __syncthreads();
     const uint32_t gw = blockIdx.x * FEW_WARPS + warp;
-    if (gw == gridDim.x * FEW_WARPS - 1) {  // the last warp, which has the least to do: the table for the merge
-        uint32_t before = 0;
-        for (uint32_t s0 = 0; s0 < a.n_seqs; s0 += 32) {
-            const uint32_t v = s0 + lane < a.n_seqs ? FewSeq(a, q, o.plan, s0 + lane).units() : 0;
-            uint32_t upto = v;
+    uint32_t b0 = 0, h0 = 0, k0 = 0, left = 0;  // the run's first sequence, KV head and unit, and its units
+    if constexpr (NEAR) {
+        const uint32_t x = blockIdx.x / ranks;
+        b0 = x / a.kv_heads;
+        h0 = x % a.kv_heads;
+        const uint32_t nblk = FewSeq(a, q, o.plan, b0).nblk, warps = ranks * FEW_WARPS, per = (nblk + warps - 1) / warps;
+        k0 = min(nblk, (rank * FEW_WARPS + warp) * per);
+        left = min(per, nblk - k0);
+        if (lane < ATTN_FEW) s_lse[warp][lane] = -INFINITY;
+        __syncthreads();
+    } else {
+        uint32_t total = v0;
+        for (uint32_t b = lane + 32; b < a.n_seqs; b += 32) total += FewSeq(a, q, o.plan, b).units();
+        total = __reduce_add_sync(~0u, total);
+        __syncthreads();
+        if (gw == gridDim.x * FEW_WARPS - 1) {  // the last warp, which has the least to do: the table for the merge
+            uint32_t before = 0;
+            for (uint32_t s0 = 0; s0 < a.n_seqs; s0 += 32) {
+                const uint32_t v = s0 + lane < a.n_seqs ? FewSeq(a, q, o.plan, s0 + lane).units() : 0;
+                uint32_t upto = v;
 #pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const uint32_t up = __shfl_up_sync(~0u, upto, d);
-                if (lane >= (uint32_t)d) upto += up;
+                for (int d = 1; d < 32; d <<= 1) {
+                    const uint32_t up = __shfl_up_sync(~0u, upto, d);
+                    if (lane >= (uint32_t)d) upto += up;
+                }
+                if (s0 + lane < a.n_seqs) o.few_units[s0 + lane] = before + upto - v;
+                before += __shfl_sync(~0u, upto, 31);
             }
-            if (s0 + lane < a.n_seqs) o.few_units[s0 + lane] = before + upto - v;
-            before += __shfl_sync(~0u, upto, 31);
+            if (lane == 0) o.few_units[a.n_seqs] = total;
         }
-        if (lane == 0) o.few_units[a.n_seqs] = total;
-    }
-    const uint32_t run = few_run(total, a.kv_heads, gridDim.x);
-    uint32_t left = 0;  // units of this warp's run
-    {
-        const uint64_t x0 = (uint64_t)gw * run, all = (uint64_t)total * a.kv_heads;
-        left = x0 < all ? (uint32_t)min((uint64_t)run, all - x0) : 0;
-    }
-    if (!left) {
-        if (gw == 0) griddep_wait();
-        return;
-    }
-    // the run's first sequence, KV head and unit
-    uint32_t b0 = 0, h0 = 0, k0 = 0;
-    {
-        uint32_t x = gw * run;
-        for (uint32_t s0 = 0;; s0 += 32) {
-            uint32_t v = v0;
-            if (s0) v = s0 + lane < a.n_seqs ? FewSeq(a, q, o.plan, s0 + lane).units() : 0;
-            v *= a.kv_heads;
-            uint32_t upto = v;
+        const uint32_t run = few_run(total, a.kv_heads, gridDim.x);
+        {
+            const uint64_t x0 = (uint64_t)gw * run, all = (uint64_t)total * a.kv_heads;
+            left = x0 < all ? (uint32_t)min((uint64_t)run, all - x0) : 0;
+        }
+        if (!left) {
+            if (gw == 0) griddep_wait();
+            return;
+        }
+        {
+            uint32_t x = gw * run;
+            for (uint32_t s0 = 0;; s0 += 32) {
+                uint32_t v = v0;
+                if (s0) v = s0 + lane < a.n_seqs ? FewSeq(a, q, o.plan, s0 + lane).units() : 0;
+                v *= a.kv_heads;
+                uint32_t upto = v;
 #pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const uint32_t up = __shfl_up_sync(~0u, upto, d);
-                if (lane >= (uint32_t)d) upto += up;
+                for (int d = 1; d < 32; d <<= 1) {
+                    const uint32_t up = __shfl_up_sync(~0u, upto, d);
+                    if (lane >= (uint32_t)d) upto += up;
+                }
+                const uint32_t hit = __ballot_sync(~0u, x < upto);
+                if (hit) {
+                    const int at = __ffs(hit) - 1;
+                    const uint32_t mine = __shfl_sync(~0u, v, at);
+                    x -= __shfl_sync(~0u, upto, at) - mine;
+                    b0 = s0 + at;
+                    h0 = x / (mine / a.kv_heads);
+                    k0 = x % (mine / a.kv_heads);
+                    break;
+                }
+                x -= __shfl_sync(~0u, upto, 31);
             }
-            const uint32_t hit = __ballot_sync(~0u, x < upto);
-            if (hit) {
-                const int at = __ffs(hit) - 1;
-                const uint32_t mine = __shfl_sync(~0u, v, at);
-                x -= __shfl_sync(~0u, upto, at) - mine;
-                b0 = s0 + at;
-                h0 = x / (mine / a.kv_heads);
-                k0 = x % (mine / a.kv_heads);
-                break;
-            }
-            x -= __shfl_sync(~0u, upto, 31);
         }
     }
 
@@ -358,20 +380,23 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, FewGeo<HD>::CTAS)
             pgs[FEW_ST - 1] = issue();
             if (++st == FEW_ST) st = 0, ph ^= 1;
         }
-        // this warp's part of the item
-        const uint64_t part = (uint64_t)gw + (uint64_t)b * a.kv_heads + kvh;
+        // this warp's part of the item; NEAR: in the place of its stages, whose last block is done with
+        const uint64_t part = NEAR ? 0 : (uint64_t)gw + (uint64_t)b * a.kv_heads + kvh;
+        float *const part_o = NEAR ? reinterpret_cast<float *>(ring) : o.few_o;
+        float *const part_lse = NEAR ? s_lse[NEAR ? warp : 0] : o.few_lse;
+        if (NEAR) __syncwarp();
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             l[h] += __shfl_xor_sync(~0u, l[h], 1);
             l[h] += __shfl_xor_sync(~0u, l[h], 2);
             const uint32_t r = g + 8 * h;
             if (r >= rows) continue;
-            const size_t row = part * o.plan.few_rows + r;
+            const size_t row = NEAR ? r : part * o.plan.few_rows + r;
             const float inv = l[h] == 0.f ? 0.f : 1.f / l[h];  // NaN stays NaN
-            if (t4 == 0) o.few_lse[row] = l[h] == 0.f ? -INFINITY : m[h] - LIFT + log2f(l[h]);
+            if (t4 == 0) part_lse[row] = l[h] == 0.f ? -INFINITY : m[h] - LIFT + log2f(l[h]);
 #pragma unroll
             for (int d = 0; d < HD / 8; d++)
-                *reinterpret_cast<float2 *>(o.few_o + row * HD + d * 8 + t4 * 2) =
+                *reinterpret_cast<float2 *>(part_o + row * HD + d * 8 + t4 * 2) =
                     make_float2(acc[d][2 * h] * inv, acc[d][2 * h + 1] * inv);
         }
         left -= min(left, sq.units() - k);
@@ -381,7 +406,58 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, FewGeo<HD>::CTAS)
             b++;
         }
     }
-    if (gw == 0) griddep_wait();
+    if constexpr (NEAR) {
+        // a warp a row: a part's sum in each lane, then eight parts on their way at once
+        auto sync = [&] {
+            __syncwarp();
+            if (ranks > 1)
+                cluster_sync();
+            else
+                __syncthreads();
+        };
+        sync();
+        const FewSeq sq(a, q, o.plan, b0);
+        constexpr int E = HD / 32;
+        const uint32_t parts = ranks * FEW_WARPS, rows = sq.tq * q.group;
+        for (uint32_t r = rank * FEW_WARPS + warp; r < rows; r += parts) {
+            float ls = -INFINITY;
+            if (lane < parts) ls = peer_load(peer_smem(&s_lse[lane % FEW_WARPS][r], lane / FEW_WARPS));
+            float top = ls;
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+            const float w = ex2(ls - (top == -INFINITY ? 0.f : top));
+            float v[E], total = 0.f;
+#pragma unroll
+            for (int e = 0; e < E; e++) v[e] = 0.f;
+            for (uint32_t p0 = 0; p0 < parts; p0 += FEW_WARPS) {
+                float src[FEW_WARPS][E];
+#pragma unroll
+                for (int i = 0; i < FEW_WARPS; i++)
+#pragma unroll
+                    for (int e = 0; e < E; e++)
+                        src[i][e] = peer_load(peer_smem(smem + i * (FEW_ST * 2 * G::ROWS) + (r * HD + e * 32 + lane) * 4,
+                                                        p0 / FEW_WARPS));
+#pragma unroll
+                for (int i = 0; i < FEW_WARPS; i++) {
+                    const float wi = __shfl_sync(~0u, w, (p0 + i) & 31);
+                    if (wi == 0.f) continue;  // a part that saw nothing may hold anything
+                    total += wi;
+#pragma unroll
+                    for (int e = 0; e < E; e++) v[e] += wi * src[i][e];
+                }
+            }
+            const float inv = total == 0.f ? 0.f : 1.f / total;
+            const uint32_t i = q.div_group(r), tok = sq.first + i, head = h0 * q.group + (r - i * q.group);
+            TQ *dst = reinterpret_cast<TQ *>(o.out) + (size_t)tok * o.out_stride + (size_t)head * HD + lane;
+#pragma unroll
+            for (int e = 0; e < E; e++) dst[e * 32] = (TQ)(v[e] * inv);
+            if (o.lse && lane == 0)
+                o.lse[(size_t)tok * q.heads + head] = total == 0.f ? -INFINITY : (top + log2f(total)) * 0.6931471805599453f;
+        }
+        sync();  // the others may still read this CTA's parts
+    } else if (gw == 0) {
+        griddep_wait();
+    }
     if (!ok) {  // let the copies in flight land before this block's memory is given back
         if (lane == 0) g_timeout = 1;
         const unsigned long long t0 = now_ns();
@@ -479,12 +555,30 @@ int launch_few(const AttnPagedCall &c, const AttnOut &o, cudaStream_t s) {
     int rc = make_page_map(&mk, c.a.k, c.a, HD, c.cache_type, FEW_KEYS, HD / 64);
     if (rc == CUQ_OK) rc = make_page_map(&mv, c.a.v, c.a, HD, c.cache_type, FEW_KEYS, HD / 64);
     if (rc) return rc;
-    auto kern = attn_few_kernel<TQ, TC, HD>;
-    static std::atomic<uint64_t> allowed;
-    CUQ_CUDA_TRY(allow_smem(kern, FewGeo<HD>::SMEM, allowed));
-    CUQ_CUDA_TRY(launch_maybe_pdl(kern, dim3(o.plan.few_ctas), dim3(FEW_WARPS * 32), FewGeo<HD>::SMEM, s, true, c.a,
-                                  c.q, o, mk, mv));
-    return CUQ_OK;
+    auto launch = [&](auto kern, uint32_t ctas, uint32_t cluster, std::atomic<uint64_t> &allowed) -> int {
+        CUQ_CUDA_TRY(allow_smem(kern, FewGeo<HD>::SMEM, allowed));
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(ctas);
+        cfg.blockDim = dim3(FEW_WARPS * 32);
+        cfg.dynamicSmemBytes = FewGeo<HD>::SMEM;
+        cfg.stream = s;
+        cudaLaunchAttribute attrs[2];
+        attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attrs[0].val.programmaticStreamSerializationAllowed = 1;
+        attrs[1].id = cudaLaunchAttributeClusterDimension;
+        attrs[1].val.clusterDim.x = cluster;
+        attrs[1].val.clusterDim.y = attrs[1].val.clusterDim.z = 1;
+        cfg.attrs = attrs;
+        cfg.numAttrs = cluster ? 2 : 1;
+        CUQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, c.a, c.q, o, mk, mv));
+        return CUQ_OK;
+    };
+    static std::atomic<uint64_t> allowed, allowed_near;
+    const AttnPlan &p = o.plan;
+    if (p.few_cluster)
+        return launch(attn_few_kernel<TQ, TC, HD, true>, c.a.n_seqs * c.a.kv_heads * p.few_cluster, p.few_cluster,
+                      allowed_near);
+    return launch(attn_few_kernel<TQ, TC, HD, false>, p.few_ctas, 0, allowed);
 }
 
 template <typename TQ, typename TC>
@@ -493,7 +587,7 @@ int launch_all(const AttnPagedCall &c, const AttnOut &o, cudaStream_t s) {
     if (o.plan.many) rc = launch_attention_many(c, o, s);
     if (rc == CUQ_OK && o.plan.few)
         rc = c.hd == 64 ? launch_few<TQ, TC, 64>(c, o, s) : launch_few<TQ, TC, 128>(c, o, s);
-    if (rc || (!o.plan.few && o.plan.many_splits == 1)) return rc;
+    if (rc || o.plan.few_cluster || (!o.plan.few && o.plan.many_splits == 1)) return rc;
     const uint64_t rows = (uint64_t)c.a.n_tok * c.q.heads;
     const dim3 grid((unsigned)((rows + MERGE_WARPS - 1) / MERGE_WARPS)), block(MERGE_WARPS * 32);
     const cudaError_t e =
@@ -554,6 +648,19 @@ AttnPlan attention_paged_plan(const AttnPagedCall &c, int sm_count) {
         const uint64_t want = (blocks + FEW_RUN * FEW_WARPS - 1) / (FEW_RUN * FEW_WARPS);
         p.few_ctas = (uint32_t)(want < 1 ? 1 : want < most ? want : most);
         p.few_rows = max_rows < ATTN_FEW ? (uint32_t)max_rows : ATTN_FEW;
+        const uint64_t items = (uint64_t)c.a.n_seqs * c.a.kv_heads;
+        if (!p.many && items <= most) {
+            // As few blocks a warp as 8 CTAs an item, all of the call's at once on the GPU, come
+            // to, in as few CTAs; up to FEW_NEAR.  One token over 40, 600, 2000, 4000 and 8000
+            // slots (9 heads, 3 KV heads, head_dim 64, fp32, in a graph) takes 4.1, 6.6, 8.6, 12.1
+            // and 19.1 us this way, 7.9, 8.6, 10.0, 13.2 and 16.5 with runs and the merge; 16
+            // over 600 (32 heads, 8 KV heads, head_dim 128, bf16) 9.9 instead of 12.3.
+            uint64_t seen = c.a.max_kv;
+            if (c.q.window && c.q.window + (uint64_t)c.a.max_q < seen) seen = c.q.window + (uint64_t)c.a.max_q;
+            const uint64_t longest = seen / FEW_KEYS + 1, warps = (most / items < 8 ? most / items : 8) * FEW_WARPS;
+            const uint64_t each = (longest + warps - 1) / warps;
+            if (each <= FEW_NEAR) p.few_cluster = (uint32_t)((longest + each * FEW_WARPS - 1) / (each * FEW_WARPS));
+        }
     }
     if (p.many) {
         p.many_tiles = (uint32_t)((c.a.n_tok * g + 255) / 256 + c.a.n_seqs);
@@ -569,13 +676,13 @@ AttnPlan attention_paged_plan(const AttnPagedCall &c, int sm_count) {
 namespace {
 // floats of the few's outputs, the many's outputs, the few's sums, the many's sums, and the few's table
 void part_sizes(const AttnPagedCall &c, const AttnPlan &p, size_t (&n)[5]) {
-    const size_t few = p.few ? ((size_t)p.few_ctas * FEW_WARPS + (size_t)c.a.n_seqs * c.a.kv_heads) * p.few_rows : 0;
+    const size_t few = p.few && !p.few_cluster ? ((size_t)p.few_ctas * FEW_WARPS + (size_t)c.a.n_seqs * c.a.kv_heads) * p.few_rows : 0;
     const size_t many = p.many_splits > 1 ? (size_t)p.many_splits * c.a.n_tok * c.q.heads : 0;
     n[0] = few * c.hd;
     n[1] = many * c.hd;
     n[2] = few;
     n[3] = many;
-    n[4] = p.few ? (size_t)c.a.n_seqs + 1 : 0;
+    n[4] = p.few && !p.few_cluster ? (size_t)c.a.n_seqs + 1 : 0;
 }
 }  // namespace
 

@@ -89,6 +89,62 @@ def test_single_tokens_of_every_length(geo, pair):
     run_attention(TOKENS, *geo, pair)
 
 
+def workspace_of(seqs, heads, kv_heads, hd, pair):
+    b = pu.Batch(seqs, kv_heads, hd, pair[1])
+    return lib().cuq_attention_paged_workspace(b.kvp, b.bp, heads, pu.GGML[pair[0]])
+
+
+@pytest.mark.parametrize("geo", GEOS)
+@pytest.mark.parametrize("pair", PAIRS)
+@pytest.mark.parametrize("n", [1, 16, 40, 200, 609, 1100, 2000, 4000])
+def test_one_token_of_one_sequence(n, pair, geo):
+    """Short caches: a cluster of 1 to 8 CTAs joins its own parts, without a workspace (up to 16 heads a KV head)."""
+    assert workspace_of([(1, n)], *geo, pair) == 0 or geo[0] // geo[1] > 16
+    run_attention([(1, n)], *geo, pair, seed=n)
+
+
+@pytest.mark.parametrize("geo", GEOS)
+@pytest.mark.parametrize("pair", PAIRS)
+def test_short_caches(geo, pair):
+    """Ragged ones, an empty cache, a sequence without tokens, rows behind the last sequence."""
+    seqs = [(1, 1), (1, 17), (0, 40), (1, 129), (1, 0), (1, 33), (1, 480), (1, 16), (1, 255), (0, 0), (1, 500)]
+    assert workspace_of(seqs, *geo, pair) == 0 or geo[0] // geo[1] > 16
+    run_attention(seqs, *geo, pair, tail=3, q_pad=8, out_pad=16, page_pad=64, seed=11)
+
+
+@pytest.mark.parametrize("geo", [(8, 8, 64), (4, 1, 128), (14, 2, 64)])
+@pytest.mark.parametrize("pair", PAIRS)
+@pytest.mark.parametrize("window", [0, 1, 40, 300])
+def test_short_drafts(window, pair, geo):
+    """As many tokens as one tile of 16 rows holds, through windows, holes and a mask that is not causal."""
+    q = 16 * geo[1] // geo[0]
+    seqs = [(q, 900), (1, 333), (q, q), (q, max(0, q - 2)), (q, 64)]
+    assert workspace_of(seqs, *geo, pair) == 0
+    holes = [(0, 0), (0, 3), (0, 55), (0, 56), (1, 20), (4, 0), (4, 1), (4, 2), (4, 3)]
+    run_attention(seqs, *geo, pair, window=window, holes=holes, seed=window + 13)
+    if not window:
+        run_attention(seqs, *geo, pair, causal=False, holes=holes, seed=17)
+
+
+@pytest.mark.parametrize("geo", [(9, 3, 64), (32, 8, 128)])
+@pytest.mark.parametrize("pair", PAIRS)
+def test_short_and_long_bounds_agree(geo, pair):
+    """The same caches under a bound that asks for runs and the merge: equal within both paths' roundings."""
+    heads, kv_heads, hd = geo
+    t, cache = pair
+    b = pu.Batch([(1, 700), (1, 20), (1, 413)], kv_heads, hd, cache, seed=23)
+    q, row, qh = queries(b, heads, t, 24)
+    near = attend(b, heads, t, q, row, hd ** -0.5)
+    check_attention(b, heads, t, *near, qh, hd ** -0.5)
+    wide = torch.full((3, 1024), -1, dtype=torch.int32)
+    wide[:, : b.table.shape[1]] = b.table
+    b.d_wide = wide.cuda()
+    b.desc.pages, b.desc.pages_stride, b.desc.max_kv = b.d_wide.data_ptr(), 1024, 16384
+    assert lib().cuq_attention_paged_workspace(b.kvp, b.bp, heads, pu.GGML[t]) > 0
+    far = attend(b, heads, t, q, row, hd ** -0.5)
+    check_attention(b, heads, t, *far, qh, hd ** -0.5)
+
+
 @pytest.mark.parametrize("pair", PAIRS)
 @pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
 def test_page_sizes(page, pair):
