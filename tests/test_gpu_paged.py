@@ -720,6 +720,44 @@ def test_graph_replay_follows_the_arrays():
             assert abs(float(mass[i, :, :n].sum()) - (heads if n else 0)) < 2.0 ** -10 * heads
 
 
+@pytest.mark.parametrize("slots", [512, 16384])
+@pytest.mark.parametrize("pair", PAIRS)
+def test_graph_replay_of_single_tokens(pair, slots):
+    """A captured decode step under a bound of few and of many slots (one launch, or runs and the merge), lengths changing."""
+    t, cache = pair
+    L, heads, hd = lib(), 9, 64
+    b = pu.Batch([(1, 40), (1, 500), (1, 7), (1, 129)], 3, hd, cache, 16, seed=41, tail=1)
+    wide = torch.full((4, slots // 16), -1, dtype=torch.int32)
+    wide[:, : b.table.shape[1]] = b.table
+    d_wide = wide.cuda()
+    b.desc.pages, b.desc.pages_stride, b.desc.max_kv = d_wide.data_ptr(), slots // 16, slots
+    need = L.cuq_attention_paged_workspace(b.kvp, b.bp, heads, pu.GGML[t])
+    assert (need == 0) == (slots == 512)
+    ws = torch.full((max(1, need),), 255, dtype=torch.uint8, device="cuda")
+    q, row, qh = queries(b, heads, t, 42)
+    out = torch.full((b.n_tok, heads * hd), 7.0, dtype=pu.DT[t], device="cuda")
+    lse = torch.full((b.n_tok, heads), 7.0, device="cuda")
+
+    def call(s):
+        rt.check(L.cuq_attention_paged(b.kvp, b.bp, ptr(out), heads * hd, ptr(q), row, pu.GGML[t], ptr(lse), heads, 0.125, 1,
+                                       0, ptr(ws) if need else None, need, s))
+
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    call(stream.cuda_stream)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        for _ in range(3):
+            call(torch.cuda.current_stream().cuda_stream)
+    for lens in ([40, 500, 7, 129], [1, 2, 0, 16], [33, 17, 7, 1], [0, 0, 0, 0]):
+        b.d_len.copy_(torch.tensor(lens, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        b.seqs = [(1, n) for n in lens]
+        check_attention(b, heads, t, out, lse, qh, 0.125)
+
+
 def test_two_calls_at_once():
     """Two batches on two streams with a workspace each."""
     bs = [pu.Batch([(1, 3000 + 500 * i), (200, 700)], 2, 128, "f16", 64, seed=i) for i in range(2)]
