@@ -233,14 +233,14 @@ int launch_rope_append(const RopeArgs &p, const RopeTable &t, int out_type, int 
 // Selection, bound by latency: a cluster of CTAs takes one (sequence, KV head),
 // each a contiguous slice of its slots.  Masses become 32-bit keys in their order
 // (NaN lowest), eight a thread, kept in registers where the slice fits.
-// Three histogram passes (11, 11, 10 bits) find the key of the last slot kept and how
-// many of its equals are kept: every CTA counts its own slice, adds the bins it hit
+// Up to three histogram passes (11, 11, 10 bits) find the key of the last slot kept and
+// how many of its equals are kept, and end at a bin that is kept whole: every CTA counts its own slice, adds the bins it hit
 // into every CTA's sums through distributed shared memory, and works the digit out
 // for itself.  Then the slices' counts are exchanged and the kept slots written at
 // their prefix sums.  Histogram atomics count whole numbers, so their order does not
-// matter.  Five cluster barriers in all; with rank 0 finding the digits it was ten.
-// 4096 slots take one CTA 9 us, 32768 a cluster of eight 13 us, mostly barriers and
-// latencies.
+// matter.  At most five cluster barriers; with rank 0 finding the digits it was ten.
+// 4096 slots take one CTA about 8.5 us, 32768 a cluster of eight 12 us, mostly barriers
+// and latencies; always in three passes it was 9 and 13.
 constexpr int SEL_THREADS = 512, SEL_BINS = 2048, SEL_PER = 8;
 constexpr uint32_t SEL_TILE = SEL_THREADS * SEL_PER;
 
@@ -270,7 +270,7 @@ __device__ __forceinline__ void peer_store(uint32_t at, uint32_t v) {
 __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(EvictArgs p) {
     __shared__ __align__(16) uint32_t hist[SEL_BINS];     // this slice's counts
     __shared__ __align__(16) uint32_t sums[3][SEL_BINS];  // the cluster's, one set a pass
-    __shared__ uint32_t s_digit, s_need, s_above[8], s_equal[8], warp_a[SEL_THREADS / 32];
+    __shared__ uint32_t s_digit, s_need, s_whole, s_above[8], s_equal[8], warp_a[SEL_THREADS / 32];
     __shared__ uint2 s_run[SEL_PER * SEL_THREADS / 32];  // kept for sure and equal, by warps of slots
     uint32_t rank, ranks;
     griddep_wait();
@@ -309,6 +309,7 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(EvictArgs p) 
     for (uint32_t i = tid; i < SEL_BINS; i += SEL_THREADS) hist[i] = sums[0][i] = sums[1][i] = sums[2][i] = 0;
     sync();  // the sums are clear everywhere
     uint32_t need = p.keep - p.sink - p.recent, prefix = 0;
+    uint32_t edge = 0xFFFFFFFFu;  // no float has this key: nothing in between is kept
     constexpr int SHIFT[3] = {21, 10, 0}, BITS[3] = {11, 11, 10};
 #pragma unroll 1
     for (int pass = 0; pass < 3; pass++) {
@@ -361,16 +362,20 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(EvictArgs p) 
             if (above < need && above + down[e] >= need) {  // one thread only (need > 0)
                 s_digit = (uint32_t)(bin0 + PER - 1 - e);
                 s_need = need - above;
+                s_whole = above + down[e] == need;
             }
             above += down[e];
         }
         __syncthreads();
-        prefix = (prefix << bits) | s_digit;
+        edge = prefix = (prefix << bits) | s_digit;
         need = s_need;
+        if (s_whole) {  // the bin is kept to its last key; it is not the lowest, since some slot goes
+            edge = (prefix << shift) - 1;
+            need = 0;
+            break;
+        }
     }
-    // kept: keys above `prefix`, and the first `need` equal to it.  The key 2^32 - 1
-    // stands for "none" when nothing in between is kept (no float has it).
-    const uint32_t edge = need == 0 ? 0xFFFFFFFFu : prefix;
+    // kept: keys above `edge`, and the first `need` equal to it
     // a tile's slots that are kept for sure and those equal to the edge, a bit a slot
     // (this thread's), and the counts of them before each 32 slots of the tile (s_run)
     auto kinds = [&](uint32_t t0, uint32_t &above, uint32_t &equal, uint32_t &na, uint32_t &ne) {

@@ -589,6 +589,25 @@ def test_evict_ties_and_odd_masses():
         run_evict([n], 4, 64, "f16", 16, keep, 1, 0, mass=m.clone(), place="in")
 
 
+@pytest.mark.parametrize("n", [700, 9000])
+@pytest.mark.parametrize("place", ["in", "out"])
+def test_evict_edges_between_bits(place, n):
+    """Groups of equal masses that differ from bit 27, 20, 9 or 0 on, kept to a group's last member, one short of it
+    and one past it."""
+    m = torch.zeros(1, 4, n, dtype=torch.int32)
+    group = torch.randint(0, 5, (4, n), generator=torch.Generator().manual_seed(7))
+    for h, bit in enumerate((27, 20, 9, 0)):
+        m[0, h] = 0x20000000 + (group[h] << bit).int()
+    m = m.view(torch.float32)
+    m[0, 3, ::2] *= -1
+    for top in (1, 2, 4):
+        edge = int((group[0] >= top).sum())
+        for keep in (edge - 1, edge, edge + 1):
+            run_evict([n], 4, 64, "bf16", 32, keep, 0, 0, mass=m.clone(), place=place)
+    for h in range(4):  # the boundary right behind each head's own groups
+        run_evict([n], 4, 64, "bf16", 32, int((group[h] >= 3).sum()), 0, 0, mass=m.clone(), place=place)
+
+
 def test_evict_holes_stay_out_of_it():
     run_evict([300, 200], 2, 64, "f16", 16, 100, 4, 16, holes=[(0, 3), (0, 9), (1, 0)])
 
