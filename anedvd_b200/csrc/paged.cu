@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_append_kernel(RopeArgs p, R
     }
     if (warp < T) {
         const int tok = (int)(tok0 + warp);
-        const int given = p.positions && tok < (int)p.a.n_tok ? __ldg(p.positions + tok) : 0;
+        const int given = p.positions && tok < (int)p.a.n_tok ? p.positions[tok] : 0;
         const uint32_t n = p.a.sequence_of(tok);
         if (lane == 0) {
             int seq = -1, slot = -1, page = -1;
@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(EvictArgs p) 
 #pragma unroll
         for (int e = 0; e < SEL_PER; e++) {
             const uint32_t i = t0 + e * SEL_THREADS + tid;
-            key[e] = i < i1 ? mass_key(__ldg(mass + i)) : 0u;
+            key[e] = i < i1 ? mass_key(mass[i]) : 0u;
         }
     };
     if (resident) load(i0);
@@ -525,7 +525,7 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(EvictArgs p) {
         const uint32_t j = c + rank * MOVE_ROWS + threadIdx.x;
         from_next = to_next = -1;
         if (threadIdx.x >= MOVE_ROWS || j >= p.keep) return;
-        const uint32_t src = (uint32_t)__ldg(kept + j);
+        const uint32_t src = (uint32_t)kept[j];
         if (src == j || src >= n) return;
         to_next = place(j);
         from_next = to_next < 0 ? -1 : place(src);

@@ -13,7 +13,10 @@ namespace cuq {
 // Every kernel of these ops is launched as a programmatic dependent of what the
 // stream holds before it, and waits (griddepcontrol.wait) before it reads anything
 // that may come from there: the order is the stream's, and a launch costs 1 to 2 us
-// less than one that waits for the stream to run dry.
+// less than one that waits for the stream to run dry.  A kernel may thus be resident
+// while its inputs are still written (the selection's list and the move that reads it),
+// so all of them are read by plain loads: the read-only path (ld.global.nc) asks for
+// data that does not change while the kernel lives.
 
 // SM count of the current device, asked for once per device.
 int paged_sm_count();
@@ -60,12 +63,12 @@ struct PagedArgs {
     uint32_t n_seqs, n_tok, pages_stride, max_q, max_kv;  // max_kv: already cut to the table's slots
 
     __device__ __forceinline__ uint32_t len(uint32_t b) const {
-        const int n = __ldg(kv_len + b);
+        const int n = kv_len[b];
         return n <= 0 ? 0u : min((uint32_t)n, max_kv);
     }
     // first token row of sequence b and its token count (at most n_tok rows in all)
     __device__ __forceinline__ uint32_t tokens(uint32_t b, uint32_t &first) const {
-        const int a = __ldg(q_start + b), e = __ldg(q_start + b + 1);
+        const int a = q_start[b], e = q_start[b + 1];
         first = a <= 0 ? 0u : min((uint32_t)a, n_tok);
         const uint32_t end = e <= 0 ? 0u : min((uint32_t)e, n_tok);
         return end > first ? end - first : 0u;
@@ -77,13 +80,13 @@ struct PagedArgs {
         uint32_t lo = 0, size = n_seqs;
         while (size) {
             const uint32_t step = (size + 31) / 32, end = lo + size, last = lo + (lane + 1) * step - 1;
-            lo += step * __popc(__ballot_sync(~0u, last < end && __ldg(q_start + last + 1) <= tok));
+            lo += step * __popc(__ballot_sync(~0u, last < end && q_start[last + 1] <= tok));
             size = lo < end ? min(step - 1, end - lo) : 0;
         }
         return min(lo, n_seqs);
     }
     __device__ __forceinline__ int page(uint32_t b, uint32_t col) const {
-        const int id = __ldg(pages + (size_t)b * pages_stride + col);
+        const int id = pages[(size_t)b * pages_stride + col];
         return (id >= 0 && (uint32_t)id < n_pages) ? id : -1;
     }
     // element offset of row `slot` of KV head h inside a pool; the page id is valid
@@ -164,7 +167,7 @@ template <typename T>
 __device__ __forceinline__ void load8(const T *p, float (&v)[8]) {
     uint4 u[sizeof(T) == 4 ? 2 : 1];
 #pragma unroll
-    for (int w = 0; w < (sizeof(T) == 4 ? 2 : 1); w++) u[w] = __ldg(reinterpret_cast<const uint4 *>(p) + w);
+    for (int w = 0; w < (sizeof(T) == 4 ? 2 : 1); w++) u[w] = reinterpret_cast<const uint4 *>(p)[w];
     unpack8<T>(u, v);
 }
 template <typename T>

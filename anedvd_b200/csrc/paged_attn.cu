@@ -189,9 +189,9 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, FewGeo<HD>::CTAS)
     int ids = 0;
     auto look = [&]() {
         ids_at = lk;
-        ids = lk + lane < ls.nblk ? __ldg(a.pages + (size_t)lb * a.pages_stride +
-                                          (((ls.blk0 + lk + lane) * FEW_KEYS) >> a.page_shift))
-                                  : -1;
+        ids = lk + lane < ls.nblk
+                  ? a.pages[(size_t)lb * a.pages_stride + (((ls.blk0 + lk + lane) * FEW_KEYS) >> a.page_shift)]
+                  : -1;
     };
     if (lk < ls.nblk) look();  // on its way while the queries are loaded
     auto issue = [&]() -> int {  // the next block into its stage; its page, or -1
@@ -265,11 +265,11 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, FewGeo<HD>::CTAS)
 #pragma unroll
                 for (int e = 0; e < 2; e++) {  // dims 2 t4, 2 t4 + 1 and those 8 on
                     if constexpr (SPLIT) {
-                        const float2 f = src ? __ldg(reinterpret_cast<const float2 *>(src + ks * 16 + e * 8))
+                        const float2 f = src ? *reinterpret_cast<const float2 *>(src + ks * 16 + e * 8)
                                              : make_float2(0.f, 0.f);
                         split_pack<TC>(f.x, f.y, qf[ks][2 * e + h], ql[ks][2 * e + h]);
                     } else {
-                        qf[ks][2 * e + h] = src ? __ldg(reinterpret_cast<const uint32_t *>(src + ks * 16 + e * 8)) : 0u;
+                        qf[ks][2 * e + h] = src ? *reinterpret_cast<const uint32_t *>(src + ks * 16 + e * 8) : 0u;
                     }
                 }
         }

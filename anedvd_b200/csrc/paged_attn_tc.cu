@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(NT, 1) attn_many_kernel(PagedArgs a, PagedQuer
                     const bool in = s * 128 + r < my_rows;
                     const uint4 *src = reinterpret_cast<const uint4 *>(qb + (size_t)tok * q.q_stride + head * HD + c * 8);
 #pragma unroll
-                    for (int w = 0; w < W; w++) raw[e][w] = in ? __ldg(src + w) : make_uint4(0, 0, 0, 0);
+                    for (int w = 0; w < W; w++) raw[e][w] = in ? src[w] : make_uint4(0, 0, 0, 0);
                 }
 #pragma unroll
                 for (int e = 0; e < BATCH; e++) {

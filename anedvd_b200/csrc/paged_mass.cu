@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
                 if (t128 < nr) {
                     const uint32_t tok = t.first + (r0 + t128) / q.group;
                     const uint32_t head = t.h * q.group + (r0 + t128) % q.group;
-                    ls = __ldg(p.lse + (size_t)tok * q.heads + head);
+                    ls = p.lse[(size_t)tok * q.heads + head];
                     src = reinterpret_cast<const TQ *>(q.q) + (size_t)tok * q.q_stride + (size_t)head * HD;
                 }
                 constexpr int CH = HD / 8, BATCH = 4;
@@ -358,8 +358,8 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
                             const uint32_t r = r1 + (part * BATCH + k) * (128 / CH);
                             const TQ *row = reinterpret_cast<const TQ *>(s_row[qx & 1][r]);
                             const uint4 *from = reinterpret_cast<const uint4 *>(row + c * 8);
-                            raw[k][0] = row ? __ldg(from) : make_uint4(0, 0, 0, 0);
-                            raw[k][1] = row ? __ldg(from + 1) : make_uint4(0, 0, 0, 0);
+                            raw[k][0] = row ? *from : make_uint4(0, 0, 0, 0);
+                            raw[k][1] = row ? from[1] : make_uint4(0, 0, 0, 0);
                         }
 #pragma unroll
                         for (int k = 0; k < BATCH; k++) {
@@ -417,7 +417,7 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
             float old = 0.f, sum = 0.f;
             int page_id = -1;  // looked at when the sums are there
             if (half == 0 && k < t.n) {
-                page_id = __ldg(a.pages + (size_t)t.b * a.pages_stride + (k >> a.page_shift));
+                page_id = a.pages[(size_t)t.b * a.pages_stride + (k >> a.page_shift)];
                 if (ranks == 1 && p.decay != 0.f) old = p.decay * *m;
             }
             for (uint32_t e = 0; e < t.steps; e++, st++) {
