@@ -480,10 +480,10 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(EvictArgs p) {
     const uint32_t part = x % 3;  // K, V, mass
     x /= 3;
     const uint32_t h = x % p.a.kv_heads, b = x / p.a.kv_heads;
+    griddep_wait();
     const uint32_t n = p.a.len(b);
     const int32_t *kept = p.kept + ((size_t)b * p.a.kv_heads + h) * p.keep;
     if (part == 2) {
-        griddep_wait();
         if (!p.mass_out) return;
         const float *src = p.mass + ((size_t)b * p.a.kv_heads + h) * p.mass_stride;
         float *dst = p.mass_out + ((size_t)b * p.a.kv_heads + h) * p.mass_out_stride;
@@ -509,16 +509,12 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(EvictArgs p) {
         for (uint32_t i = live + rank * MOVE_THREADS + threadIdx.x; i < n; i += ranks * MOVE_THREADS) dst[i] = 0.f;
         return;
     }
-    if (n <= p.keep) {  // every slot stays where it is: the same for the whole cluster
-        griddep_wait();  // every CTA waits, so this grid ends after the selection
-        return;
-    }
+    if (n <= p.keep) return;  // every slot stays where it is: the same for the whole cluster
     uint8_t *pool = reinterpret_cast<uint8_t *>(part ? p.a.v : p.a.k);
     auto place = [&](uint32_t slot) -> int64_t {  // offset of its row, below 0 on a hole
         const int pg = p.a.page(b, slot >> p.a.page_shift);
         return pg < 0 ? -1 : (int64_t)(p.a.row<HD>(pg, h, slot) * 2);
     };
-    griddep_wait();  // what is above reads the batch alone
     const uint32_t r0 = threadIdx.x / LANES, off = (threadIdx.x % LANES) * 16;
     int64_t from_next, to_next;  // this thread's row of the next chunk, looked up while a chunk is read
     auto look = [&](uint32_t c) {

@@ -11,9 +11,13 @@
 namespace cuq {
 
 // Every kernel of these ops is launched as a programmatic dependent of what the
-// stream holds before it, and waits (griddepcontrol.wait) before it reads anything
-// that may come from there: the order is the stream's, and a launch costs 1 to 2 us
-// less than one that waits for the stream to run dry.  A kernel may thus be resident
+// stream holds before it, and waits (griddepcontrol.wait) in every thread before it
+// reads anything that may come from there: the order is the stream's, and a launch
+// costs 1 to 2 us less than one that waits for the stream to run dry.  That an earlier
+// grid has waited is not enough for a later one that it let start: only its own wait
+// makes what was written before visible to it.  (Reading the batch before the wait
+// gained 0.5 us in the merge and 0.3 in the eviction's move, and starting the few-row
+// kernel beside the many-row one 8 us of 31 in a mixed batch.)  A kernel may thus be resident
 // while its inputs are still written (the selection's list and the move that reads it),
 // so all of them are read by plain loads: the read-only path (ld.global.nc) asks for
 // data that does not change while the kernel lives.

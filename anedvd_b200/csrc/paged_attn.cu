@@ -99,9 +99,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, FewGeo<HD>::CTAS)
         asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
         asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
     }
-    // alone: wait for what came before.  Behind the many-row kernel, which has waited
-    // for it, run beside that one's tail and end after it, for the merge's sake.
-    if (NEAR || !o.plan.many) griddep_wait();
+    griddep_wait();
     if (!NEAR) griddep_launch();  // the merge may take its place; it waits for this grid's end
     // units of the sequences [0, 32), one a lane, and of all
     const uint32_t v0 = !NEAR && lane < a.n_seqs ? FewSeq(a, q, o.plan, lane).units() : 0;
@@ -149,10 +147,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, FewGeo<HD>::CTAS)
             const uint64_t x0 = (uint64_t)gw * run, all = (uint64_t)total * a.kv_heads;
             left = x0 < all ? (uint32_t)min((uint64_t)run, all - x0) : 0;
         }
-        if (!left) {
-            if (gw == 0) griddep_wait();
-            return;
-        }
+        if (!left) return;
         {
             uint32_t x = gw * run;
             for (uint32_t s0 = 0;; s0 += 32) {
@@ -455,8 +450,6 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, FewGeo<HD>::CTAS)
                 o.lse[(size_t)tok * q.heads + head] = total == 0.f ? -INFINITY : (top + log2f(total)) * 0.6931471805599453f;
         }
         sync();  // the others may still read this CTA's parts
-    } else if (gw == 0) {
-        griddep_wait();
     }
     if (!ok) {  // let the copies in flight land before this block's memory is given back
         if (lane == 0) g_timeout = 1;
@@ -479,22 +472,26 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) attn_merge_kernel(PagedArgs 
     constexpr int E = HD / 32;
     const uint32_t lane = threadIdx.x & 31;
     const uint32_t row = blockIdx.x * MERGE_WARPS + (threadIdx.x >> 5);
+    griddep_wait();
     const uint32_t tok = row / q.heads, head = row % q.heads;
     const uint32_t b = tok < a.n_tok ? a.sequence_of((int)tok) : a.n_seqs;
-    uint32_t first = 0, nq = 0;
+    uint32_t first = 0, nq = 0, before = 0, total_units = 0;
+    if (o.plan.few && b < a.n_seqs) {  // on their way beside the batch's
+        before = o.few_units[b];
+        total_units = o.few_units[a.n_seqs];
+    }
     if (b < a.n_seqs) nq = a.tokens(b, first);
     const uint32_t tq = min(nq, a.max_q), i = tok - first;
     const bool few = o.plan.is_few(tq, q.group);
     // a row of no sequence, past max_q, or written by its kernel
     const bool none = b >= a.n_seqs || tok < first || i >= tq || (!few && o.plan.many_splits == 1);
     const FewSeq sq(a, q, o.plan, none ? 0 : b);
-    griddep_wait();  // what is above reads the batch alone; every warp waits, so this grid ends last
     if (none) return;
     uint32_t parts = o.plan.many_splits;
     size_t step = (size_t)a.n_tok * q.heads, at = (size_t)tok * q.heads + head;
     const float *part_o = o.many_o, *part_lse = o.many_lse;
     if (few) {  // the warps whose runs hold blocks of this item
-        const uint32_t before = o.few_units[b], run = few_run(o.few_units[a.n_seqs], a.kv_heads, o.plan.few_ctas);
+        const uint32_t run = few_run(total_units, a.kv_heads, o.plan.few_ctas);
         const uint32_t kvh = head / q.group;
         const uint64_t x0 = (uint64_t)before * a.kv_heads + (uint64_t)kvh * sq.units();
         const uint32_t w0 = (uint32_t)(x0 / run), w1 = (uint32_t)((x0 + sq.nblk + run - 1) / run);

@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(NT, 1) attn_many_kernel(PagedArgs a, PagedQuer
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = warp_index();
     const uint32_t kvh = blockIdx.x % a.kv_heads, split = blockIdx.y;
     griddep_wait();
-    griddep_launch();  // the few-row kernel and the merge may follow into free SMs; the merge waits for the end
+    griddep_launch();  // the few-row kernel or the merge may follow into free SMs; it waits for this grid's end
 
     // the tile: tiles are counted over the sequences that are this kernel's
     uint32_t b = 0, tile = blockIdx.x / a.kv_heads, ntile = 0;

@@ -1,0 +1,85 @@
+"""The paged-cache ops as a server runs them: captured steps whose batch changes, many items a CTA, and what a wait that
+gives up leaves behind.  Tolerances are those of test_gpu_paged.py unless a test derives its own."""
+import ctypes
+
+import pytest
+import torch
+
+from anedvd_b200 import runtime as rt
+
+from . import paged_util as pu
+from .gpu_util import lib, ptr
+from .test_gpu_paged import PAIRS, check_attention
+
+pytestmark = pytest.mark.gpu
+
+
+class Step:
+    """Append, attention and gathered weight of one batch, with the buffers that a server keeps for them."""
+
+    def __init__(self, b, heads, pair, window=0):
+        t, _ = pair
+        self.b, self.heads, self.t, self.window = b, heads, t, window
+        self.plan = rt.RopePlan(rt.CuqRopeParams(rot_dim=b.hd, theta=1e4))
+        dt, self.cols = pu.DT[t], heads * b.hd
+        self.x = torch.zeros(b.n_tok, (heads + 2 * b.kv_heads) * b.hd, dtype=dt, device="cuda")
+        self.q, self.out = (torch.full((b.n_tok, self.cols), 7.0, dtype=dt, device="cuda") for _ in range(2))
+        self.lse = torch.full((b.n_tok, heads), 7.0, device="cuda")
+        self.mass = torch.zeros(len(b.seqs), b.kv_heads, b.max_kv, device="cuda")
+        self.need = lib().cuq_attention_paged_workspace(b.kvp, b.bp, heads, pu.GGML[t])
+        self.space = torch.full((max(1, self.need),), 255, dtype=torch.uint8, device="cuda")
+
+    def calls(self, stream):
+        b, L, ty, row = self.b, rt.load(), pu.GGML[self.t], self.x.shape[1]
+        k = self.x.data_ptr() + self.cols * self.x.element_size()
+        v = k + b.kv_heads * b.hd * self.x.element_size()
+        rt.check(L.cuq_rope_append(self.plan.handle, b.kvp, b.bp, None, ptr(self.q), self.cols, ty, ptr(self.x), row,
+                                   ctypes.c_void_p(k), ctypes.c_void_p(v), row, ty, self.heads, stream))
+        rt.check(L.cuq_attention_paged(b.kvp, b.bp, ptr(self.out), self.cols, ptr(self.q), self.cols, ty, ptr(self.lse),
+                                       self.heads, 0.1, 1, self.window, ptr(self.space), self.need, stream))
+        rt.check(L.cuq_attention_mass(b.kvp, b.bp, ptr(self.mass), b.max_kv, ptr(self.q), self.cols, ty, ptr(self.lse),
+                                      self.heads, 0.1, 1, self.window, 0, 0.0, stream))
+
+    def check(self):
+        b = self.b
+        b.k_host, b.v_host = b.k.cpu(), b.v.cpu()
+        q = self.q[: b.n_tok].view(b.n_tok, self.heads, b.hd).cpu()
+        # only rows of the batch are the model's: the others keep what an earlier step left there
+        out, lse = self.out.clone(), self.lse.clone()
+        out[b.used:], lse[b.used:] = 7.0, 7.0
+        check_attention(b, self.heads, self.t, out, lse, q, 0.1, window=self.window)
+        for i, (a, n) in enumerate(b.seqs):  # each row's weights sum to one over the live slots
+            want = self.heads * min(a, n)
+            assert abs(float(self.mass[i, :, :n].double().sum()) - want) <= 2.0 ** -10 * max(1, want)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("pair", PAIRS)
+def test_captured_mixed_steps_follow_the_batch(pair, hd):
+    """Chunks beside single tokens in one captured graph (both attention kernels and the merge): which sequence has the
+    chunk, the lengths, the queries and the cached rows all change between replays, three steps behind one another."""
+    b = pu.Batch([(48, 200), (48, 300), (48, 48), (48, 90)], 2, hd, pair[1], 16, seed=3, tail=0)
+    b.n_tok = b.desc.n_tok = 64
+    step = Step(b, 8, pair)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    step.calls(stream.cuda_stream)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        for _ in range(3):  # the later steps write the same rows again
+            step.calls(torch.cuda.current_stream().cuda_stream)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    for seqs in ([(40, 150), (1, 300), (1, 20), (1, 90)], [(1, 151), (48, 300), (1, 21), (2, 90)],
+                 [(2, 150), (0, 300), (48, 48), (1, 1)], [(1, 200), (1, 299), (1, 48), (1, 89)],
+                 [(10, 150), (10, 30), (30, 48), (3, 2)], [(0, 200), (1, 7), (0, 0), (0, 1)]):
+        b.seqs, b.starts = seqs, [0]
+        for a, _ in seqs:
+            b.starts.append(b.starts[-1] + a)
+        b.used = b.starts[-1]
+        b.d_start.copy_(torch.tensor(b.starts, dtype=torch.int32))
+        b.d_len.copy_(torch.tensor([n for _, n in seqs], dtype=torch.int32))
+        step.x.normal_(generator=g)
+        graph.replay()
+        torch.cuda.synchronize()
+        step.check()
