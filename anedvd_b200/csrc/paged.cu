@@ -3,8 +3,11 @@
 // over the cache is in paged_attn.cu, the gathered attention weight in
 // paged_mass.cu.
 #include <cmath>
+#include <map>
+#include <mutex>
 #include <new>
 #include <type_traits>
+#include <utility>
 
 #include "paged.cuh"
 
@@ -692,6 +695,23 @@ int check_query(const char *who, const cuq_paged_kv *kv, uint32_t n_tok, const v
     return CUQ_OK;
 }
 
+// Whether a caller that polls this stream has not been told of all `count` give-ups of
+// the device; it has been then.  False when out of memory.
+bool told_of_give_ups(int dev, cudaStream_t s, unsigned int count, bool &news) {
+    static std::mutex mu;
+    static std::map<std::pair<int, cudaStream_t>, unsigned int> told;  // none: 0
+    std::lock_guard<std::mutex> lock(mu);
+    try {
+        unsigned int &last = told[{dev, s}];
+        if (count < last) last = 0;  // the device was reset
+        news = count != last;
+        last = count;
+    } catch (const std::bad_alloc &) {
+        return false;
+    }
+    return true;
+}
+
 }  // namespace
 }  // namespace cuq
 
@@ -896,16 +916,28 @@ int cuq_kv_evict(const cuq_paged_kv *kv, const cuq_batch *batch, const float *ma
 }
 
 int cuq_paged_status(void *stream) {
-    CUQ_CUDA_TRY(cudaStreamSynchronize((cudaStream_t)stream));
-    int few = 0, many = 0, mass = 0;
-    int rc = attention_few_status((cudaStream_t)stream, &few);
-    if (rc == CUQ_OK) rc = attention_many_status((cudaStream_t)stream, &many);
-    if (rc == CUQ_OK) rc = attention_mass_status((cudaStream_t)stream, &mass);
-    if (rc == CUQ_OK && (few || many || mass)) {
-        set_error("a wait inside a paged-cache kernel gave up");
-        rc = CUQ_ETIMEOUT;
+    const cudaStream_t s = (cudaStream_t)stream;
+    int dev = 0;
+    CUQ_CUDA_TRY(cudaGetDevice(&dev));
+    CUQ_CUDA_TRY(cudaStreamSynchronize(s));
+    unsigned int few = 0, many = 0, mass = 0;
+    int rc = attention_few_gave_up(s, &few);
+    if (rc == CUQ_OK) rc = attention_many_gave_up(s, &many);
+    if (rc == CUQ_OK) rc = attention_mass_gave_up(s, &mass);
+    if (rc) return rc;
+    bool news = false;
+    if (!told_of_give_ups(dev, s, few + many + mass, news)) {
+        set_error("cuq_paged_status: out of memory");
+        return CUQ_ENOMEM;
     }
-    return rc;
+    if (!news) return CUQ_OK;
+    set_error("a wait inside a paged-cache kernel gave up");
+    return CUQ_ETIMEOUT;
+}
+
+int cuq_paged_wait_probe(uint32_t limit_us, void *stream) {
+    CUQ_CHECK_ARG(limit_us > 0 && limit_us <= 1000000u, "cuq_paged_wait_probe: limit of %u us (1 to 1000000)", limit_us);
+    return launch_wait_probe(limit_us, (cudaStream_t)stream);
 }
 
 }  // extern "C"

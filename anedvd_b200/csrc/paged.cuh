@@ -235,8 +235,10 @@ struct AttnOut {
     AttnPlan plan;
 };
 int launch_attention_many(const AttnPagedCall &c, const AttnOut &o, cudaStream_t s);
-int attention_many_status(cudaStream_t s, int *timed_out);  // read and cleared
-int attention_few_status(cudaStream_t s, int *timed_out);
+// bounded waits that gave up on this device so far (waits for the stream)
+int attention_many_gave_up(cudaStream_t s, unsigned int *n);
+int attention_few_gave_up(cudaStream_t s, unsigned int *n);
+int launch_wait_probe(uint32_t limit_us, cudaStream_t s);
 
 struct MassPagedCall {
     PagedArgs a;
@@ -249,6 +251,6 @@ struct MassPagedCall {
     float decay;
 };
 int launch_attention_mass(const MassPagedCall &c, int sm_count, cudaStream_t s);
-int attention_mass_status(cudaStream_t s, int *timed_out);
+int attention_mass_gave_up(cudaStream_t s, unsigned int *n);
 
 }  // namespace cuq

@@ -11,8 +11,6 @@ using namespace ptc;
 
 namespace {
 
-__device__ int g_timeout;  // a bounded wait of this file's kernels gave up
-
 // ------------------------------------------------------------ few rows ----
 //
 // Bound by HBM: each K and V row is read once for all the rows of its group.  The
@@ -451,12 +449,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, FewGeo<HD>::CTAS)
         }
         sync();  // the others may still read this CTA's parts
     }
-    if (!ok) {  // let the copies in flight land before this block's memory is given back
-        if (lane == 0) g_timeout = 1;
-        const unsigned long long t0 = now_ns();
-        while (now_ns() - t0 < 1000000ull) {
-        }
-    }
+    if (!ok) give_up(lane == 0);
 }
 
 // --------------------------------------------------------------- merge ----
@@ -707,15 +700,27 @@ int launch_attention_paged(const AttnPagedCall &c, int sm_count, cudaStream_t s)
     return launch_all<__nv_bfloat16, __nv_bfloat16>(c, o, s);
 }
 
-int attention_few_status(cudaStream_t s, int *timed_out) {
-    CUQ_CUDA_TRY(cudaMemcpyFromSymbolAsync(timed_out, g_timeout, sizeof(int), 0, cudaMemcpyDeviceToHost, s));
-    CUQ_CUDA_TRY(cudaStreamSynchronize(s));
-    if (*timed_out) {
-        const int zero = 0;
-        CUQ_CUDA_TRY(cudaMemcpyToSymbolAsync(g_timeout, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, s));
-        CUQ_CUDA_TRY(cudaStreamSynchronize(s));
+namespace {
+// A bounded wait that nothing ends, given up and counted as the kernels' own are.
+__global__ void __launch_bounds__(32) wait_probe_kernel(unsigned long long limit_ns) {
+    __shared__ uint64_t bar;
+    __shared__ int abort_flag;
+    griddep_wait();
+    if (threadIdx.x == 0) {
+        abort_flag = 0;
+        mbar_init(&bar, 1);
+        mbar_init_fence();
     }
+    __syncthreads();
+    if (!mbar_wait_slow(&bar, 0, &abort_flag, limit_ns)) give_up(threadIdx.x == 0);
+}
+}  // namespace
+
+int launch_wait_probe(uint32_t limit_us, cudaStream_t s) {
+    CUQ_CUDA_TRY(launch_maybe_pdl(wait_probe_kernel, dim3(1), dim3(32), 0, s, true, limit_us * 1000ull));
     return CUQ_OK;
 }
+
+int attention_few_gave_up(cudaStream_t s, unsigned int *n) { return gave_up_count(s, n); }
 
 }  // namespace cuq

@@ -35,8 +35,6 @@ using namespace ptc;
 
 namespace {
 
-__device__ int g_timeout;
-
 constexpr int NT = 384;  // warps 0-3, 4-7 softmax, 8 MMA, 9 TMA, 10-11 idle
 constexpr int KEYS = 128;
 
@@ -580,12 +578,7 @@ __global__ void __launch_bounds__(NT, 1) attn_many_kernel(PagedArgs a, PagedQuer
     }
     tc_fence_before();
     __syncthreads();
-    if (abort_flag) {  // let the copies and products in flight end before the block's memory is given back
-        if (tid == 0) g_timeout = 1;
-        const unsigned long long t0 = now_ns();
-        while (now_ns() - t0 < 1000000ull) {
-        }
-    }
+    if (abort_flag) give_up(tid == 0);
     if (warp == 8) {
         tc_fence_after();
         tmem_free512(tmem);
@@ -619,15 +612,6 @@ int launch_attention_many(const AttnPagedCall &c, const AttnOut &o, cudaStream_t
                       : launch_many<__nv_bfloat16, __nv_bfloat16, 128>(c, o, s);
 }
 
-int attention_many_status(cudaStream_t s, int *timed_out) {
-    CUQ_CUDA_TRY(cudaMemcpyFromSymbolAsync(timed_out, g_timeout, sizeof(int), 0, cudaMemcpyDeviceToHost, s));
-    CUQ_CUDA_TRY(cudaStreamSynchronize(s));
-    if (*timed_out) {
-        const int zero = 0;
-        CUQ_CUDA_TRY(cudaMemcpyToSymbolAsync(g_timeout, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, s));
-        CUQ_CUDA_TRY(cudaStreamSynchronize(s));
-    }
-    return CUQ_OK;
-}
+int attention_many_gave_up(cudaStream_t s, unsigned int *n) { return gave_up_count(s, n); }
 
 }  // namespace cuq

@@ -32,8 +32,6 @@ using namespace ptc;
 
 namespace {
 
-__device__ int g_timeout;
-
 constexpr int NT = 704;  // warps 0-15 sums, 16 MMA, 17 TMA, 18-21 query tiles
 constexpr int ITEM = 256;         // slots
 constexpr int LISTED = 64;        // items of a CTA that are worked out at its start
@@ -491,12 +489,7 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
     }
     tc_fence_before();
     __syncthreads();
-    if (abort_flag) {
-        if (tid == 0) g_timeout = 1;
-        const unsigned long long t0 = now_ns();
-        while (now_ns() - t0 < 1000000ull) {
-        }
-    }
+    if (abort_flag) give_up(tid == 0);
     if (warp == 16) {
         tc_fence_after();
         tmem_free512(tmem);
@@ -582,15 +575,6 @@ int launch_attention_mass(const MassPagedCall &c, int sm_count, cudaStream_t s) 
                       : launch_mass<__nv_bfloat16, __nv_bfloat16, 128>(c, sm_count, s);
 }
 
-int attention_mass_status(cudaStream_t s, int *timed_out) {
-    CUQ_CUDA_TRY(cudaMemcpyFromSymbolAsync(timed_out, g_timeout, sizeof(int), 0, cudaMemcpyDeviceToHost, s));
-    CUQ_CUDA_TRY(cudaStreamSynchronize(s));
-    if (*timed_out) {
-        const int zero = 0;
-        CUQ_CUDA_TRY(cudaMemcpyToSymbolAsync(g_timeout, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, s));
-        CUQ_CUDA_TRY(cudaStreamSynchronize(s));
-    }
-    return CUQ_OK;
-}
+int attention_mass_gave_up(cudaStream_t s, unsigned int *n) { return gave_up_count(s, n); }
 
 }  // namespace cuq

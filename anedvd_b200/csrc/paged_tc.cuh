@@ -12,6 +12,20 @@ namespace cuq {
 
 namespace ptc {
 
+namespace {
+
+// Waits that gave up (one a warp or a block): counted, never cleared, so that any reader can
+// compare with what it saw last.  Every file of kernels has its own counter.
+__device__ unsigned int g_gave_up;
+
+int gave_up_count(cudaStream_t s, unsigned int *n) {
+    CUQ_CUDA_TRY(cudaMemcpyFromSymbolAsync(n, g_gave_up, sizeof(*n), 0, cudaMemcpyDeviceToHost, s));
+    CUQ_CUDA_TRY(cudaStreamSynchronize(s));
+    return CUQ_OK;
+}
+
+}  // namespace
+
 constexpr unsigned long long WAIT_NS = 2000000000ull;  // a wait gives up after 2 s
 constexpr uint32_t SUSPEND_NS = 20000;
 
@@ -48,14 +62,23 @@ __device__ __forceinline__ unsigned long long now_ns() {
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(v));
     return v;
 }
+// After a wait has given up: counted by one thread, and the copies and products in
+// flight end before the block's memory is given back.
+__device__ __forceinline__ void give_up(bool counts) {
+    if (counts) atomicAdd(&g_gave_up, 1u);
+    const unsigned long long t0 = now_ns();
+    while (now_ns() - t0 < 1000000ull) {
+    }
+}
 // Bounded wait for the phase with `parity`; false once this or another thread
 // of the block has given up (*abort_flag).
-__device__ __forceinline__ bool mbar_wait_slow(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
+__device__ __forceinline__ bool mbar_wait_slow(uint64_t *bar, uint32_t parity, volatile int *abort_flag,
+                                               unsigned long long limit_ns = WAIT_NS) {
     const unsigned long long t0 = now_ns();
     while (true) {
         if (mbar_try_wait(bar, parity)) return true;
         if (*abort_flag) return false;
-        if (now_ns() - t0 > WAIT_NS) break;
+        if (now_ns() - t0 > limit_ns) break;
     }
     *abort_flag = 1;
     return false;

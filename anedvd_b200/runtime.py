@@ -55,6 +55,7 @@ SIGNATURES = [
     ("cuq_attention_mass", I32, [P, P, P, SZ, P, SZ, I32, P, U32, F32, I32, U32, U32, F32, P]),
     ("cuq_kv_evict", I32, [P, P, P, SZ, U32, U32, U32, P, P, P, SZ, P]),
     ("cuq_paged_status", I32, [P]),
+    ("cuq_paged_wait_probe", I32, [U32, P]),
     ("cuq_model_create", P, [P, P]),
     ("cuq_upload_tensor", I32, [P, I32, I32, I32, P, SZ, U32, U32]),
     ("cuq_upload_f32", I32, [P, I32, I32, P, SZ]),

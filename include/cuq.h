@@ -315,10 +315,17 @@ int cuq_kv_evict(const cuq_paged_kv *kv, const cuq_batch *batch, const float *ma
                  uint32_t keep, uint32_t sink, uint32_t recent, int32_t *kept, int32_t *new_len, float *mass_out,
                  size_t mass_out_stride, void *stream);
 
-/* Waits for `stream` and reports whether a bounded wait inside one of the
- * current device's paged kernels gave up since the last such call
- * (CUQ_ETIMEOUT, then cleared). */
+/* Waits for `stream` and reports whether a bounded wait (2 s) inside any of the
+ * current device's paged kernels gave up since the last such call for this
+ * stream, or, for its first one, since the library was loaded: CUQ_ETIMEOUT, and
+ * the results since then are not to be relied on.  A caller on another stream is
+ * told of it too. */
 int cuq_paged_status(void *stream);
+
+/* Enqueues a kernel whose bounded wait runs out after limit_us (at most 10^6), so
+ * that a host can try what it does about CUQ_ETIMEOUT.  It touches no memory but
+ * the count that cuq_paged_status reads. */
+int cuq_paged_wait_probe(uint32_t limit_us, void *stream);
 
 /* ------------------------------------------------------------ engine ---- */
 

@@ -9,7 +9,7 @@ from anedvd_b200 import runtime as rt
 
 from . import paged_util as pu
 from .gpu_util import lib, ptr
-from .test_gpu_paged import PAIRS, check_attention
+from .test_gpu_paged import PAIRS, check_attention, run_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -83,3 +83,43 @@ def test_captured_mixed_steps_follow_the_batch(pair, hd):
         graph.replay()
         torch.cuda.synchronize()
         step.check()
+
+
+def test_every_stream_is_told_of_a_wait_that_gave_up():
+    """A wait that nothing ends gives up after its limit; each polled stream is told once, whoever asks first, and the
+    next calls are as before."""
+    L = lib()
+    one, two = torch.cuda.Stream().cuda_stream, torch.cuda.Stream().cuda_stream
+    for s in (one, two, None):
+        L.cuq_paged_status(s)  # whatever came before
+        assert L.cuq_paged_status(s) == rt.OK
+    rt.check(L.cuq_paged_wait_probe(1000, one))
+    assert L.cuq_paged_status(one) == rt.ETIMEOUT
+    assert "gave up" in rt.last_error()
+    assert L.cuq_paged_status(one) == rt.OK
+    assert L.cuq_paged_status(two) == rt.ETIMEOUT
+    rt.check(L.cuq_paged_wait_probe(500, two))
+    rt.check(L.cuq_paged_wait_probe(500, two))
+    assert L.cuq_paged_status(two) == rt.ETIMEOUT
+    for s in (one, None):
+        assert L.cuq_paged_status(s) == rt.ETIMEOUT
+        assert L.cuq_paged_status(s) == rt.OK
+    assert L.cuq_paged_status(two) == rt.OK
+    run_attention([(1, 70), (40, 90)], 4, 2, 64, ("f16", "f16"))
+
+
+def test_a_give_up_in_a_graph_is_told_where_it_is_replayed():
+    L = lib()
+    stream, other = torch.cuda.Stream(), torch.cuda.Stream()
+    for s in (stream.cuda_stream, other.cuda_stream, None):
+        L.cuq_paged_status(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        rt.check(L.cuq_paged_wait_probe(500, torch.cuda.current_stream().cuda_stream))
+    assert L.cuq_paged_status(other.cuda_stream) == rt.OK
+    for _ in range(2):
+        with torch.cuda.stream(other):
+            graph.replay()
+        assert L.cuq_paged_status(other.cuda_stream) == rt.ETIMEOUT
+        assert L.cuq_paged_status(other.cuda_stream) == rt.OK
+    assert L.cuq_paged_status(None) == rt.ETIMEOUT
