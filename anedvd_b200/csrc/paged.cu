@@ -3,6 +3,7 @@
 // over the cache is in paged_attn.cu, the gathered attention weight in
 // paged_mass.cu.
 #include <cmath>
+#include <limits>
 #include <map>
 #include <mutex>
 #include <new>
@@ -31,7 +32,9 @@ constexpr int ROPE_MAX_PAIRS = 64;
 
 // Angle per position of each pair, as a fraction of a turn in units of 2^-64.
 // pos * turns then wraps by itself: the product modulo 2^64 is the angle's
-// fractional turn, off by at most |pos| 2^-65 turns (2^-34 at pos = 2^31).
+// fractional turn.  The frequencies are worked out with 64-bit significands (x87's),
+// a few of whose steps, for at most 0.16 turns a position, and the rounding to 2^-64
+// are at most 2^-63: |pos| 2^-63 turns in all (2^-32 at pos = 2^31).
 struct RopeTable {
     uint64_t turns[ROPE_MAX_PAIRS];
     float mul;  // factor on cosine and sine
@@ -134,8 +137,8 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_append_kernel(RopeArgs p, R
     for (uint32_t i = threadIdx.x; i < T * half; i += ROPE_THREADS) {
         const uint32_t t = i / half, j = i % half;
         const int64_t turn = (int64_t)((uint64_t)(int64_t)s_pos[t] * tab.turns[j]);
-        // the top 32 bits are the turn in [-1/2, 1/2): 2^-32 turns is far below
-        // the fp32 step of the cosine and sine
+        // the top 32 bits are the turn in [-1/2, 1/2); as an fp32 it is off by at most
+        // 2^-26 turns (9.4e-8 radians, the fp32 rounding of any angle up to pi)
         const float x = (float)(int32_t)(turn >> 32) * 0x1p-31f;  // in units of pi
         float si, co;
         sincospif(x, &si, &co);
@@ -740,30 +743,31 @@ cuq_rope_plan *cuq_rope_plan_create(const cuq_rope_params *p) {
         return bad("YARN needs orig_ctx, 0 < beta_slow <= beta_fast and attn_factor >= 0");
     cuq_rope_plan *plan = new (std::nothrow) cuq_rope_plan();
     if (!plan) return bad("out of memory");
-    const double two_pi = 6.283185307179586476925286766559;
+    static_assert(std::numeric_limits<long double>::digits >= 64, "the table's error counts on 64-bit significands");
+    const long double two_pi = 6.283185307179586476925286766559005768L;
     const uint32_t half = p->rot_dim / 2;
     double low = 0, high = 1;
     if (p->scaling == CUQ_ROPE_YARN) {
         auto at = [&](double turns) {  // the pair index at which orig_ctx holds that many turns
-            return p->rot_dim * std::log((double)p->orig_ctx / (turns * two_pi)) / (2 * std::log((double)p->theta));
+            return p->rot_dim * std::log((double)p->orig_ctx / (turns * (double)two_pi)) / (2 * std::log((double)p->theta));
         };
         low = std::fmax(0.0, std::floor(at(p->beta_fast)));
         high = std::fmin((double)p->rot_dim - 1, std::ceil(at(p->beta_slow)));
     }
     plan->t.mul = 1.f;
     for (uint32_t j = 0; j < half; j++) {
-        double f = std::pow((double)p->theta, -2.0 * j / p->rot_dim);
+        long double f = std::pow((long double)p->theta, -2.0L * j / p->rot_dim);
         if (p->scaling == CUQ_ROPE_LINEAR) {
             f /= p->factor;
         } else if (p->scaling == CUQ_ROPE_LLAMA3) {
-            double s = ((double)p->orig_ctx * f / two_pi - p->low_freq) / ((double)p->high_freq - p->low_freq);
-            s = std::fmin(1.0, std::fmax(0.0, s));
+            long double s = (p->orig_ctx * f / two_pi - p->low_freq) / ((long double)p->high_freq - p->low_freq);
+            s = std::fmin(1.0L, std::fmax(0.0L, s));
             f = (1 - s) * f / p->factor + s * f;
         } else if (p->scaling == CUQ_ROPE_YARN) {
-            const double r = std::fmin(1.0, std::fmax(0.0, (j - low) / std::fmax(high - low, 0.001)));
+            const long double r = std::fmin(1.0L, std::fmax(0.0L, (j - low) / std::fmax(high - low, 0.001L)));
             f = f / p->factor * r + f * (1 - r);
         }
-        plan->t.turns[j] = (uint64_t)std::llrint(std::ldexp(f / two_pi, 63)) * 2;  // f <= 1: below 2^61
+        plan->t.turns[j] = (uint64_t)std::llrint(std::ldexp(f / two_pi, 64));  // f <= 1: below 2^62
     }
     for (uint32_t j = half; j < (uint32_t)ROPE_MAX_PAIRS; j++) plan->t.turns[j] = 0;
     if (p->scaling == CUQ_ROPE_YARN)

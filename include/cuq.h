@@ -239,8 +239,9 @@ typedef struct {
  *   YARN   f / factor * r + f (1 - r) with r rising linearly over the pair
  *     indices at which orig_ctx holds beta_fast (floor) to beta_slow (ceil)
  *     turns, and cosine and sine times attn_factor (0: 0.1 ln(factor) + 1).
- * Unlike cuq_rope, which follows the reference's fp32 angles, the angle here is
- * exact for every position (64-bit fixed-point turns). */
+ * Unlike cuq_rope, which follows the reference's fp32 angles, the angle here is as
+ * good at every position: off by at most |pos| 2^-63 turns (64-bit fixed point),
+ * and rounded to fp32 once its whole turns are gone. */
 #define CUQ_ROPE_NONE 0
 #define CUQ_ROPE_LINEAR 1
 #define CUQ_ROPE_LLAMA3 2

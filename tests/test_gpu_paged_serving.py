@@ -1,6 +1,8 @@
 """The paged-cache ops as a server runs them: captured steps whose batch changes, many items a CTA, and what a wait that
 gives up leaves behind.  Tolerances are those of test_gpu_paged.py unless a test derives its own."""
 import ctypes
+import math
+from decimal import Decimal, getcontext
 
 import pytest
 import torch
@@ -123,3 +125,40 @@ def test_a_give_up_in_a_graph_is_told_where_it_is_replayed():
         assert L.cuq_paged_status(other.cuda_stream) == rt.ETIMEOUT
         assert L.cuq_paged_status(other.cuda_stream) == rt.OK
     assert L.cuq_paged_status(None) == rt.ETIMEOUT
+
+
+def turns(params):
+    """Turns per position of each pair, to 50 digits."""
+    getcontext().prec = 50
+    two_pi = 2 * Decimal("3.14159265358979323846264338327950288419716939937510582097494459")
+    rot, theta = params.rot_dim, Decimal(float(params.theta))
+    f = [(-(2 * Decimal(j) / rot) * theta.ln()).exp() for j in range(rot // 2)]
+    if params.scaling == rt.ROPE_LINEAR:
+        f = [x / Decimal(float(params.factor)) for x in f]
+    return [x / two_pi for x in f]
+
+
+@pytest.mark.parametrize("theta", [1e4, 1e6])
+@pytest.mark.parametrize("scaling", [rt.ROPE_NONE, rt.ROPE_LINEAR])
+def test_angles_hold_at_the_farthest_positions(scaling, theta):
+    """cos and sin themselves (pairs (1, 0)) at positions up to 2^31.  The angle is off by 2^-32 turns from the table and
+    pi 2^-25 from its rounding to fp32, the functions by 2 steps of a value below one, 2^-23 in all."""
+    hd, n = 128, 96
+    params = rt.CuqRopeParams(rot_dim=hd, theta=theta, scaling=scaling, factor=3.0)
+    plan = rt.RopePlan(params)
+    b = pu.Batch([(n, n)], 1, hd, "f16", 16)
+    pos = [(-1) ** i * ((1 << 31) - 1 - 12345677 * i) for i in range(n)]
+    x = torch.zeros(n, 3, hd, device="cuda")
+    x[:, 0, : hd // 2] = 1.0
+    q = torch.empty(n, hd, device="cuda")
+    at = torch.tensor(pos, dtype=torch.int32, device="cuda")
+    rt.check(lib().cuq_rope_append(plan.handle, b.kvp, b.bp, ptr(at), ptr(q), hd, 0, ptr(x), 3 * hd,
+                                   ctypes.c_void_p(x.data_ptr() + 4 * hd), ctypes.c_void_p(x.data_ptr() + 8 * hd), 3 * hd,
+                                   0, 1, None))
+    got = q.double().cpu()
+    tol = 2 * math.pi * 2.0 ** -32 + math.pi * 2.0 ** -25 + 2.0 ** -23
+    for j, t in enumerate(turns(params)):
+        angle = [2 * math.pi * float(p * t % 1) for p in pos]
+        for k, f in ((j, math.cos), (j + hd // 2, math.sin)):
+            want = torch.tensor([f(a) for a in angle], dtype=torch.float64)
+            assert float((got[:, k] - want).abs().max()) <= tol, (j, k)
