@@ -11,7 +11,7 @@ from anedvd_b200 import runtime as rt
 
 from . import paged_util as pu
 from .gpu_util import lib, ptr
-from .test_gpu_paged import PAIRS, check_attention, run_attention
+from .test_gpu_paged import PAIRS, attend, check_attention, run_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -162,3 +162,124 @@ def test_angles_hold_at_the_farthest_positions(scaling, theta):
         for k, f in ((j, math.cos), (j + hd // 2, math.sin)):
             want = torch.tensor([f(a) for a in angle], dtype=torch.float64)
             assert float((got[:, k] - want).abs().max()) <= tol, (j, k)
+
+
+def wide_table(b, slots):
+    """The same caches under a bound of `slots` slots, which asks for runs and the merge."""
+    wide = torch.full((len(b.seqs), slots // b.page), -1, dtype=torch.int32)
+    wide[:, : b.table.shape[1]] = b.table
+    b.d_wide = wide.cuda()
+    b.desc.pages, b.desc.pages_stride, b.desc.max_kv = b.d_wide.data_ptr(), slots // b.page, slots
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("seqs,form", [
+    ([(1, 300), (1, 900), (1, 77)], "cluster"), ([(1, 300), (1, 900), (3, 2000)], "runs"), ([(100, 500)], "whole"),
+    ([(40, 1500)], "split"), ([(1, 700), (100, 500), (2, 300)], "mixed")])
+def test_fp32_queries_keep_what_fp32_holds(seqs, form, hd):
+    """Against 64 bits, relative to sum p |v| / sum p = mag, each row at its own length.  Values are 1 + noise, so that what
+    an accumulator cuts off adds up.  Counted, with T = scale sum |q k| (below 2.5 here) and a cut of at most 2^-22 of the
+    sum at each of the matrix instructions behind one another (two a step, one of them in the other half's place):
+      scores: hd / 16 steps and two roundings more, (hd / 16 + 2) 2^-22 T, twice (numerator and sum);
+      probabilities: the exponent's rounding below 16, 2^-21, the exponential 2^-22 and the split 2^-22: below 2^-20;
+      products with V: 16 instructions a tile of 128 slots, up to 40 in a warp's run: 40 * 2^-22;
+      sums of up to 64 probabilities a thread, and the parts' weights: 2^-18.
+    The mean square counts cuts as half a step on average, growing with the sum (a quarter of the bound: 10 * 2^-22 = 2.4e-6
+    at most, 16 instructions 1e-6), and the rest as independent over the slots.  Probabilities rounded to fp16
+    without their low parts, worked out for these inputs, give 1.3e-5 at 300 slots and 8.5e-6 at 900 (root mean square)."""
+    b = pu.Batch(seqs, 2, hd, "f16", 16, seed=31)
+    for host, dev in ((b.k_host, b.k), (b.v_host, b.v)):
+        if host is b.v_host:
+            host.mul_(0.5).add_(1.0)
+        dev.copy_(host)
+    if form == "runs":
+        wide_table(b, 16384)
+    heads, scale = 8, 1.0 / 64
+    g = torch.Generator().manual_seed(32)
+    q = torch.randn(b.n_tok, heads, hd, generator=g)
+    need = lib().cuq_attention_paged_workspace(b.kvp, b.bp, heads, 0)
+    assert (need == 0) == (form in ("cluster", "whole"))
+    out, lse = attend(b, heads, "f32", q.cuda().view(b.n_tok, -1), heads * hd, scale)
+    want, wl, mag, top = b.attention(q, scale)
+    assert float(top.max()) < 2.5
+    off = (out.view(b.n_tok, heads, hd).double().cpu() - want).abs() / mag
+    tol = 2 * top[..., None] * (hd / 16 + 2) * 2.0 ** -22 + 2.0 ** -20 + 40 * 2.0 ** -22 + 2.0 ** -18
+    assert float((off - tol).max()) <= 0, float((off / tol).max())
+    for i, (a, n) in enumerate(seqs):
+        t = b.starts[i]
+        if 300 <= n <= 900:
+            assert float(off[t:t + a].square().mean().sqrt()) <= 2.4e-6
+    assert float((lse.double().cpu() - wl).abs().max()) <= 2.5 * (hd / 16 + 2) * 2.0 ** -22 + 2.0 ** -18 + 2.0 ** -20
+
+
+@pytest.mark.parametrize("pair", PAIRS)
+@pytest.mark.parametrize("long", [False, True])
+def test_mass_of_more_items_than_a_block_lists(pair, long):
+    """More than 64 items of 256 slots for every block of the GPU: neighbouring ones where the queries are few, dealt out
+    where some sequence has more than 128 rows; ragged lengths, empty caches, sequences without tokens.  All caches share
+    a few pages, which this operator only reads."""
+    t, cache = pair
+    heads, kvh, hd, page, n_seqs = 4, 2, 64, 256, 640
+    g = torch.Generator().manual_seed(51)
+    lens = torch.randint(1500, 3001, (n_seqs,), generator=g).tolist()
+    toks = torch.randint(1, 4, (n_seqs,), generator=g).tolist()
+    for i in range(0, n_seqs, 37):
+        toks[i] = 90 if long else 0
+    for i in range(5, n_seqs, 41):
+        lens[i] = 0
+    for i in range(7, n_seqs, 43):
+        toks[i] = 0
+    lens = [max(n, a) if n else 0 for n, a in zip(lens, toks)]
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    assert sum(-(-n // 256) for n in lens) * kvh > 64 * sms
+    n_pages, cols = 40, 13
+    table = torch.randint(0, n_pages, (n_seqs, cols), generator=g).int()
+    table[::53, 3] = -1  # holes
+    starts = [0]
+    for a in toks:
+        starts.append(starts[-1] + a)
+    n_tok, max_kv, max_q = starts[-1], max(lens), max(toks)
+    assert (max_q * 2 > 128) == long
+    k = torch.randn(n_pages, kvh, page, hd, generator=g).to(pu.DT[cache]).cuda()
+    q = (1.5 * torch.randn(n_tok, heads, hd, generator=g)).to(pu.DT[t]).cuda()
+    dev = [torch.tensor(x, dtype=torch.int32, device="cuda") for x in (starts, lens)] + [table.cuda()]
+    kv = rt.CuqPagedKv(k=k.data_ptr(), v=k.data_ptr(), type=pu.GGML[cache], n_pages=n_pages, page_size=page, kv_heads=kvh,
+                       head_dim=hd, page_stride=0)
+    batch = rt.CuqBatch(q_start=dev[0].data_ptr(), kv_len=dev[1].data_ptr(), pages=dev[2].data_ptr(), n_seqs=n_seqs,
+                        n_tok=n_tok, pages_stride=cols, max_q=max_q, max_kv=max_kv)
+    # the definition in 64 bits; terms and their error weights as in paged_util.Batch.mass
+    scale = hd ** -0.5
+    lse = torch.zeros(n_tok, heads, dtype=torch.float64, device="cuda")
+    parts = []
+    for i, (a, n) in enumerate(zip(toks, lens)):
+        if not a or not n:
+            parts.append(None)
+            continue
+        slot = torch.arange(n, device="cuda")
+        ids = dev[2][i].long()[slot // page]
+        rows = k[ids.clamp(min=0), :, slot % page].double()                           # [n][kvh][hd]
+        qq = q[starts[i]:starts[i + 1]].double().view(a, kvh, heads // kvh, hd)
+        x = torch.einsum("akgd,nkd->kgan", qq, rows) * scale
+        ok = (ids >= 0) & (slot <= torch.arange(n - a, n, device="cuda")[:, None])
+        x = x.masked_fill(~ok, -math.inf)
+        far = torch.einsum("akgd,nkd->kgan", qq.abs(), rows.abs()) * scale
+        lse[starts[i]:starts[i + 1]] = torch.logsumexp(x, 3).permute(2, 0, 1).reshape(a, heads)
+        parts.append((x, far))
+    ls = lse.float()
+    mass = torch.rand(n_seqs, kvh, max_kv, generator=g).cuda()
+    before = mass.double()
+    rt.check(lib().cuq_attention_mass(ctypes.byref(kv), ctypes.byref(batch), ptr(mass), max_kv, ptr(q), heads * hd,
+                                      pu.GGML[t], ptr(ls), heads, scale, 1, 0, 0, 0.5, None))
+    rt.check(lib().cuq_paged_status(None))
+    got = mass.double()
+    for i, (a, n) in enumerate(zip(toks, lens)):
+        assert torch.equal(got[i, :, n:], before[i, :, n:])
+        add = err = torch.zeros(kvh, n, dtype=torch.float64, device="cuda")
+        if parts[i]:
+            x, far = parts[i]
+            ll = ls[starts[i]:starts[i + 1]].double().view(a, kvh, heads // kvh).permute(1, 2, 0)[..., None]
+            p = torch.exp(x - ll)
+            add, err = p.sum((1, 2)), (p * (far + ll.abs())).sum((1, 2))
+        want = 0.5 * before[i, :, :n] + add
+        tol = 2.0 ** -17 * err + 2.0 ** -18 * want + 1e-30
+        assert ((got[i, :, :n] - want).abs() <= tol).all(), i
