@@ -70,7 +70,6 @@ struct RopeArgs {
     uint32_t heads;
 };
 
-template <typename T>
 __device__ __forceinline__ void store_as(int type, void *base, size_t at, const float (&v)[8]) {
     if (type == CUQ_F32)
         store8(reinterpret_cast<float *>(base) + at, v);
@@ -214,8 +213,8 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_append_kernel(RopeArgs p, R
                 v[3] = x * c.w + y * c.y;
             }
         }
-        store_as<TI>(type, to, at + e0, a);
-        store_as<TI>(type, to, at + e1, b);
+        store_as(type, to, at + e0, a);
+        store_as(type, to, at + e1, b);
     }
 }
 

@@ -168,13 +168,6 @@ __device__ __forceinline__ void unpack8(const uint4 (&u)[sizeof(T) == 4 ? 2 : 1]
     }
 }
 template <typename T>
-__device__ __forceinline__ void load8(const T *p, float (&v)[8]) {
-    uint4 u[sizeof(T) == 4 ? 2 : 1];
-#pragma unroll
-    for (int w = 0; w < (sizeof(T) == 4 ? 2 : 1); w++) u[w] = reinterpret_cast<const uint4 *>(p)[w];
-    unpack8<T>(u, v);
-}
-template <typename T>
 __device__ __forceinline__ void store8(T *p, const float (&v)[8]) {
     *reinterpret_cast<uint4 *>(p) = make_uint4(Pair<T>::pack(v[0], v[1]), Pair<T>::pack(v[2], v[3]),
                                                Pair<T>::pack(v[4], v[5]), Pair<T>::pack(v[6], v[7]));

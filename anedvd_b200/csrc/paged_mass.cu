@@ -495,27 +495,19 @@ __global__ void __launch_bounds__(NT, 1) mass_kernel(MassArgs p, const __grid_co
         tmem_free512(tmem);
     }
     if (ranks > 1) {  // one item per cluster: rank 0 joins the sums in rank order
-        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        cluster_sync();
         if (rank == 0 && tid < ITEM && x0 < x1) {
             Item t;
             item(x0, t);
             const uint32_t k = t.k0 + tid;
             float sum = 0.f;
-            for (uint32_t r = 0; r < ranks; r++) {
-                uint32_t at;
-                float v;
-                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(&s_red[1][tid])), "r"(r));
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
-                sum += v;
-            }
+            for (uint32_t r = 0; r < ranks; r++) sum += peer_load(peer_smem(&s_red[1][tid], r));
             if (k < t.n) {
                 float *m = p.mass + ((size_t)t.b * a.kv_heads + t.h) * p.mass_stride + k;
                 *m = p.decay == 0.f ? sum : p.decay * *m + sum;
             }
         }
-        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        cluster_sync();
     }
 }
 

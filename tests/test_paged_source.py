@@ -49,3 +49,16 @@ def test_kernels_wait_before_they_read(name):
         reads = re.findall(r"\.(?:len|tokens|page|sequence_of|range)\(|\bFewSeq\b|\*\s*reinterpret_cast<const|"
                            r"\b(?:q_start|kv_len|pages|positions|kept|mass|lse)\s*\[|\[\s*j\s*\]", head)
         assert not reads, (kernel, reads)
+
+
+def test_no_function_is_left_that_nothing_calls():
+    text = {f: source(f) for f in FILES}
+    whole = "\n".join(text.values())
+    names = {m[1] for f in ("paged.cuh", "paged_tc.cuh")
+             for m in re.finditer(r"__device__ (?:__forceinline__ )?[\w:<> ]+?[\s*&](\w+)\((?!\()", text[f])}
+    names |= {m[1] for f in ("paged.cuh", "paged_tc.cuh") for m in re.finditer(r"^(?:int|size_t|AttnPlan|constexpr uint32_t) (\w+)\(",
+                                                                            text[f], re.M)}
+    assert {"mbar_wait", "tmem_ld32", "peer_smem", "tokens", "launch_attention_many"} <= names
+    unused = {n for n in names if len(re.findall(r"\b%s\b(?=\s*(?:<[\w:, ]+>)?\s*\()" % n, whole)) <
+              1 + len(re.findall(r"(?:__forceinline__ [\w:<> ]+?[\s*&]|^(?:int|size_t|AttnPlan) )%s\(" % n, whole, re.M))}
+    assert not unused
