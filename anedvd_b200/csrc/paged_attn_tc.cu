@@ -17,6 +17,10 @@
 // tensor cores cut off what falls below the accumulator's last place, always towards
 // zero: over a long context that is 2e-6 of an fp32 output.  So with fp32 queries O is
 // of one tile only and the softmax threads sum the tiles in registers (4e-7).
+// 16-bit queries have one 16-bit P; the row's sum takes it unrounded.  Two operands as
+// for fp32 queries would add half of the products again.  Sums of the rounded
+// probabilities beside the unrounded ones, which lse needs, took a prompt of 4096 tokens
+// from 151 to 158 us for an error of 2.74e-5 instead of 2.79e-5 (root mean square).
 // What bounds it: per 128 x 128 tile the two products take 1024 cycles of the
 // tensor pipe at head_dim 128 (512 at 64) and the exponentials 1024 of the MUFU; but
 // Q K^T reads both operands from shared memory, 8 KB a product of 64 cycles, and runs

@@ -283,3 +283,27 @@ def test_mass_of_more_items_than_a_block_lists(pair, long):
         want = 0.5 * before[i, :, :n] + add
         tol = 2.0 ** -17 * err + 2.0 ** -18 * want + 1e-30
         assert ((got[i, :, :n] - want).abs() <= tol).all(), i
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("form", ["cluster", "runs"])
+def test_few_rows_round_the_output_alone(form, t, hd):
+    """Decode steps in 16 bits: half a step of the output, and beside it what fp32 queries are allowed above, with
+    probabilities of two 16-bit operands (u^2 of themselves, 2^-16 in bf16, in the products alone).  One rounded operand is
+    off by up to u of each probability, and outputs near zero show it."""
+    seqs = [(1, 300), (1, 900), (2, 150)]
+    b = pu.Batch(seqs, 2, hd, t, 16, seed=61)
+    if form == "runs":
+        wide_table(b, 16384)
+    heads, scale = 8, 1.0 / 64
+    q = torch.randn(b.n_tok, heads, hd, generator=torch.Generator().manual_seed(62)).to(pu.DT[t])
+    need = lib().cuq_attention_paged_workspace(b.kvp, b.bp, heads, pu.GGML[t])
+    assert (need == 0) == (form == "cluster")
+    out, _ = attend(b, heads, t, q.cuda().view(b.n_tok, -1), heads * hd, scale)
+    want, _, mag, top = b.attention(q, scale)
+    off = (out.view(b.n_tok, heads, hd).double().cpu() - want).abs()
+    u = pu.unit(t)
+    tol = mag * (2 * top[..., None] * (hd / 16 + 2) * 2.0 ** -22 + 2.0 ** -20 + 40 * 2.0 ** -22 + 2.0 ** -18 + u * u)
+    tol = tol + 1.01 * u * want.abs() + 2.0 ** -25
+    assert float((off - tol).max()) <= 0, float((off / tol).max())
