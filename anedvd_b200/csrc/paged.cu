@@ -58,8 +58,8 @@ namespace {
 // one each, into shared memory, and then walk the rows (token, head) in units:
 // the 16 values that hold 8 whole pairs, two 16-byte vectors at j and j + rot/2,
 // or 16 values in a row.  4096 tokens (32 heads, 8 KV heads, head_dim 128, fp16, 101 MB)
-// take 21.3 us, 4.7 TB/s, 73 % of a copy's rate; more loads in flight a thread cost
-// occupancy and made it slower (31 us).
+// take 21.2 us, 4.75 TB/s, 74 % of a copy's rate (from fp32 34.8 us, 5.3 TB/s); more loads
+// in flight a thread cost occupancy and made it slower (31 us).
 struct RopeArgs {
     PagedArgs a;
     const int32_t *positions;
@@ -221,8 +221,10 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_append_kernel(RopeArgs p, R
 template <typename TI>
 int launch_rope_append(const RopeArgs &p, const RopeTable &t, int out_type, int cache_type, uint32_t hd,
                        cudaStream_t s) {
-    // two tokens a CTA once there are CTAs enough: 4096 tokens took 24.6 us, with one
-    // each 28.6 and with four 26.7; 16 tokens 9.3 us with one, 9.4 with two
+    // two tokens a CTA once there are CTAs enough.  16, 512, 1024, 2048, 4096 and 8192
+    // tokens (32 heads, 8 KV heads, head_dim 128, fp16, in a graph) take 3.4, 4.3, 7.3, 14.0,
+    // 24.5 and 44.5 us with one each, 4.4, 4.9, 6.8, 14.1, 21.3 and 35.1 with two; four each
+    // made 4096 tokens 2 us slower
     const bool many = p.a.n_tok >= 1024;
     const uint32_t grid = many ? (p.a.n_tok + 1) / 2 : p.a.n_tok;
     auto launch = [&](auto kernel) {
@@ -235,12 +237,12 @@ int launch_rope_append(const RopeArgs &p, const RopeTable &t, int out_type, int 
 
 // ------------------------------------------------------- eviction ----
 //
-// Selection, bound by latency: a cluster of CTAs takes one (sequence, KV head),
+// Radix selection, bound by latency: a cluster of CTAs takes one (sequence, KV head),
 // each a contiguous slice of its slots.  Masses become 32-bit keys in their order
 // (NaN lowest), eight a thread, kept in registers where the slice fits.
 // Up to three histogram passes (11, 11, 10 bits) find the key of the last slot kept and
-// how many of its equals are kept, and end at a bin that is kept whole: every CTA counts its own slice, adds the bins it hit
-// into every CTA's sums through distributed shared memory, and works the digit out
+// how many of its equals are kept, and end at a bin that is kept whole: every CTA
+// counts its own slice, adds the bins it hit into every CTA's sums through distributed shared memory, and works the digit out
 // for itself.  Then the slices' counts are exchanged and the kept slots written at
 // their prefix sums.  Histogram atomics count whole numbers, so their order does not
 // matter.  At most five cluster barriers; with rank 0 finding the digits it was ten.

@@ -25,13 +25,14 @@ namespace {
 // in the 128-byte swizzle, which ldmatrix reads without bank conflicts.  Scores and
 // outputs run on mma.sync.m16n8k16 (16 rows x 16 slots, fp32 accumulate); fp32
 // queries are two fp16 operands, hi and lo, and so are the probabilities of every type:
-// the products behind the cache's bytes are nearly free (32 requests 39.3 -> 39.6 us),
-// and what is left of the error is the output's own rounding (3.5e-4 root mean square,
-// with one rounded operand 4.0e-4).
+// the second operand costs 0 to 5 % (32 requests 39.3 -> 39.6 us, 16 of 600 slots
+// 11.8 -> 12.3), and what is left of the error is the output's own rounding (3.5e-4 root
+// mean square, with one rounded operand 4.0e-4).
 // A decode step of 32 requests up to 8192 slots (32 heads, 8 KV heads, head_dim 128,
-// bf16, 186 MB) takes 39 us with the merge, 4.8 TB/s, 74 % of a copy's rate; the walk
+// bf16, 186 MB) takes 39.6 us with the merge, 4.7 TB/s, 73 % of a copy's rate; the walk
 // itself runs at the rate of HBM, and the rest is the start (three dependent loads
-// before the first copy) and the merge.  Two blocks in flight a warp: with three the
+// before the first copy) and the merge.  Larger batches come nearer: 128 requests up to
+// 4096 slots 82 us, 5.6 TB/s.  fp32 queries over fp16 take 41.6 us.  Two blocks in flight a warp: with three the
 // step took 42.4 us and with four 48.6, since queries and page ids then wait behind
 // 28 MB of copies.  With a CTA for each part of 256 to 1024 slots instead of equal runs
 // it took 51 to 67 us.
@@ -457,8 +458,9 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, FewGeo<HD>::CTAS)
 //
 // out = sum_s w_s o_s / sum_s w_s, w_s = 2^(lse2_s - max), over the parts that a
 // row's kernel wrote.  A warp per (token, head): lanes hold HD / 32 dims.  Bound by the
-// latency of three dependent loads; reading one part after the other it took 16 us for
-// 26 parts, with eight on their way 8.7.
+// latency of its dependent loads (sequence, lengths and units, sums, outputs): 9.8 us
+// alone under a profiler for the 26 parts an item of a decode step of 32 requests, of
+// which 5 show behind the walk.  Reading one part after the other it took twice as long.
 constexpr int MERGE_WARPS = 4;
 
 template <typename TQ, int HD>
@@ -643,9 +645,9 @@ AttnPlan attention_paged_plan(const AttnPagedCall &c, int sm_count) {
         if (!p.many && items <= most) {
             // As few blocks a warp as 8 CTAs an item, all of the call's at once on the GPU, come
             // to, in as few CTAs; up to FEW_NEAR.  One token over 40, 600, 2000, 4000 and 8000
-            // slots (9 heads, 3 KV heads, head_dim 64, fp32, in a graph) takes 4.1, 6.6, 8.6, 12.1
-            // and 19.1 us this way, 7.9, 8.6, 10.0, 13.2 and 16.5 with runs and the merge; 16
-            // over 600 (32 heads, 8 KV heads, head_dim 128, bf16) 9.9 instead of 12.3.
+            // slots (9 heads, 3 KV heads, head_dim 64, fp32, in a graph) takes 4.3, 6.6, 8.6, 12.1
+            // and 19.1 us this way, 8.7, 9.5, 10.7, 13.5 and 16.2 with runs and the merge; 16
+            // over 600 (32 heads, 8 KV heads, head_dim 128, bf16) 12.2 instead of 15.7.
             uint64_t seen = c.a.max_kv;
             if (c.q.window && c.q.window + (uint64_t)c.a.max_q < seen) seen = c.q.window + (uint64_t)c.a.max_q;
             const uint64_t longest = seen / FEW_KEYS + 1, warps = (most / items < 8 ? most / items : 8) * FEW_WARPS;
@@ -656,6 +658,14 @@ AttnPlan attention_paged_plan(const AttnPagedCall &c, int sm_count) {
     if (p.many) {
         p.many_tiles = (uint32_t)((c.a.n_tok * g + 255) / 256 + c.a.n_seqs);
         const uint64_t base = ((c.a.n_tok * g + 255) / 256) * c.a.kv_heads;
+        // as many parts of the slots as leave all CTAs on the GPU at once (one an SM), of 512
+        // slots at least.  With one part, this many and twice as many (12 heads, 2 KV heads,
+        // head_dim 128, bf16, in a graph): 64 tokens over 2048 slots 34, 19 and 19 us, over
+        // 32768 410, 33 and 48; 512 over 8192 109, 36 and 49, over 32768 414, 87 and 98; 1024
+        // over 32768 413, 161 and 168.  Where half a wave or more is there without parts a
+        // second wave may pay (2048 over 32768 425 and 314 us) or not (over 2048 35 and 51);
+        // the window is left out of account, and its empty parts cost little: 64 tokens with a
+        // window of 128 over 32768 slots take 23 us.
         uint64_t want = base ? sms / base : 1, most = ((uint64_t)c.a.max_kv + 511) / 512;
         if (want > most) want = most;
         if (want > 64) want = 64;

@@ -284,10 +284,10 @@ int cuq_rope_append(const cuq_rope_plan *rope, const cuq_paged_kv *kv, const cuq
  * it.  Scores, sums and outputs are held in fp32; where a sequence has more than 16
  * (token, head) rows a KV head, each probability over a 16-bit type is rounded to it
  * once before it multiplies V (its row's sum takes it unrounded).  fp32 queries lie
- * within fp16's range.  out overlaps no other array.  lse [n_tok][heads] (may be NULL): the natural log of the sum of
- * exponentials.  workspace: cuq_attention_paged_workspace bytes, 256-byte
- * aligned (may be NULL when that is 0); two calls that may run at the same
- * time need one each. */
+ * within fp16's range.  out overlaps no other array.  lse [n_tok][heads] (may be
+ * NULL): the natural log of the sum of exponentials.  workspace:
+ * cuq_attention_paged_workspace bytes, 256-byte aligned (may be NULL when that is
+ * 0); two calls that may run at the same time need one each. */
 size_t cuq_attention_paged_workspace(const cuq_paged_kv *kv, const cuq_batch *batch, uint32_t heads, int type);
 int cuq_attention_paged(const cuq_paged_kv *kv, const cuq_batch *batch, void *out, size_t out_stride, const void *q,
                         size_t q_stride, int type, float *lse, uint32_t heads, float scale, int causal,
@@ -309,7 +309,9 @@ int cuq_attention_mass(const cuq_paged_kv *kv, const cuq_batch *batch, float *ma
  * the lowest slot; NaN counts as the smallest), `keep` in all (sink + recent <=
  * keep), in their order, moved to slots [0, n), n = min(kv_len, keep).  The
  * rows move in place inside the sequence's own pages; rows on a hole are not
- * moved and rows are not moved onto one.  kept [n_seqs][kv_heads][keep] gets the old slot of each new one
+ * moved and rows are not moved onto one, so that their new slots keep what they
+ * held (a cache whose pages were given back is not one to evict from).
+ * kept [n_seqs][kv_heads][keep] gets the old slot of each new one
  * (-1 behind the last), new_len [n_seqs] the new length (not the array of
  * kv_len).  mass_out (NULL: none; mass itself: in place; otherwise no overlap)
  * gets the kept slots' mass at [0, n) and 0 at [n, kv_len).  Keys keep the
