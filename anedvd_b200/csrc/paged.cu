@@ -242,8 +242,8 @@ int launch_rope_append(const RopeArgs &p, const RopeTable &t, int out_type, int 
 // (NaN lowest), eight a thread, kept in registers where the slice fits.
 // Up to three histogram passes (11, 11, 10 bits) find the key of the last slot kept and
 // how many of its equals are kept, and end at a bin that is kept whole: every CTA
-// counts its own slice, adds the bins it hit into every CTA's sums through distributed shared memory, and works the digit out
-// for itself.  Then the slices' counts are exchanged and the kept slots written at
+// counts its own slice, adds the bins it hit into every CTA's sums through distributed
+// shared memory, and works the digit out for itself.  Then the slices' counts are exchanged and the kept slots written at
 // their prefix sums.  Histogram atomics count whole numbers, so their order does not
 // matter.  At most five cluster barriers; with rank 0 finding the digits it was ten.
 // 4096 slots take one CTA about 8.5 us, 32768 a cluster of eight 12 us, mostly barriers

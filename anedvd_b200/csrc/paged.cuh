@@ -17,10 +17,10 @@ namespace cuq {
 // grid has waited is not enough for a later one that it let start: only its own wait
 // makes what was written before visible to it.  (Reading the batch before the wait
 // gained 0.5 us in the merge and 0.3 in the eviction's move, and starting the few-row
-// kernel beside the many-row one 8 us of 31 in a mixed batch.)  A kernel may thus be resident
-// while its inputs are still written (the selection's list and the move that reads it),
-// so all of them are read by plain loads: the read-only path (ld.global.nc) asks for
-// data that does not change while the kernel lives.
+// kernel beside the many-row one 8 us of 31 in a mixed batch.)  A kernel may thus be
+// resident while its inputs are still written (the selection's list and the move that
+// reads it), so all of them are read by plain loads: the read-only path (ld.global.nc)
+// asks for data that does not change while the kernel lives.
 
 // SM count of the current device, asked for once per device.
 int paged_sm_count();

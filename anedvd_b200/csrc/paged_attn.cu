@@ -32,9 +32,9 @@ namespace {
 // bf16, 186 MB) takes 39.6 us with the merge, 4.7 TB/s, 73 % of a copy's rate; the walk
 // itself runs at the rate of HBM, and the rest is the start (three dependent loads
 // before the first copy) and the merge.  Larger batches come nearer: 128 requests up to
-// 4096 slots 82 us, 5.6 TB/s.  fp32 queries over fp16 take 41.6 us.  Two blocks in flight a warp: with three the
-// step took 42.4 us and with four 48.6, since queries and page ids then wait behind
-// 28 MB of copies.  With a CTA for each part of 256 to 1024 slots instead of equal runs
+// 4096 slots 82 us, 5.6 TB/s.  fp32 queries over fp16 take 41.6 us.  Two blocks in
+// flight a warp: with three the step took 42.4 us and with four 48.6, since queries and
+// page ids then wait behind 28 MB of copies.  With a CTA for each part of 256 to 1024 slots instead of equal runs
 // it took 51 to 67 us.
 // Where all items are short, a cluster of CTAs takes each instead and joins its parts
 // through distributed shared memory: one launch, no workspace (attention_paged_plan has

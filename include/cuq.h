@@ -281,10 +281,10 @@ int cuq_rope_append(const cuq_rope_plan *rope, const cuq_paged_kv *kv, const cuq
  * of those the last `window`.  A token that sees nothing gets out 0 and lse
  * -inf.  Slots at or past kv_len and slots on a hole may hold anything; a NaN or
  * infinity in a V row before kv_len can reach tokens of its tile that do not see
- * it.  Scores, sums and outputs are held in fp32; where a sequence has more than 16
- * (token, head) rows a KV head, each probability over a 16-bit type is rounded to it
- * once before it multiplies V (its row's sum takes it unrounded).  fp32 queries lie
- * within fp16's range.  out overlaps no other array.  lse [n_tok][heads] (may be
+ * it.  Scores, sums and outputs are held in fp32.  Where a sequence has more than 16
+ * (token, head) rows a KV head (or, alone in its batch, may have by max_q), each
+ * probability of 16-bit queries is rounded to their type once before it multiplies
+ * V, and its row's sum takes it unrounded.  fp32 queries lie within fp16's range.  out overlaps no other array.  lse [n_tok][heads] (may be
  * NULL): the natural log of the sum of exponentials.  workspace:
  * cuq_attention_paged_workspace bytes, 256-byte aligned (may be NULL when that is
  * 0); two calls that may run at the same time need one each. */
